@@ -23,6 +23,10 @@ FA_DEVERR_SEQLEN = 0x10
 FA_DEVERR_PAIR = 0x20
 FA_DEVERR_POSITION = 0x40
 FA_DEVERR_LAUNCH = 0x80
+FA_DEVERR_VALUE = 0x100
+FA_DEVERR_TOKEN = 0x200
+FA_KV8_E4M3, FA_KV8_I8 = 16, 17
+FA_MAX_TOP_LOGPROBS = 32
 FA_MAX_COPY_LAYERS = 128
 FA_NOALLOC_DECODE_SCRATCH_BYTES = 8 * 1024 * 1024
 
@@ -45,6 +49,25 @@ class FaKvLayer(ctypes.Structure):
 
 
 _LP = ctypes.POINTER(FaKvLayer)
+
+
+class FaKv8Layer(ctypes.Structure):
+    """``fa_kv8_layer``: one layer of an 8-bit pool, byte slabs and f32 scales per (block, head)."""
+
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+_L8 = ctypes.POINTER(FaKv8Layer)
 
 
 class FaQkvWeights(ctypes.Structure):
@@ -118,6 +141,15 @@ SIGNATURES = {
     "fa_qkv_rope_cache": (_I32, [_LP, _WP, _P, _P, _P, _I32, _P, _P]),
     "fa_o_proj_residual": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
     "fa_last_token_logits": (_I32, [_P, _P, _I32, _I32, _P, _F, _P, _I32, _I32, _I32, _P, _P, _P]),
+    "fa_paged_append_kv8": (_I32, [_L8, _P, _P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32,
+                                   _I32, _P]),
+    "fa_paged_decode_kv8_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "fa_paged_decode_kv8": (_I32, [_L8, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, _P,
+                                   _SZ, _P]),
+    "fa_paged_prefill_kv8_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "fa_paged_prefill_kv8": (_I32, [_L8, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32,
+                                    _I32, _I32, _F, _P, _SZ, _P]),
+    "fa_token_logprobs": (_I32, [_P, _I32, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P]),
     "fa_ipc_alloc": (_I32, [_SZ, ctypes.POINTER(_P), _HP]),
     "fa_ipc_free": (_I32, [_P]),
     "fa_ipc_open": (_I32, [_HP, ctypes.POINTER(_P)]),

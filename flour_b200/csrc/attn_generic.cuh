@@ -7,10 +7,12 @@
 // src/models/common/cache.rs:83-96) and folded with the same online softmax, in f32, with
 // accurate expf, so f32 pools match the reference to ~1e-6. The bf16/f16 fast paths live in
 // decode_sm100.cuh / prefill_sm100.cuh; this kernel serves f32 pools and shapes those do not
-// cover (e.g. the reference's unit-test shapes: head_dim 4, block sizes 2-4).
+// cover (e.g. the reference's unit-test shapes: head_dim 4, block sizes 2-4). With an 8-bit pool
+// (format F) it serves the shapes that kv8_decode_sm100.cuh does not: a block's K scale multiplies
+// its scores, its V scale its probabilities.
 #pragma once
 
-#include "fa_common.cuh"
+#include "kv8_common.cuh"
 
 namespace fa {
 
@@ -33,6 +35,8 @@ struct GenericParams {
   int32_t total_q;
   float scale;
   int32_t ref_scores;  // 1: the reference's dtype rounding of the scores (ref_score)
+  const float *k_scale;  // 8-bit pools: [num_blocks, num_kv_heads]
+  const float *v_scale;
 };
 
 constexpr int kGenericWarps = 16;
@@ -52,8 +56,14 @@ __host__ __device__ constexpr size_t generic_smem_floats(int block_size) {
 // acc = acc * corr + sum_j p_j v_j), lanes over the block's rows for the scores and over
 // head_dim for the accumulation; the 16 partial states are merged at the end. Only blocks up to
 // the last visible position are folded, so every folded block holds at least one visible key.
-template <typename T>
+template <typename T, class F = void>
 __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const GenericParams p) {
+  constexpr bool k8 = !std::is_void<F>::value;
+  using C = typename std::conditional<k8, uint8_t, T>::type;  // cache element
+  auto elem = [](C x) -> float {
+    if constexpr (k8) return byte_to_f<F>(x);
+    else return Elem<T>::to_f(x);
+  };
   extern __shared__ float gsm[];
   const int D = p.head_dim, BS = p.block_size;
   auto score = [&](float dot) { return p.ref_scores ? ref_score<T>(dot, p.scale) : dot * p.scale; };
@@ -99,8 +109,8 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
   for (int x = tid; x < D; x += kGenericThreads) qs[x] = Elem<T>::to_f(qp[x]);
   __syncthreads();
 
-  const T *kc = static_cast<const T *>(p.k_cache);
-  const T *vc = static_cast<const T *>(p.v_cache);
+  const C *kc = static_cast<const C *>(p.k_cache);
+  const C *vc = static_cast<const C *>(p.v_cache);
   constexpr int kPerLane = kGenericMaxDim / 32;
   float acc[kPerLane];
 #pragma unroll
@@ -123,7 +133,14 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
     if (b + kGenericWarps < nb) next_id = table[b + kGenericWarps];
     if (uint32_t(id) >= uint32_t(p.num_blocks)) { bad_id = true; id = 0; }
     const int kv_start = b * BS;
-    const int bn = min(BS, L - kv_start);
+    // An 8-bit pool's rows past the query's own position are not touched at all: their bytes may
+    // be NaN, which a probability of 0 would not mask.
+    const int bn = min(BS, (k8 ? limit + 1 : L) - kv_start);
+    float ks = 1.f, vs = 1.f;
+    if constexpr (k8) {
+      ks = p.k_scale[size_t(id) * p.num_kv_heads + kh];
+      vs = p.v_scale[size_t(id) * p.num_kv_heads + kh];
+    }
     const size_t base = (size_t(id) * p.num_kv_heads + kh) * BS * size_t(D);
     if (small) {
       float kr[kSmallRows][2], vr[kSmallRows][2];
@@ -133,8 +150,8 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
         for (int k = 0; k < 2; ++k) {
           const bool in = j < bn && lane + 32 * k < D;
           const size_t off = base + size_t(j) * D + lane + 32 * k;
-          kr[j][k] = in ? Elem<T>::to_f(kc[off]) : 0.f;
-          vr[j][k] = in ? Elem<T>::to_f(vc[off]) : 0.f;
+          kr[j][k] = in ? elem(kc[off]) : 0.f;
+          vr[j][k] = in ? elem(vc[off]) : 0.f;
         }
       float sc[kSmallRows];
 #pragma unroll
@@ -148,6 +165,7 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
       float bmax = neg_inf();
 #pragma unroll
       for (int j = 0; j < kSmallRows; ++j) {
+        if constexpr (k8) sc[j] *= ks;
         sc[j] = (j < bn && kv_start + j <= limit) ? score(sc[j]) : neg_inf();
         bmax = fmaxf(bmax, sc[j]);
       }
@@ -158,8 +176,9 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
       for (int k = 0; k < 2; ++k) acc[k] *= corr;
 #pragma unroll
       for (int j = 0; j < kSmallRows; ++j) {
-        const float pj = j < bn ? expf(sc[j] - new_max) : 0.f;
+        float pj = j < bn ? expf(sc[j] - new_max) : 0.f;
         psum += pj;
+        if constexpr (k8) pj *= vs;
 #pragma unroll
         for (int k = 0; k < 2; ++k) acc[k] = fmaf(pj, vr[j][k], acc[k]);
       }
@@ -176,10 +195,10 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
       for (int r = 0; r < 4; ++r) {
         dot[r] = 0.f;
         if (j0 + r < bn) {
-          const T *kr = kc + base + size_t(j0 + r) * D;
+          const C *kr = kc + base + size_t(j0 + r) * D;
 #pragma unroll
           for (int k = 0; k < kPerLane; ++k)
-            if (lane + 32 * k < D) dot[r] = fmaf(qv[k], Elem<T>::to_f(kr[lane + 32 * k]), dot[r]);
+            if (lane + 32 * k < D) dot[r] = fmaf(qv[k], elem(kr[lane + 32 * k]), dot[r]);
         }
       }
 #pragma unroll
@@ -189,6 +208,7 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (j0 + r < bn) {
+          if constexpr (k8) dot[r] *= ks;
           const float sc = (kv_start + j0 + r > limit) ? neg_inf() : score(dot[r]);
           if (lane == 0) pw[j0 + r] = sc;
           bmax = fmaxf(bmax, sc);
@@ -212,11 +232,11 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
     for (int k = 0; k < kPerLane; ++k) acc[k] *= corr;
 #pragma unroll 4
     for (int j = 0; j < bn; ++j) {
-      const float pj = pw[j];
-      const T *vr = vc + base + size_t(j) * D;
+      const float pj = k8 ? pw[j] * vs : pw[j];
+      const C *vr = vc + base + size_t(j) * D;
 #pragma unroll
       for (int k = 0; k < kPerLane; ++k)
-        if (lane + 32 * k < D) acc[k] = fmaf(pj, Elem<T>::to_f(vr[lane + 32 * k]), acc[k]);
+        if (lane + 32 * k < D) acc[k] = fmaf(pj, elem(vr[lane + 32 * k]), acc[k]);
     }
     l = l * corr + psum;
     m = new_max;

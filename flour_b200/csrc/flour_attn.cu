@@ -10,11 +10,15 @@
 #include <cstdint>
 #include <mutex>
 #include <unordered_map>
+#include <utility>
 
 #include "attn_generic.cuh"
 #include "cache_ops.cuh"
 #include "decode_sm100.cuh"
 #include "gemm_sm100.cuh"
+#include "kv8_decode_sm100.cuh"
+#include "kv8_expand.cuh"
+#include "logprobs.cuh"
 #include "prefill_sm100.cuh"
 #include "flour_attn.h"
 
@@ -409,7 +413,7 @@ fa_status launch_prefill_t(const fa::PrefillParams &p, const CUtensorMap &tq, co
 fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const int32_t *cu,
                          const int32_t *ctx, const int32_t *tables, int max_blocks, int num_seqs,
                          int num_heads, int n_rep, int total_q, float scale, int score_flow,
-                         void *ws, size_t ws_bytes, cudaStream_t stream) {
+                         void *ws, size_t ws_bytes, cudaStream_t stream, int q_rows = 0) {
   if (!ws) return fail(FA_EINVAL, "prefill: workspace is NULL but %zu bytes are needed", kPrefillWorkspace);
   if (ws_bytes < kPrefillWorkspace)
     return fail(FA_ERANGE, "prefill: workspace of %zu bytes, %zu needed", ws_bytes, kPrefillWorkspace);
@@ -429,7 +433,11 @@ fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const i
   const bool ref = score_flow == FA_SCORES_REFERENCE;
   const int64_t rows = int64_t(L->num_blocks) * L->num_kv_heads * L->block_size;
   CUtensorMap tmq, tk, tv;
-  if (fa_status s = make_q_map(&tmq, q, total_q, num_heads, n_rep, p.tq, L->dtype); s != FA_OK) return s;
+  // q_rows: rows behind `q` where they are more than total_q (a short batch copied and padded to
+  // one box).
+  if (fa_status s = make_q_map(&tmq, q, std::max(q_rows, total_q), num_heads, n_rep, p.tq, L->dtype);
+      s != FA_OK)
+    return s;
   if (fa_status s = make_page_map(&tk, L->k_cache, rows, 128, L->dtype); s != FA_OK) return s;
   if (fa_status s = make_page_map(&tv, L->v_cache, rows, 128, L->dtype); s != FA_OK) return s;
   // One persistent CTA per SM; at most kPfMaxSeqs sequences per launch (their chunk table lives
@@ -758,6 +766,287 @@ fa_status bundle_launch(const fa::BundleParams &p, int vec, cudaStream_t stream,
     default: fa::bundle_payload_kernel<2, kImport><<<grid, 256, 0, stream>>>(p); break;
   }
   return check_launch(who);
+}
+
+// ---- 8-bit cache ----------------------------------------------------------------------------
+
+fa_status check_layer8(const fa_kv8_layer *L, const char *who) {
+  if (!L) return fail(FA_EINVAL, "%s: layer is NULL", who);
+  if (!L->k_cache || !L->v_cache || !L->k_scale || !L->v_scale)
+    return fail(FA_EINVAL, "%s: k_cache/v_cache/k_scale/v_scale is NULL", who);
+  if (L->dtype != FA_KV8_E4M3 && L->dtype != FA_KV8_I8)
+    return fail(FA_EINVAL, "%s: unknown 8-bit format %d", who, L->dtype);
+  if (L->num_blocks <= 0 || L->num_kv_heads <= 0 || L->block_size <= 0 || L->head_dim <= 0)
+    return fail(FA_EINVAL, "%s: layer dims must be positive (blocks=%d kv_heads=%d bs=%d d=%d)",
+                who, L->num_blocks, L->num_kv_heads, L->block_size, L->head_dim);
+  if (L->head_dim > fa::kGenericMaxDim)
+    return fail(FA_EUNSUPPORTED, "%s: head_dim %d > %d is not supported", who, L->head_dim, fa::kGenericMaxDim);
+  if (L->block_size > 1024)
+    return fail(FA_EUNSUPPORTED, "%s: block_size %d > 1024 is not supported", who, L->block_size);
+  if (!aligned(L->k_scale, 4) || !aligned(L->v_scale, 4))
+    return fail(FA_EINVAL, "%s: scales must be 4-byte aligned", who);
+  return FA_OK;
+}
+
+// The checks shared by attention over a 16/32-bit pool, on the 8-bit layer's sizes.
+fa_status check_attention8_args(const char *who, const fa_kv8_layer *L, const void *q, const void *out,
+                                int32_t dtype, const int32_t *ctx, const int32_t *tables, int max_blocks,
+                                int num_seqs, int num_heads, int n_rep, int max_context_len, float scale) {
+  if (fa_status s = check_layer8(L, who); s != FA_OK) return s;
+  const fa_kv_layer as{L->k_cache, L->v_cache, L->num_blocks, L->num_kv_heads, L->block_size,
+                       L->head_dim, dtype};
+  if (fa_status s = check_attention_args(who, &as, q, out, ctx, tables, max_blocks, num_seqs, num_heads,
+                                         n_rep, max_context_len, scale);
+      s != FA_OK)
+    return s;
+  if (!aligned(q, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)))
+    return fail(FA_EINVAL, "%s: misaligned query/out", who);
+  return FA_OK;
+}
+
+// 2-D map over an 8-bit slab viewed as [rows, head_dim] bytes; one box is a page of one head,
+// swizzled by 128 bytes (head_dim 128) or 64 (head_dim 64).
+fa_status make_page8_map(CUtensorMap *map, void *base, int64_t rows, int head_dim) {
+  if (fa_status s = get_encoder(); s != FA_OK) return s;
+  cuuint64_t dims[2] = {cuuint64_t(head_dim), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(head_dim)};
+  cuuint32_t box[2] = {cuuint32_t(head_dim), 16};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FA_ECUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return FA_OK;
+}
+
+// Calls f with the types of (query dtype, 8-bit format).
+template <class Fn> fa_status with_types8(int32_t dtype, int32_t fmt, Fn f) {
+  auto with_t = [&](auto t) { return fmt == FA_KV8_E4M3 ? f(t, fa::E4m3{}) : f(t, fa::I8{}); };
+  switch (dtype) {
+    case FA_F32: return with_t(float{});
+    case FA_BF16: return with_t(__nv_bfloat16{});
+    default: return with_t(__half{});
+  }
+}
+
+// Launch with programmatic stream serialization: the kernel waits for its predecessor before it
+// touches memory, and its successor may be set up while it runs.
+template <class... KArgs, class... Args>
+fa_status launch_pdl(const char *who, void (*kern)(KArgs...), dim3 grid, int threads, size_t smem,
+                     cudaStream_t stream, int cluster, Args &&...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  if (e != cudaSuccess) return fail(FA_ECUDA, "%s: launch: %s", who, cudaGetErrorString(e));
+  return check_launch(who);
+}
+
+bool decode8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, const void *q, const void *out) {
+  return (dtype == FA_BF16 || dtype == FA_F16) && L->block_size == fa::kPage &&
+         (L->head_dim == 64 || L->head_dim == 128) && n_rep >= 1 && n_rep <= 8 &&
+         int64_t(L->num_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
+         aligned(L->k_cache, 16) && aligned(L->v_cache, 16) && aligned(q, 8) && aligned(out, 2);
+}
+
+constexpr int kKv8Stages = 2;
+
+template <typename T, class F, int HD>
+fa_status launch_decode8_t(const fa::DecodeParams &p, const fa::Kv8Cache &c, const CUtensorMap &tk,
+                           const CUtensorMap &tv, cudaStream_t stream) {
+  using S = fa::Kv8DecodeSmem<HD, kKv8Stages>;
+  auto kern = fa::kv8_decode_kernel<T, F, HD, kKv8Stages>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAlloc);
+  if (e != cudaSuccess)
+    return fail(FA_ECUDA, "paged_decode_kv8: set smem attribute: %s", cudaGetErrorString(e));
+  return launch_pdl("paged_decode_kv8", kern, dim3(p.max_splits, p.num_kv_heads, p.num_seqs),
+                    fa::kDecodeThreads, S::kAlloc, stream, 1, p, c, tk, tv);
+}
+
+fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *ctx,
+                         const int32_t *tables, int max_blocks, int num_seqs, int num_heads, int n_rep,
+                         int max_context_len, float scale, void *ws, size_t ws_bytes, cudaStream_t stream) {
+  DecodePlan plan;
+  if (!plan_decode(num_seqs, L->num_kv_heads, max_context_len, &plan))
+    return fail(FA_EUNSUPPORTED, "paged_decode_kv8: context of %d tokens needs more than %d splits",
+                max_context_len, fa::kDecodeMaxSplits);
+  const DecodeWorkspace w =
+      decode_workspace_layout(num_seqs, num_heads, L->num_kv_heads, L->head_dim, plan);
+  if (w.bytes > 0) {
+    if (!ws) return fail(FA_EINVAL, "paged_decode_kv8: workspace is NULL but %zu bytes are needed", w.bytes);
+    if (ws_bytes < w.bytes)
+      return fail(FA_ERANGE, "paged_decode_kv8: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
+    if (!aligned(ws, 256)) return fail(FA_EINVAL, "paged_decode_kv8: workspace must be 256-byte aligned");
+    if (fa_status s = zero_stale_tickets(ws, w.lse_off, stream); s != FA_OK) return s;
+  }
+  fa::DecodeParams p{};
+  p.q = q;
+  p.out = out;
+  p.context_lens = ctx;
+  p.block_tables = tables;
+  char *wsb = static_cast<char *>(ws);
+  p.counters = w.bytes ? reinterpret_cast<int32_t *>(wsb + w.counters_off) : nullptr;
+  p.part_lse = w.bytes ? reinterpret_cast<float *>(wsb + w.lse_off) : nullptr;
+  p.part_o = w.bytes ? reinterpret_cast<float *>(wsb + w.o_off) : nullptr;
+  p.max_blocks_per_seq = max_blocks;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_heads;
+  p.num_kv_heads = L->num_kv_heads;
+  p.n_rep = n_rep;
+  p.num_blocks = L->num_blocks;
+  p.pages_per_split = plan.pages_per_split;
+  p.max_splits = plan.max_splits;
+  p.max_context_len = max_context_len;
+  p.scale_log2 = scale * fa::kLog2e;
+  p.scale = scale;
+  const fa::Kv8Cache c{L->k_scale, L->v_scale};
+  const int64_t rows = int64_t(L->num_blocks) * L->num_kv_heads * L->block_size;
+  CUtensorMap tk, tv;
+  if (fa_status s = make_page8_map(&tk, L->k_cache, rows, L->head_dim); s != FA_OK) return s;
+  if (fa_status s = make_page8_map(&tv, L->v_cache, rows, L->head_dim); s != FA_OK) return s;
+  return with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
+    using T = decltype(t);
+    using F = decltype(f);
+    if constexpr (sizeof(T) == 2) {
+      if (L->head_dim == 128) return launch_decode8_t<T, F, 128>(p, c, tk, tv, stream);
+      return launch_decode8_t<T, F, 64>(p, c, tk, tv, stream);
+    } else {
+      return fail(FA_EUNSUPPORTED, "paged_decode_kv8: f32 queries take the generic kernel");
+    }
+  });
+}
+
+fa_status launch_generic8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *cu,
+                          const int32_t *ctx, const int32_t *tables, int max_blocks, int num_seqs,
+                          int num_heads, int n_rep, int total_q, float scale, cudaStream_t stream,
+                          const char *who) {
+  if (num_heads > 65535) return fail(FA_EUNSUPPORTED, "%s: more than 65535 heads", who);
+  fa::GenericParams p{};
+  p.q = q;
+  p.out = out;
+  p.k_cache = L->k_cache;
+  p.v_cache = L->v_cache;
+  p.k_scale = L->k_scale;
+  p.v_scale = L->v_scale;
+  p.cu_seqlens_q = cu;
+  p.context_lens = ctx;
+  p.block_tables = tables;
+  p.max_blocks_per_seq = max_blocks;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_heads;
+  p.num_kv_heads = L->num_kv_heads;
+  p.n_rep = n_rep;
+  p.head_dim = L->head_dim;
+  p.block_size = L->block_size;
+  p.num_blocks = L->num_blocks;
+  p.total_q = total_q;
+  p.scale = scale;
+  const size_t smem = fa::generic_smem_floats(L->block_size) * sizeof(float);
+  return with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
+    auto kern = fa::generic_attn_kernel<decltype(t), decltype(f)>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return fail(FA_ECUDA, "%s: set smem attribute: %s", who, cudaGetErrorString(e));
+    kern<<<dim3(total_q, num_heads), fa::kGenericThreads, smem, stream>>>(p);
+    return check_launch(who);
+  });
+}
+
+// Whether the tcgen05 prefill serves a call, over a copy of the cache in the query type.
+bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float scale, const void *q,
+                        const void *out, int num_seqs, int32_t total_blocks) {
+  return (dtype == FA_BF16 || dtype == FA_F16) && L->block_size == fa::kPage && L->head_dim == 128 &&
+         n_rep >= 1 && n_rep <= 128 && scale > 0.f && num_seqs <= fa::kExpandMaxSeqs &&
+         int64_t(total_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
+         aligned(L->k_cache, 8) && aligned(L->v_cache, 8) && aligned(q, 16) && aligned(out, 32);
+}
+
+struct Prefill8Workspace {
+  size_t q_off, ctx_off, tables_off, k_off, v_off, bytes;
+};
+
+// Work counters of the prefill kernel, a padded copy of a query batch shorter than one box, the
+// copy's context lengths and block tables, the copied pages.
+Prefill8Workspace prefill8_workspace_layout(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                            int max_context_len, int32_t total_blocks) {
+  auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
+  Prefill8Workspace w{};
+  const int width = std::max(1, (max_context_len + fa::kPage - 1) / fa::kPage);
+  w.q_off = kPrefillWorkspace;
+  w.ctx_off = w.q_off + r256(size_t(128) * num_heads * head_dim * 2);
+  w.tables_off = w.ctx_off + r256(size_t(num_seqs) * 4);
+  w.k_off = w.tables_off + r256(size_t(num_seqs) * width * 4);
+  const size_t slab = r256(size_t(std::max(1, total_blocks)) * num_kv_heads * fa::kPage * head_dim * 2);
+  w.v_off = w.k_off + slab;
+  w.bytes = w.v_off + slab;
+  return w;
+}
+
+fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *cu,
+                          const int32_t *ctx, const int32_t *tables, int max_blocks, int num_seqs,
+                          int num_heads, int n_rep, int total_q, int max_context_len, int32_t total_blocks,
+                          float scale, void *ws, size_t ws_bytes, cudaStream_t stream) {
+  const char *who = "paged_prefill_kv8";
+  const Prefill8Workspace w = prefill8_workspace_layout(num_seqs, num_heads, L->num_kv_heads, L->head_dim,
+                                                        max_context_len, total_blocks);
+  if (!ws) return fail(FA_EINVAL, "%s: workspace is NULL but %zu bytes are needed", who, w.bytes);
+  if (ws_bytes < w.bytes)
+    return fail(FA_ERANGE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, w.bytes);
+  if (!aligned(ws, 256)) return fail(FA_EINVAL, "%s: workspace must be 256-byte aligned", who);
+  // The work counters must be zero and this call's copy lies behind them, as a decode's partials
+  // lie behind its tickets.
+  if (fa_status s = zero_stale_tickets(ws, kPrefillWorkspace, stream); s != FA_OK) return s;
+  char *wsb = static_cast<char *>(ws);
+  const int box = 128 / n_rep;
+  const bool pad = total_q < box;
+  fa::Kv8ExpandParams e{};
+  e.cache[0] = static_cast<const uint8_t *>(L->k_cache);
+  e.cache[1] = static_cast<const uint8_t *>(L->v_cache);
+  e.scale[0] = L->k_scale;
+  e.scale[1] = L->v_scale;
+  e.out[0] = wsb + w.k_off;
+  e.out[1] = wsb + w.v_off;
+  e.context_lens = ctx;
+  e.block_tables = tables;
+  e.out_ctx = reinterpret_cast<int32_t *>(wsb + w.ctx_off);
+  e.out_tables = reinterpret_cast<int32_t *>(wsb + w.tables_off);
+  if (pad) {
+    e.q = q;
+    e.q_out = wsb + w.q_off;
+    e.q_elems = int64_t(total_q) * num_heads * L->head_dim;
+    e.q_out_elems = int64_t(box) * num_heads * L->head_dim;
+  }
+  e.max_blocks_per_seq = max_blocks;
+  e.out_width = std::max(1, (max_context_len + fa::kPage - 1) / fa::kPage);
+  e.num_seqs = num_seqs;
+  e.total_blocks = total_blocks;
+  e.num_kv_heads = L->num_kv_heads;
+  e.num_blocks = L->num_blocks;
+  e.block_size = L->block_size;
+  e.head_dim = L->head_dim;
+  e.max_context_len = max_context_len;
+  const int grid = std::max(1, std::min(total_blocks, sm_count() * 8));
+  fa_status st = with_types8(dtype, L->dtype, [&](auto t, auto f) {
+    return launch_pdl(who, fa::kv8_expand_kernel<decltype(t), decltype(f), true>, dim3(grid),
+                      fa::kExpandThreads, 0, stream, 1, e);
+  });
+  if (st != FA_OK) return st;
+  const fa_kv_layer copy{wsb + w.k_off, wsb + w.v_off, total_blocks, L->num_kv_heads, L->block_size,
+                         L->head_dim, dtype};
+  return launch_prefill(&copy, pad ? e.q_out : q, out, cu, e.out_ctx, e.out_tables, e.out_width, num_seqs,
+                        num_heads, n_rep, total_q, scale, FA_SCORES_F32, ws, kPrefillWorkspace, stream,
+                        pad ? box : 0);
 }
 
 }  // namespace
@@ -1232,6 +1521,194 @@ fa_status fa_last_token_logits(const void *hidden, const int32_t *cu_seqlens, in
   if (fa_status s = check_launch(who); s != FA_OK) return s;
   return launch_gemm<T>(num_seqs, vocab, hidden_size, fa::F32Epilogue{logits_out}, normed_out,
                         lm_head, dtype, st, who);
+}
+
+// ---- 8-bit cache ----------------------------------------------------------------------------
+
+fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const void *value, int32_t dtype,
+                              int64_t key_stride_token, int64_t key_stride_head,
+                              int64_t value_stride_token, int64_t value_stride_head,
+                              const int32_t *cu_seqlens_q, const int32_t *context_lens,
+                              const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t num_seqs,
+                              int32_t total_q, fa_stream_t stream) {
+  const char *who = "paged_append_kv8";
+  if (fa_status s = check_layer8(layer, who); s != FA_OK) return s;
+  if (dtype != FA_F32 && dtype != FA_BF16 && dtype != FA_F16)
+    return fail(FA_EINVAL, "%s: unknown key/value dtype %d", who, dtype);
+  if (num_seqs < 0 || total_q < 0 || max_blocks_per_seq <= 0)
+    return fail(FA_EINVAL, "%s: num_seqs=%d total_q=%d max_blocks_per_seq=%d", who, num_seqs, total_q,
+                max_blocks_per_seq);
+  if (!cu_seqlens_q && total_q != num_seqs)
+    return fail(FA_EINVAL, "%s: without cu_seqlens_q total_q (%d) must equal num_seqs (%d)", who, total_q,
+                num_seqs);
+  if (num_seqs == 0 || total_q == 0) return ok();
+  if (!key || !value || !context_lens || !block_tables)
+    return fail(FA_EINVAL, "%s: NULL key/value/context_lens/block_tables", who);
+  if (key_stride_token < 0 || key_stride_head < 0 || value_stride_token < 0 || value_stride_head < 0)
+    return fail(FA_EINVAL, "%s: negative key/value stride", who);
+  if (!aligned(key, dtype_size(dtype)) || !aligned(value, dtype_size(dtype)))
+    return fail(FA_EINVAL, "%s: misaligned key/value", who);
+  if (layer->num_kv_heads > 32767) return fail(FA_EUNSUPPORTED, "%s: more than 32767 KV heads", who);
+  fa::Kv8AppendParams p{};
+  p.x[0] = key;
+  p.x[1] = value;
+  p.stride_t[0] = key_stride_token;
+  p.stride_t[1] = value_stride_token;
+  p.stride_h[0] = key_stride_head;
+  p.stride_h[1] = value_stride_head;
+  p.cache[0] = static_cast<uint8_t *>(layer->k_cache);
+  p.cache[1] = static_cast<uint8_t *>(layer->v_cache);
+  p.scale[0] = layer->k_scale;
+  p.scale[1] = layer->v_scale;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.context_lens = context_lens;
+  p.block_tables = block_tables;
+  p.max_blocks_per_seq = max_blocks_per_seq;
+  p.num_seqs = num_seqs;
+  p.total_q = total_q;
+  p.num_kv_heads = layer->num_kv_heads;
+  p.num_blocks = layer->num_blocks;
+  p.block_size = layer->block_size;
+  p.head_dim = layer->head_dim;
+  const int per_run = 2 * layer->num_kv_heads;
+  dim3 grid;
+  if (!cu_seqlens_q) {
+    const int64_t g = (int64_t(num_seqs) * per_run + fa::kAppendWarps - 1) / fa::kAppendWarps;
+    if (g > INT32_MAX) return fail(FA_EUNSUPPORTED, "%s: too many (sequence, head) units", who);
+    grid = dim3(unsigned(g));
+  } else {
+    // About one run begins in each 16 tokens of a long prompt, up to 16 in a batch of short ones.
+    grid = dim3(unsigned((total_q + fa::kAppendChunk - 1) / fa::kAppendChunk),
+                unsigned((per_run + fa::kAppendWarps - 1) / fa::kAppendWarps));
+  }
+  return with_types8(dtype, layer->dtype, [&](auto t, auto f) {
+    return launch_pdl(who, fa::kv8_append_kernel<decltype(t), decltype(f)>, grid, fa::kAppendThreads, 0,
+                      reinterpret_cast<cudaStream_t>(stream), 1, p);
+  });
+}
+
+size_t fa_paged_decode_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                          int32_t head_dim, int32_t max_context_len) {
+  return fa_paged_attention_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len, 1);
+}
+
+fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void *out, int32_t dtype,
+                              const int32_t *context_lens, const int32_t *block_tables,
+                              int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_heads,
+                              int32_t n_rep, int32_t max_context_len, float scale, void *workspace,
+                              size_t workspace_bytes, fa_stream_t stream) {
+  const char *who = "paged_decode_kv8";
+  if (fa_status s = check_attention8_args(who, layer, query, out, dtype, context_lens, block_tables,
+                                          max_blocks_per_seq, num_seqs, num_heads, n_rep,
+                                          max_context_len, scale);
+      s != FA_OK)
+    return s;
+  if (num_seqs == 0) return ok();
+  if (max_context_len < 1) return fail(FA_ERANGE, "%s: max_context_len must be >= 1", who);
+  if (num_seqs > 65535) return fail(FA_EUNSUPPORTED, "%s: more than 65535 sequences per call", who);
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (decode8_fast_path(layer, n_rep, dtype, query, out))
+    return launch_decode8(layer, query, out, dtype, context_lens, block_tables, max_blocks_per_seq,
+                          num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
+                          workspace_bytes, st);
+  return launch_generic8(layer, query, out, dtype, nullptr, context_lens, block_tables, max_blocks_per_seq,
+                         num_seqs, num_heads, n_rep, num_seqs, scale, st, who);
+}
+
+size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t max_context_len, int32_t max_seqlen_q,
+                                           int32_t total_blocks) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context_len <= 0 ||
+      total_blocks < 0)
+    return 0;
+  const size_t copy = prefill8_workspace_layout(num_seqs, num_heads, num_kv_heads, head_dim,
+                                                max_context_len, total_blocks)
+                          .bytes;
+  if (max_seqlen_q != 1) return copy;
+  return std::max(copy, fa_paged_decode_kv8_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim,
+                                                           max_context_len));
+}
+
+fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, void *out, int32_t dtype,
+                               const int32_t *cu_seqlens_q, const int32_t *context_lens,
+                               const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t num_seqs,
+                               int32_t num_heads, int32_t n_rep, int32_t total_q, int32_t max_seqlen_q,
+                               int32_t max_context_len, int32_t total_blocks, float scale,
+                               void *workspace, size_t workspace_bytes, fa_stream_t stream) {
+  const char *who = "paged_prefill_kv8";
+  if (fa_status s = check_attention8_args(who, layer, query, out, dtype, context_lens, block_tables,
+                                          max_blocks_per_seq, num_seqs, num_heads, n_rep,
+                                          max_context_len, scale);
+      s != FA_OK)
+    return s;
+  if (!cu_seqlens_q) return fail(FA_EINVAL, "%s: cu_seqlens_q is NULL", who);
+  if (total_q < 0 || max_seqlen_q < 0 || total_blocks < 0 || total_blocks > (1 << 30))
+    return fail(FA_EINVAL, "%s: total_q=%d max_seqlen_q=%d total_blocks=%d", who, total_q, max_seqlen_q,
+                total_blocks);
+  if (max_seqlen_q > max_context_len)
+    return fail(FA_ERANGE, "%s: max_seqlen_q %d > max_context_len %d", who, max_seqlen_q, max_context_len);
+  if (total_q == 0 || num_seqs == 0) return ok();
+  if (max_seqlen_q == 1 && total_q == num_seqs)  // one new token each
+    return fa_paged_decode_kv8(layer, query, out, dtype, context_lens, block_tables, max_blocks_per_seq,
+                               num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
+                               workspace_bytes, stream);
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (total_blocks > 0 &&
+      prefill8_fast_path(layer, n_rep, dtype, scale, query, out, num_seqs, total_blocks))
+    return launch_prefill8(layer, query, out, dtype, cu_seqlens_q, context_lens, block_tables,
+                           max_blocks_per_seq, num_seqs, num_heads, n_rep, total_q, max_context_len,
+                           total_blocks, scale, workspace, workspace_bytes, st);
+  return launch_generic8(layer, query, out, dtype, cu_seqlens_q, context_lens, block_tables,
+                         max_blocks_per_seq, num_seqs, num_heads, n_rep, total_q, scale, st, who);
+}
+
+// ---- log probabilities -------------------------------------------------------------------------
+
+fa_status fa_token_logprobs(const void *logits, int32_t dtype, int64_t row_stride, int32_t num_rows,
+                            int32_t vocab, const int32_t *token_ids, float *logprobs_out,
+                            float *entropy_out, int32_t top_k, int32_t *top_ids_out,
+                            float *top_logprobs_out, fa_stream_t stream) {
+  const char *who = "token_logprobs";
+  if (dtype != FA_F32 && dtype != FA_BF16 && dtype != FA_F16)
+    return fail(FA_EINVAL, "%s: unknown dtype %d", who, dtype);
+  if (num_rows < 0 || vocab <= 0) return fail(FA_EINVAL, "%s: num_rows=%d vocab=%d", who, num_rows, vocab);
+  if (top_k < 0 || top_k > FA_MAX_TOP_LOGPROBS)
+    return fail(FA_EINVAL, "%s: top_k %d outside [0, %d]", who, top_k, FA_MAX_TOP_LOGPROBS);
+  if (num_rows == 0) return ok();
+  if (!logits) return fail(FA_EINVAL, "%s: logits is NULL", who);
+  if ((token_ids != nullptr) != (logprobs_out != nullptr))
+    return fail(FA_EINVAL, "%s: token_ids and logprobs_out go together", who);
+  if (top_k > 0 && (!top_ids_out || !top_logprobs_out))
+    return fail(FA_EINVAL, "%s: NULL top_ids_out/top_logprobs_out with top_k %d", who, top_k);
+  if (num_rows > 1 && row_stride < vocab)
+    return fail(FA_EINVAL, "%s: row_stride %lld < vocab %d", who, (long long)row_stride, vocab);
+  if (!aligned(logits, dtype_size(dtype))) return fail(FA_EINVAL, "%s: misaligned logits", who);
+  if (num_rows > INT32_MAX / fa::kLpMaxCluster) return fail(FA_EUNSUPPORTED, "%s: %d rows", who, num_rows);
+  fa::LogprobParams p{};
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.token_ids = token_ids;
+  p.logprobs = logprobs_out;
+  p.entropy = entropy_out;
+  p.top_ids = top_ids_out;
+  p.top_logprobs = top_logprobs_out;
+  p.vocab = vocab;
+  p.top_k = top_k;
+  // CTAs per row: as many as fill the GPU, each with a tile of the row or more.
+  int ranks = 1;
+  while (ranks < fa::kLpMaxCluster && int64_t(num_rows) * ranks * 2 <= int64_t(sm_count()) * 4 &&
+         vocab / (ranks * 2) >= fa::kLpThreads * fa::kLpTile / 2)
+    ranks *= 2;
+  const dim3 grid(unsigned(num_rows * ranks));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case FA_F32:
+      return launch_pdl(who, fa::token_logprobs_kernel<float>, grid, fa::kLpThreads, 0, st, ranks, p);
+    case FA_BF16:
+      return launch_pdl(who, fa::token_logprobs_kernel<__nv_bfloat16>, grid, fa::kLpThreads, 0, st, ranks, p);
+    default:
+      return launch_pdl(who, fa::token_logprobs_kernel<__half>, grid, fa::kLpThreads, 0, st, ranks, p);
+  }
 }
 
 // ---- head-sharded decode ------------------------------------------------------------------

@@ -373,3 +373,180 @@ def o_proj_residual(attn, weight, residual=None, out=None, stream=None) -> torch
                                    fout, fa_dtype(dt), _stream(stream)),
           "o_proj_residual")
     return out
+
+
+# ---- 8-bit KV cache -------------------------------------------------------------------------
+
+_KV8 = {torch.float8_e4m3fn: _lib.FA_KV8_E4M3, torch.int8: _lib.FA_KV8_I8}
+
+
+def _device(device: torch.device, *tensors: torch.Tensor | None) -> torch.device:
+    """The one CUDA device that all tensors live on; the call is made with it current."""
+    if device.type != "cuda":
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"tensors must be on a CUDA device, not {device}")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise _lib.FlourAttnError(_lib.FA_EINVAL, f"tensors on {device} and {t.device} in one call")
+    return device
+
+
+def _call_on(device: torch.device, stream, what: str, fn, *args) -> None:
+    """fn(*args, stream) on `stream`, or on the device's current stream, with it current."""
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    elif stream.device != device:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"{what}: stream of {stream.device}, tensors on {device}")
+    if torch.cuda.current_device() == device.index:
+        st = fn(*args, ctypes.c_void_p(stream.cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, ctypes.c_void_p(stream.cuda_stream))
+    check(st, what)
+
+
+def kv8_layer_desc(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor) -> _lib.FaKv8Layer:
+    """``fa_kv8_layer`` of 8-bit slabs [num_blocks, kv_heads, bs, head_dim] (torch.float8_e4m3fn
+    or torch.int8) and their f32 scales [num_blocks, kv_heads]."""
+    if k_cache.dtype not in _KV8:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"unsupported 8-bit cache dtype {k_cache.dtype}")
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, "k_cache and v_cache differ in shape or dtype")
+    if k_cache.dim() != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                  "cache slabs must be contiguous [num_blocks, kv_heads, bs, d]")
+    nb, kvh, bs, d = k_cache.shape
+    for t in (k_scale, v_scale):
+        if t.dtype != torch.float32 or t.shape != (nb, kvh) or not t.is_contiguous():
+            raise _lib.FlourAttnError(_lib.FA_EINVAL, f"scales must be contiguous f32 [{nb}, {kvh}]")
+    _device(k_cache.device, v_cache, k_scale, v_scale)
+    return _lib.FaKv8Layer(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                           v_scale.data_ptr(), nb, kvh, bs, d, _KV8[k_cache.dtype])
+
+
+def _tables(block_tables, context_lens, num_seqs: int):
+    bt, cl = _i32(block_tables, "block_tables"), _i32(context_lens, "context_lens")
+    if bt.dim() != 2 or bt.shape[0] != num_seqs or cl.numel() != num_seqs:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                  f"block_tables must be [{num_seqs}, max_blocks], context_lens [{num_seqs}]")
+    return bt, cl
+
+
+def _cu(cu_seqlens_q, num_seqs: int):
+    cu = _i32(cu_seqlens_q, "cu_seqlens_q")
+    if cu.numel() != num_seqs + 1:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"cu_seqlens_q must be [{num_seqs + 1}]")
+    return cu
+
+
+def _query8(query, k_cache, out):
+    if query.dim() != 3 or query.shape[2] != k_cache.shape[3]:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"query must be [tokens, heads, {k_cache.shape[3]}]")
+    query = query.contiguous()
+    if out is None:
+        return query, torch.empty_like(query)
+    if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, "out must be contiguous, of the query's shape and dtype")
+    return query, out
+
+
+def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_tables, context_lens,
+                     cu_seqlens_q=None, stream=None) -> None:
+    """Quantise new tokens into an 8-bit pool. key/value [T, kv_heads, d] (bf16, f16 or f32, any
+    token/head strides, unit stride on d) are the last tokens of their sequences: sequence s
+    holds context_lens[s] tokens, the new ones (cu_seqlens_q[s] .. cu_seqlens_q[s+1], or one each
+    when cu_seqlens_q is None) included. A block's scale is a power of two that grows as it
+    fills. A block that receives tokens belongs to one sequence of the call."""
+    layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
+    if key.shape != value.shape or key.dtype != value.dtype or \
+            key.dim() != 3 or key.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
+        raise _lib.FlourAttnError(
+            _lib.FA_EINVAL, f"key/value must be [T, {k_cache.shape[1]}, {k_cache.shape[3]}] of one dtype")
+    if key.stride(-1) != 1 or value.stride(-1) != 1:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, "key/value need unit stride on head_dim")
+    T = key.shape[0]
+    S = T if cu_seqlens_q is None else context_lens.numel()
+    bt, cl = _tables(block_tables, context_lens, S)
+    cu = None if cu_seqlens_q is None else _cu(cu_seqlens_q, S)
+    dev = _device(k_cache.device, key, value, bt, cl, cu)
+    _call_on(dev, stream, "paged_append_kv8", lib().fa_paged_append_kv8, ctypes.byref(layer),
+             _ptr(key), _ptr(value), fa_dtype(key.dtype), key.stride(0), key.stride(1),
+             value.stride(0), value.stride(1), _ptr(cu), _ptr(cl), _ptr(bt), bt.shape[1], S, T)
+
+
+def _ws8(workspace: Workspace | None, need: int, device: torch.device):
+    if workspace is None or not need:
+        return _ws_args(workspace, need)
+    if torch.cuda.current_device() == device.index:
+        args = _ws_args(workspace, need)
+    else:
+        with torch.cuda.device(device):
+            args = _ws_args(workspace, need)
+    if workspace.buf.device != device:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"workspace on {workspace.buf.device}, tensors on {device}")
+    return args
+
+
+def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
+                     n_rep: int, scale: float, max_context_len: int,
+                     workspace: Workspace | None = None, out=None, stream=None):
+    """paged_decode over an 8-bit pool: query [B, Hq, d] (bf16, f16 or f32) -> out [B, Hq, d]."""
+    layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
+    query, out = _query8(query, k_cache, out)
+    B, hq, d = query.shape
+    bt, cl = _tables(block_tables, context_lens, B)
+    dev = _device(k_cache.device, query, out, bt, cl)
+    need = int(lib().fa_paged_decode_kv8_workspace_size(B, hq, k_cache.shape[1], d, max_context_len))
+    wp, wn = _ws8(workspace, need, dev)
+    _call_on(dev, stream, "paged_decode_kv8", lib().fa_paged_decode_kv8, ctypes.byref(layer),
+             _ptr(query), _ptr(out), fa_dtype(query.dtype), _ptr(cl), _ptr(bt), bt.shape[1], B, hq,
+             n_rep, max_context_len, scale, wp, wn)
+    return out
+
+
+def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, context_lens,
+                      block_tables, n_rep: int, scale: float, max_seqlen_q: int,
+                      max_context_len: int, total_blocks: int,
+                      workspace: Workspace | None = None, out=None, stream=None):
+    """paged_prefill over an 8-bit pool whose suffix tokens are already appended. `total_blocks`:
+    at least the sum of ceil(context_len / block_size) over the batch."""
+    layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
+    query, out = _query8(query, k_cache, out)
+    tq, hq, d = query.shape
+    S = context_lens.numel()
+    bt, cl = _tables(block_tables, context_lens, S)
+    cu = _cu(cu_seqlens_q, S)
+    dev = _device(k_cache.device, query, out, bt, cl, cu)
+    need = int(lib().fa_paged_prefill_kv8_workspace_size(S, hq, k_cache.shape[1], d, max_context_len,
+                                                         max_seqlen_q, total_blocks))
+    wp, wn = _ws8(workspace, need, dev)
+    _call_on(dev, stream, "paged_prefill_kv8", lib().fa_paged_prefill_kv8, ctypes.byref(layer),
+             _ptr(query), _ptr(out), fa_dtype(query.dtype), _ptr(cu), _ptr(cl), _ptr(bt), bt.shape[1],
+             S, hq, n_rep, tq, max_seqlen_q, max_context_len, total_blocks, scale, wp, wn)
+    return out
+
+
+# ---- log probabilities ----------------------------------------------------------------------
+
+def token_logprobs(logits, token_ids=None, top_k: int = 0, stream=None):
+    """Log probabilities of logits rows [R, V] (f32, bf16 or f16; any row stride, unit stride on
+    V). token_ids int32 [R] (-1: none) or None. Returns (logprobs f32 [R] or None without
+    token_ids, entropy f32 [R], top_ids int32 [R, top_k], top_logprobs f32 [R, top_k]); ties go
+    to the lower id, tokens masked with -inf are not listed (id -1, -inf)."""
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, "logits must be [rows, vocab] with unit stride on vocab")
+    R, V = logits.shape
+    ids = None if token_ids is None else _i32(token_ids, "token_ids")
+    if ids is not None and ids.numel() != R:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"token_ids must be [{R}]")
+    if not 0 <= top_k <= _lib.FA_MAX_TOP_LOGPROBS:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"top_k {top_k} outside [0, {_lib.FA_MAX_TOP_LOGPROBS}]")
+    dev = _device(logits.device, ids)
+    logprobs = None if ids is None else torch.empty(R, dtype=torch.float32, device=dev)
+    entropy = torch.empty(R, dtype=torch.float32, device=dev)
+    top_ids = torch.empty((R, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((R, top_k), dtype=torch.float32, device=dev)
+    _call_on(dev, stream, "token_logprobs", lib().fa_token_logprobs, _ptr(logits), fa_dtype(logits.dtype),
+             logits.stride(0), R, V, _ptr(ids), _ptr(logprobs), _ptr(entropy), top_k,
+             _ptr(top_ids) if top_k else None, _ptr(top) if top_k else None)
+    return logprobs, entropy, top_ids, top

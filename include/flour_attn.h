@@ -74,6 +74,8 @@ typedef enum fa_dtype { FA_F32 = 0, FA_BF16 = 1, FA_F16 = 2 } fa_dtype;
 #define FA_DEVERR_PAIR 0x20      /* copy_blocks pair entry outside [0, num_blocks) */
 #define FA_DEVERR_POSITION 0x40  /* RoPE position outside [0, max_position) */
 #define FA_DEVERR_LAUNCH 0x80    /* a kernel refused a launch shape it does not support */
+#define FA_DEVERR_VALUE 0x100    /* fa_paged_append_kv8: an infinite or NaN key or value */
+#define FA_DEVERR_TOKEN 0x200    /* fa_token_logprobs: token id outside [-1, vocab) */
 
 /* How attention scores are formed before the softmax (the `score_flow` argument).
  *   FA_SCORES_F32        q.k accumulated in f32 and multiplied by scale in f32 (the default:
@@ -280,6 +282,101 @@ FA_API fa_status fa_paged_prefill(const fa_kv_layer *layer, const void *query, v
                            int32_t max_seqlen_q, int32_t max_context_len, float scale, int32_t score_flow,
                            void *workspace, size_t workspace_bytes, fa_stream_t stream);
 
+/* ---- 8-bit KV cache ----------------------------------------------------------------------
+ * No counterpart in the reference, whose pool holds the model's type. Half the bytes of a 16-bit
+ * pool: twice the tokens in the same HBM, and a decode step that reads half as much.
+ *
+ * One layer: K and V slabs of bytes [num_blocks, num_kv_heads, block_size, head_dim], laid out
+ * like the 16-bit pool's, and for each an f32 scale per (block, KV head). A value is
+ * byte * scale. Attention takes any finite scales (a cache quantised elsewhere); those that
+ * fa_paged_append_kv8 writes are powers of two. Blocks are copied, exported and shared like any
+ * block, with their scales: fa_copy_blocks takes the slabs as a 16-bit layer of head_dim / 2 and
+ * the scales as an FA_F32 layer of block_size 1 and head_dim 1. */
+typedef enum fa_kv8_dtype {
+  FA_KV8_E4M3 = 16,  /* 8-bit float, 4 exponent and 3 fraction bits, largest 448, no infinities */
+  FA_KV8_I8 = 17     /* signed integer, -127..127 */
+} fa_kv8_dtype;
+
+typedef struct fa_kv8_layer {
+  void *k_cache;          /* device, [num_blocks, num_kv_heads, block_size, head_dim] bytes */
+  void *v_cache;
+  float *k_scale;         /* device, [num_blocks, num_kv_heads] */
+  float *v_scale;
+  int32_t num_blocks;
+  int32_t num_kv_heads;
+  int32_t block_size;     /* <= 1024 */
+  int32_t head_dim;       /* <= 256 */
+  int32_t dtype;          /* fa_kv8_dtype */
+} fa_kv8_layer;
+
+/* Append new tokens to an 8-bit cache (the write of fa_reshape_and_cache, quantising).
+ *   key/value [total_q tokens, num_kv_heads, head_dim] of `dtype` (an fa_dtype), any token and
+ *     head strides in elements, unit stride on head_dim;
+ *   cu_seqlens_q device int32 [num_seqs + 1], or NULL: one new token per sequence
+ *     (total_q == num_seqs);
+ *   context_lens, block_tables as for the attention that follows: sequence s holds L tokens, the
+ *     new ones among them, and its n new tokens are positions L - n .. L - 1.
+ * For each block that receives tokens, each KV head, K and V apart, with o the block's first new
+ * row and a the largest finite magnitude among its new rows:
+ *   need  = the smallest power of two >= 2^-126 with a <= 448 need (e4m3) or 127 need (int8)
+ *   scale = need when o == 0 (a block that starts afresh: what an earlier owner left does not
+ *           count), else max(scale, need)
+ *   rows before o: re-encoded when the scale grew, q' = round(q * old / new); else untouched
+ *   new rows: round(x / scale), to nearest, ties to even; rows behind them: untouched.
+ * A scale only grows while its block fills, at most by factors of two or more, so re-encoding
+ * loses at most one int8 step in all, and nothing in e4m3 above its subnormals.
+ * Infinities saturate; NaN is stored as e4m3's NaN or int8's 0; either sets FA_DEVERR_VALUE and
+ * leaves the scale to the finite values.
+ * A block that receives tokens must belong to one sequence of the call (a shared prefix block is
+ * copied before it is written). Rows of key/value behind cu_seqlens_q[num_seqs] are not read. A
+ * sequence with bad lengths (FA_DEVERR_CONTEXT / FA_DEVERR_SEQLEN) or block ids
+ * (FA_DEVERR_BLOCK_ID) is not written there. No workspace. */
+FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const void *value,
+                                     int32_t dtype, int64_t key_stride_token, int64_t key_stride_head,
+                                     int64_t value_stride_token, int64_t value_stride_head,
+                                     const int32_t *cu_seqlens_q, const int32_t *context_lens,
+                                     const int32_t *block_tables, int32_t max_blocks_per_seq,
+                                     int32_t num_seqs, int32_t total_q, fa_stream_t stream);
+
+/* fa_paged_decode over an 8-bit cache: query/out [num_seqs, num_heads, head_dim] of `dtype` (an
+ * fa_dtype). Scores, softmax and sums in f32; the bytes enter the products exactly, probabilities
+ * rounded to f16. Rows of the last page behind the context are not used, whatever they hold (NaN
+ * bytes among them). A sequence with an invalid length gives zeros and FA_DEVERR_CONTEXT.
+ * The fast kernel takes FA_BF16 / FA_F16 queries, block_size 16, head_dim 64 or 128, n_rep <= 8,
+ * 16-byte aligned slabs and an 8-byte aligned query; everything else runs the generic kernel.
+ * Workspace: fa_paged_decode_kv8_workspace_size bytes, under the rules of
+ * fa_paged_attention_workspace_size (it may be the same buffer). */
+FA_API size_t fa_paged_decode_kv8_workspace_size(int32_t num_seqs, int32_t num_heads,
+                                                 int32_t num_kv_heads, int32_t head_dim,
+                                                 int32_t max_context_len);
+FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void *out,
+                                     int32_t dtype, const int32_t *context_lens,
+                                     const int32_t *block_tables, int32_t max_blocks_per_seq,
+                                     int32_t num_seqs, int32_t num_heads, int32_t n_rep,
+                                     int32_t max_context_len, float scale, void *workspace,
+                                     size_t workspace_bytes, fa_stream_t stream);
+
+/* fa_paged_prefill over an 8-bit cache (the suffix tokens already appended). Arguments as there,
+ * and total_blocks, a host-side upper bound of the sum over the sequences of
+ * ceil(context_len / block_size): the tensor-core path (FA_BF16 / FA_F16, block_size 16,
+ * head_dim 128, at most 2048 sequences, scale > 0, 16-byte aligned query, 32-byte aligned out)
+ * turns those blocks into the query type in the workspace first, in one launch. Sequences that no
+ * longer fit total_blocks give zeros and FA_DEVERR_CONTEXT. Other shapes, and total_blocks 0, run
+ * the generic kernel, which needs no workspace. One new token per sequence (max_seqlen_q 1,
+ * total_q == num_seqs) is fa_paged_decode_kv8. Output rows behind cu_seqlens_q[num_seqs] are not
+ * written by the tensor-core path. */
+FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads,
+                                                  int32_t num_kv_heads, int32_t head_dim,
+                                                  int32_t max_context_len, int32_t max_seqlen_q,
+                                                  int32_t total_blocks);
+FA_API fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, void *out,
+                                      int32_t dtype, const int32_t *cu_seqlens_q,
+                                      const int32_t *context_lens, const int32_t *block_tables,
+                                      int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_heads,
+                                      int32_t n_rep, int32_t total_q, int32_t max_seqlen_q,
+                                      int32_t max_context_len, int32_t total_blocks, float scale,
+                                      void *workspace, size_t workspace_bytes, fa_stream_t stream);
+
 /* ---- the steps either side of attention (CausalSelfAttention::forward) ----------------- */
 
 /* Weights of one layer's q/k/v projections, as candle's Linear stores them (out, in). */
@@ -347,6 +444,30 @@ FA_API fa_status fa_last_token_logits(const void *hidden, const int32_t *cu_seql
                                       int32_t hidden_size, int32_t vocab, int32_t dtype,
                                       void *normed_out, float *logits_out, fa_stream_t stream);
 
+/* Log probabilities of given tokens, with entropy and top alternatives, from logits rows such as
+ * fa_last_token_logits writes: the `logprobs` / `top_logprobs` of an answer, the scoring of given
+ * text, and the way to see what an 8-bit cache costs. No counterpart in the reference, whose
+ * engine hands logits to a host sampler (engine.rs:220-222).
+ *   logits        device, row r at r * row_stride elements of `dtype` (an fa_dtype), vocab logits
+ *                 each; row_stride >= vocab, any alignment of the element type
+ *   token_ids     device int32 [num_rows] or NULL; -1: no token (its log probability reads 0)
+ *   logprobs_out  f32 [num_rows], ln p(token); given exactly when token_ids is
+ *   entropy_out   f32 [num_rows] or NULL: -sum p ln p, in nats
+ *   top_k         0 .. FA_MAX_TOP_LOGPROBS
+ *   top_ids_out / top_logprobs_out  [num_rows, top_k] int32 / f32: the tokens of highest logit,
+ *                 highest first, ties to the lower id
+ * A logit of -inf is a token that a mask took out: probability 0, log probability -inf, never
+ * among the alternatives; missing alternatives are id -1 with -inf. A row of nothing else gives
+ * -inf for any token, entropy 0 and no alternatives. A NaN or +inf logit makes the row's results
+ * NaN, its ids -1. A token id outside [-1, vocab) gives NaN and FA_DEVERR_TOKEN. Sums in f32.
+ * Results do not depend on the other rows of the call, other than through how many CTAs share a
+ * row (the order of the f32 sums). No workspace. */
+#define FA_MAX_TOP_LOGPROBS 32
+FA_API fa_status fa_token_logprobs(const void *logits, int32_t dtype, int64_t row_stride,
+                                   int32_t num_rows, int32_t vocab, const int32_t *token_ids,
+                                   float *logprobs_out, float *entropy_out, int32_t top_k,
+                                   int32_t *top_ids_out, float *top_logprobs_out, fa_stream_t stream);
+
 /* Width in output columns of the tiles the projection GEMMs above use for an M x N x K problem
  * (128 or 256; 128 when K is split over a thread-block cluster), as chosen on the current device.
  * A reporting aid: the choice depends only on the shape and the device's SM count. No
@@ -357,8 +478,8 @@ FA_API int32_t fa_gemm_tile_width(int32_t M, int32_t N, int32_t K);
  * launched with programmatic stream serialization: each may start its prologue and request its
  * first weight tiles while the preceding kernel on the stream finishes, and waits for that
  * kernel's completion before it reads activations or writes outputs. So are the decode kernels,
- * fa_tp_sync, fa_reshape_and_cache and fa_paged_prefill, which set up only on-chip state before
- * that wait. For a caller this changes nothing: stream order holds for every call. */
+ * fa_tp_sync, fa_reshape_and_cache, fa_paged_prefill, the 8-bit cache's entry points and
+ * fa_token_logprobs, which set up only on-chip state before that wait. For a caller this changes nothing: stream order holds for every call. */
 
 /* ---- head-sharded decode (tensor parallel over KV heads, one process per GPU) ----------
  * The reference runs attention on one CPU and has no sharding (its plan shards sequences,

@@ -1,0 +1,487 @@
+"""The 8-bit KV cache on the GPU: append, decode and prefill against plain 64-bit forms.
+
+The append is compared code by code: its scales are powers of two, so every quotient is exact and
+there is one right answer. Attention is held to the element-wise bound of _kv8.attention_ref plus
+half a step of the output type."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from flour_b200 import FlourAttnError, _lib, ops
+
+import _kv8
+from _kv8 import FMTS, append_ref, assert_close, attention_ref, inv_sqrt, make_tables, random_pool
+
+pytestmark = pytest.mark.gpu
+
+U16 = 2.0 ** -11  # half a step of f16, relative: how the decode rounds probabilities
+
+
+def gen_of(device, seed):
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return g
+
+
+def i32(x, device):
+    return torch.as_tensor(np.asarray(x, dtype=np.int32), device=device)
+
+
+def run_append(pool, key, value, bt, ctx, new, device, one=False, **kw):
+    cu = None if one else i32(np.concatenate([[0], np.cumsum(new)]), device)
+    ops.paged_append_kv8(*pool, key, value, i32(bt, device), i32(ctx, device), cu, **kw)
+
+
+def check_append(pool, before, key, value, bt, ctx, new):
+    """pool after the call against append_ref on `before` (clones from before the call)."""
+    for c, s, c0, s0, x in ((pool[0], pool[2], before[0], before[2], key),
+                            (pool[1], pool[3], before[1], before[3], value)):
+        raw = c0.view(torch.uint8).cpu().numpy().copy()
+        sc = s0.cpu().numpy().copy()
+        append_ref(raw, sc, c.dtype, x.double().cpu().numpy(), bt, ctx, new)
+        np.testing.assert_array_equal(s.cpu().numpy(), sc)
+        got = c.view(torch.uint8).cpu().numpy()
+        if c.dtype == torch.float8_e4m3fn:  # NaN's sign is not pinned
+            raw, got = [np.where((a & 0x7F) == 0x7F, 0x7F, a) for a in (raw, got)]
+        np.testing.assert_array_equal(got, raw)
+
+
+def clone(pool):
+    return [t.clone() for t in pool]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads, d, bs", [(8, 128, 16), (2, 64, 16), (3, 40, 16), (4, 128, 8), (1, 256, 32),
+                                          (5, 6, 4)])
+def test_append_prompts(device, fmt, dtype, heads, d, bs):
+    ctx, new = [1, 15, 16, 17, 33, 200, 64, 5], [1, 15, 16, 1, 18, 200, 16, 0]
+    bt, nb = make_tables(ctx, bs, 1)
+    g = gen_of(device, 2)
+    pool = random_pool(nb, heads, bs, d, fmt, g, device)
+    T = sum(new)
+    key = (torch.randn((T, heads, d), device=device, generator=g) * 3).to(dtype)
+    value = torch.randn((T, heads, d), device=device, generator=g).to(dtype)
+    before = clone(pool)
+    run_append(pool, key, value, bt, ctx, new, device)
+    check_append(pool, before, key, value, bt, ctx, new)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads, d", [(4, 128), (2, 64), (3, 24)])
+def test_append_token_by_token_grows_the_scale(device, fmt, heads, d):
+    # 40 steps of one token each, louder and quieter in turns, starting on reused blocks.
+    S = 3
+    bt, nb = make_tables([48] * S, 16, 3)
+    g = gen_of(device, 4)
+    pool = random_pool(nb, heads, 16, d, fmt, g, device)
+    one = True
+    for step in range(40):
+        ctx = [step + 1, step + 5, step + 8]
+        loud = 2.0 ** ((step * 7) % 11 - 5)
+        key = (torch.randn((S, heads, d), device=device, generator=g) * loud).to(torch.bfloat16)
+        value = torch.zeros_like(key) if step == 16 else key.flip(0).contiguous()
+        before = clone(pool)
+        run_append(pool, key, value, bt, ctx, [1] * S, device, one=one)
+        check_append(pool, before, key, value, bt, ctx, [1] * S)
+        one = not one  # the one-token and the varlen form in turns
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_append_values_at_the_borders(device, fmt):
+    # Largest codes exactly, halfway cases, the floor of the scale, f32 extremes, zeros.
+    d = 128
+    top = _kv8.QMAX[fmt]
+    rows = [torch.full((d,), top), torch.full((d,), math.nextafter(top, math.inf) * (1 + 1e-6)),
+            torch.linspace(-top, top, d), torch.arange(d) + 0.5, torch.zeros(d), torch.full((d,), 1e-45),
+            torch.full((d,), 3.4e38), torch.full((d,), -1.2e-38),
+            torch.tensor([0.0009765625 * (i + 1) for i in range(d)])]
+    x = torch.stack([r.float() for r in rows])[:, None, :].to(device)
+    T = len(rows)
+    for new, ctx in (([T], [T]), ([1] * T, list(range(1, T + 1)))):
+        bt, nb = make_tables(ctx, 16, 5)
+        pool = random_pool(nb, 1, 16, d, fmt, gen_of(device, 6), device)
+        before = clone(pool)
+        run_append(pool, x, -x, bt, ctx, new, device)
+        check_append(pool, before, x, -x, bt, ctx, new)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_append_nonfinite_values_are_reported_and_do_not_set_the_scale(device, fmt):
+    bt, nb = make_tables([20], 16, 7)
+    g = gen_of(device, 8)
+    pool = random_pool(nb, 2, 16, 64, fmt, g, device)
+    key = torch.randn((20, 2, 64), device=device, generator=g).to(torch.bfloat16)
+    value = key.clone()
+    key[3, 0, 5], key[4, 1, 6], key[17, 0, 0] = math.inf, math.nan, -math.inf
+    key[18:, 1] = math.nan
+    before = clone(pool)
+    ops.device_status()
+    run_append(pool, key, value, bt, [20], [20], device)
+    assert ops.device_status() == _lib.FA_DEVERR_VALUE
+    check_append(pool, before, key, value, bt, [20], [20])
+
+
+def test_append_strides(device):
+    # The (1, Hkv, n, d) layout (token stride d, head stride n d) and a slice of fused qkv rows.
+    g = gen_of(device, 9)
+    n, H, d = 37, 4, 128
+    bt, nb = make_tables([n], 16, 10)
+    qkv = torch.randn((n, 8 + 2 * H, d), device=device, generator=g).to(torch.bfloat16)
+    key, value = qkv[:, 8:8 + H], torch.randn((H, n, d), device=device, generator=g).to(torch.bfloat16).transpose(0, 1)
+    odd = torch.randn((n * H * d + 1,), device=device, generator=g).to(torch.bfloat16)[1:].view(n, H, d)
+    for k, v in ((key, value), (odd, key)):  # `odd` starts 2 bytes past an aligned address
+        pool = random_pool(nb, H, 16, d, torch.int8, g, device)
+        before = clone(pool)
+        run_append(pool, k, v, bt, [n], [n], device)
+        check_append(pool, before, k, v, bt, [n], [n])
+
+
+def test_append_leaves_everything_else_alone(device):
+    # Bad lengths, bad ids, padded rows behind the last sequence, an empty batch.
+    g = gen_of(device, 11)
+    ctx, new = [10, 4, 30, 12], [10, 5, 8, 12]   # sequence 1: more new tokens than its length
+    bt, nb = make_tables([16, 16, 32, 16], 16, 12)
+    bt[2, 1] = nb + 5                             # sequence 2's second block
+    pool = random_pool(nb, 2, 16, 64, torch.float8_e4m3fn, g, device)
+    key = torch.randn((sum(new) + 9, 2, 64), device=device, generator=g).to(torch.float16)
+    key[sum(new):] = math.nan                     # padding
+    before = clone(pool)
+    ops.device_status()
+    run_append(pool, key, key, bt, ctx, new, device)
+    assert ops.device_status() == _lib.FA_DEVERR_CONTEXT | _lib.FA_DEVERR_BLOCK_ID
+    for c, s, c0, s0 in ((pool[0], pool[2], before[0], before[2]), (pool[1], pool[3], before[1], before[3])):
+        raw, sc = c0.view(torch.uint8).cpu().numpy().copy(), s0.cpu().numpy().copy()
+        x = key.double().cpu().numpy()
+        append_ref(raw, sc, c.dtype, x[:10], bt[:1], [10], [10])
+        append_ref(raw, sc, c.dtype, x[23:35], bt[3:], [12], [12])
+        np.testing.assert_array_equal(s.cpu().numpy(), sc)
+        np.testing.assert_array_equal(c.view(torch.uint8).cpu().numpy(), raw)
+    run_append(pool, key[:0], key[:0], bt, ctx, [0, 0, 0, 0], device)
+    assert ops.device_status() == 0
+    # A cu_seqlens entry past the packed tokens is reported, and nothing of that sequence written.
+    after = clone(pool)
+    ops.paged_append_kv8(*pool, key[:8], key[:8], i32(bt[:2], device), i32([10, 20], device),
+                         i32([0, 4, 11], device))
+    assert ops.device_status() == _lib.FA_DEVERR_SEQLEN
+    assert torch.equal(pool[2][int(bt[1, 0])], after[2][int(bt[1, 0])])
+
+
+def decode_case(device, fmt, dtype, Hq, Hkv, d, ctx, seed, bs=16, q_scale=1.0, kernel_u=U16):
+    bt, nb = make_tables(ctx, bs, seed)
+    g = gen_of(device, seed)
+    pool = random_pool(nb, Hkv, bs, d, fmt, g, device)
+    q = (torch.randn((len(ctx), Hq, d), device=device, generator=g) * q_scale).to(dtype)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [1] * len(ctx),
+                              Hq // Hkv, inv_sqrt(d), kernel_u)
+    return pool, q, i32(bt, device), i32(ctx, device), want, tol
+
+
+def run_decode(pool, q, bt, cl, ctx, Hkv, ws=None, **kw):
+    return ops.paged_decode_kv8(q, *pool, bt, cl, q.shape[1] // Hkv, inv_sqrt(q.shape[2]), int(max(ctx)),
+                                ws or ops.Workspace(), **kw)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq, Hkv, d", [(32, 8, 128), (28, 4, 128), (14, 2, 64), (8, 8, 128), (8, 1, 64)])
+@pytest.mark.parametrize("ctx", [[1], [15, 16, 17, 31, 32, 33], [511, 2, 1200, 513]])
+def test_decode(device, fmt, dtype, Hq, Hkv, d, ctx):
+    pool, q, bt, cl, want, tol = decode_case(device, fmt, dtype, Hq, Hkv, d, ctx, 20)
+    assert_close(run_decode(pool, q, bt, cl, ctx, Hkv), want, tol)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype, Hq, Hkv, d, bs", [
+    (torch.float32, 8, 2, 128, 16), (torch.float32, 14, 2, 64, 16), (torch.bfloat16, 16, 1, 128, 16),
+    (torch.float16, 6, 3, 96, 8), (torch.float32, 4, 4, 6, 4), (torch.bfloat16, 4, 2, 256, 32)])
+def test_decode_other_shapes(device, fmt, dtype, Hq, Hkv, d, bs):
+    ctx = [1, bs, bs + 1, 300]
+    pool, q, bt, cl, want, tol = decode_case(device, fmt, dtype, Hq, Hkv, d, ctx, 21, bs=bs, kernel_u=0.0)
+    assert_close(run_decode(pool, q, bt, cl, ctx, Hkv), want, tol)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_decode_long_context_splits(device, fmt):
+    ctx = [9001, 4097, 12345]
+    pool, q, bt, cl, want, tol = decode_case(device, fmt, torch.bfloat16, 8, 2, 128, ctx, 22)
+    ws = ops.Workspace()
+    out = run_decode(pool, q, bt, cl, ctx, 2, ws)
+    assert_close(out, want, tol)
+    assert torch.equal(out, run_decode(pool, q, bt, cl, ctx, 2, ws))
+
+
+def test_decode_scales_that_differ_from_page_to_page(device):
+    # Scales over 2^+-24 that are not powers of two: accumulators of neighbouring pages differ.
+    ctx = [400, 37]
+    pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, ctx, 23)
+    g = gen_of(device, 24)
+    pool = (pool[0], pool[1], pool[2] * 1.37, torch.exp2(torch.rand_like(pool[3]) * 48 - 24))
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, bt, ctx, [1, 1], 4, inv_sqrt(128), U16)
+    assert_close(run_decode(pool, q, bt, cl, ctx, 2), want, tol)
+
+
+@pytest.mark.parametrize("q_scale", [2.0 ** -60, 2.0 ** 40, 0.0])
+def test_decode_queries_outside_f16(device, q_scale):
+    ctx = [100]
+    bt, nb = make_tables(ctx, 16, 25)
+    pool = random_pool(nb, 2, 16, 64, torch.float8_e4m3fn, gen_of(device, 25), device)
+    pool = (pool[0], pool[1], pool[2] / (q_scale or 1.0), pool[3])
+    q = (torch.randn((1, 4, 64), device=device, generator=gen_of(device, 26)) * q_scale).to(torch.bfloat16)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [1], 2, inv_sqrt(64), U16)
+    assert_close(run_decode(pool, q, i32(bt, device), i32(ctx, device), ctx, 2), want, tol)
+
+
+def poison_tails(pool, bt, ctx):
+    """NaN codes behind each sequence's last token, NaN scales in blocks nobody holds."""
+    bs = pool[0].shape[2]
+    used = set()
+    for s, L in enumerate(ctx):
+        n = (L + bs - 1) // bs
+        used |= {int(b) for b in bt[s, :n]}
+        if L % bs:
+            for c in pool[:2]:
+                c.view(torch.uint8)[int(bt[s, n - 1]), :, L % bs:] = 0x7F
+    for b in set(range(pool[0].shape[0])) - used:
+        pool[2][b] = math.nan
+        pool[3][b] = math.nan
+
+
+@pytest.mark.parametrize("Hq, Hkv, d, dtype", [(32, 8, 128, torch.bfloat16), (14, 2, 64, torch.float16),
+                                               (4, 2, 96, torch.float32)])
+def test_stale_nan_behind_the_context_is_not_seen(device, Hq, Hkv, d, dtype):
+    ctx, new = [1, 17, 47, 130, 16], [1, 2, 30, 130, 5]
+    bt, nb = make_tables(ctx, 16, 27)
+    g = gen_of(device, 27)
+    pool = random_pool(nb, Hkv, 16, d, torch.float8_e4m3fn, g, device)
+    poison_tails(pool, bt, ctx)
+    q = torch.randn((sum(new), Hq, d), device=device, generator=g).to(dtype)
+    first = np.cumsum([0] + new[:-1])
+    want, tol = attention_ref(q.double().cpu().numpy()[first], pool, torch.as_tensor(bt), ctx, [1] * 5,
+                              Hq // Hkv, inv_sqrt(d), U16)
+    assert_close(run_decode(pool, q[first].contiguous(), i32(bt, device), i32(ctx, device), ctx, Hkv), want, tol)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, Hq // Hkv,
+                              inv_sqrt(d), 2.0 ** -8)
+    assert_close(run_prefill(pool, q, bt, ctx, new, Hkv, device), want, tol)
+    assert ops.device_status() == 0
+
+
+def run_prefill(pool, q, bt, ctx, new, Hkv, device, ws=None, slack=0, **kw):
+    bs = pool[0].shape[2]
+    cu = i32(np.concatenate([[0], np.cumsum(new)]), device)
+    blocks = sum((c + bs - 1) // bs for c in ctx) + slack
+    return ops.paged_prefill_kv8(q, *pool, cu, i32(ctx, device), i32(bt, device), q.shape[1] // Hkv,
+                                 inv_sqrt(q.shape[2]), int(max(new)), int(max(ctx)), blocks,
+                                 ws or ops.Workspace(), **kw)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hq, Hkv, d", [(8, 2, 128), (7, 1, 128), (14, 2, 64)])
+@pytest.mark.parametrize("ctx, new", [
+    ([300, 90, 257], [236, 90, 129]),       # cached prefixes, ragged ends
+    ([1], [1]),                             # one token (the decode)
+    ([40, 700], [0, 3]),                    # fewer rows than one query tile; an empty sequence
+    ([64, 1, 33, 500], [1, 1, 1, 1]),       # one each
+    ([129], [128]),
+])
+def test_prefill(device, fmt, dtype, Hq, Hkv, d, ctx, new):
+    bt, nb = make_tables(ctx, 16, 30)
+    g = gen_of(device, 30)
+    pool = random_pool(nb, Hkv, 16, d, fmt, g, device)
+    q = torch.randn((sum(new), Hq, d), device=device, generator=g).to(dtype)
+    # bf16 prompts round probabilities to bf16 (half a step: 2^-8)
+    u = 0.0 if dtype == torch.float32 else (2.0 ** -8 if dtype == torch.bfloat16 else U16)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, Hq // Hkv,
+                              inv_sqrt(d), u)
+    assert_close(run_prefill(pool, q, bt, ctx, new, Hkv, device, slack=5), want, tol)
+    assert ops.device_status() == 0
+
+
+def test_prefill_equals_the_16_bit_prefill_of_the_same_values(device):
+    # Power-of-two scales make the bf16 copy exact, so both prefills see one cache.
+    ctx, new = [400, 129, 1000], [400, 60, 513]
+    bt, nb = make_tables(ctx, 16, 31)
+    g = gen_of(device, 31)
+    for fmt in FMTS:
+        pool = random_pool(nb, 8, 16, 128, fmt, g, device)
+        q = torch.randn((sum(new), 32, 128), device=device, generator=g).to(torch.bfloat16)
+        out = run_prefill(pool, q, bt, ctx, new, 8, device)
+        kc, vc = [(c.float() * s[:, :, None, None]).to(torch.bfloat16) for c, s in zip(pool[:2], pool[2:])]
+        cu = i32(np.concatenate([[0], np.cumsum(new)]), device)
+        want = ops.paged_prefill(q, kc, vc, cu, i32(ctx, device), i32(bt, device), 4, inv_sqrt(128),
+                                 max(new), max(ctx), ops.Workspace())
+        assert torch.equal(out, want)
+
+
+def test_prefill_refuses_sequences_past_total_blocks(device):
+    ctx = [64, 200, 32]
+    bt, nb = make_tables(ctx, 16, 32)
+    g = gen_of(device, 32)
+    pool = random_pool(nb, 2, 16, 128, torch.int8, g, device)
+    q = torch.randn((sum(ctx), 8, 128), device=device, generator=g).to(torch.bfloat16)
+    want = run_prefill(pool, q, bt, ctx, ctx, 2, device)
+    ops.device_status()
+    out = run_prefill(pool, q, bt, ctx, ctx, 2, device, slack=-3)
+    assert ops.device_status() == _lib.FA_DEVERR_CONTEXT
+    # 4 + 13 + 2 pages against 16 blocks: the first sequence fits, packing ends at the second.
+    assert torch.equal(out[:64], want[:64])
+    assert not out[64:].any()
+
+
+def test_prefill_rows_behind_the_last_sequence_stay(device):
+    ctx = [100, 60]
+    bt, nb = make_tables(ctx, 16, 33)
+    g = gen_of(device, 33)
+    pool = random_pool(nb, 2, 16, 128, torch.float8_e4m3fn, g, device)
+    q = torch.randn((200, 8, 128), device=device, generator=g).to(torch.bfloat16)
+    q[160:] = math.nan
+    out = torch.full_like(q, 7.0)
+    run_prefill(pool, q, bt, ctx, ctx, 2, device, out=out)
+    assert (out[160:] == 7.0).all()
+    want, tol = attention_ref(q[:160].double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, ctx, 4,
+                              inv_sqrt(128), 2.0 ** -8)
+    assert_close(out[:160], want, tol)
+
+
+def test_bad_lengths_and_ids_are_reported(device):
+    ctx = [40, 50]
+    pool, q, bt, cl, want, tol = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, ctx, 34)
+    ops.device_status()
+    out = run_decode(pool, q, bt, i32([0, 50], device), ctx, 2)
+    assert ops.device_status() == _lib.FA_DEVERR_CONTEXT
+    assert not out[0].any()
+    assert_close(out[1:], want[1:], tol[1:])
+    bad = bt.clone()
+    bad[0, 1] = -3
+    run_decode(pool, q, bad, cl, ctx, 2)
+    assert ops.device_status() == _lib.FA_DEVERR_BLOCK_ID
+    q2 = q.repeat_interleave(20, 0)
+    run_prefill(pool, q2, bad.cpu().numpy(), ctx, [20, 20], 2, device)
+    assert ops.device_status() == _lib.FA_DEVERR_BLOCK_ID
+
+
+def test_one_workspace_two_graphs_and_other_calls(device):
+    # A decode and a prefill captured on one workspace, replayed between eager calls of other sizes.
+    ctx, new = [3000, 2500], [200, 100]
+    pool, q, bt, cl, want, tol = decode_case(device, torch.float8_e4m3fn, torch.bfloat16, 8, 2, 128, ctx, 35)
+    big_ctx = [600] * 40
+    bpool, bq, bbt, bcl, bwant, btol = decode_case(device, torch.int8, torch.bfloat16, 32, 8, 128, big_ctx, 36)
+    qp = torch.randn((sum(new), 8, 128), device=device, generator=gen_of(device, 37)).to(torch.bfloat16)
+    ws = ops.Workspace()
+    ws.get(64 << 20)
+    want_p = run_prefill(pool, qp, bt.cpu().numpy(), ctx, new, 2, device)
+    cu, blocks = i32([0, 200, 300], device), sum((c + 15) // 16 for c in ctx)
+    out_d, out_p = torch.empty_like(q), torch.empty_like(qp)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    with torch.cuda.graph(graphs[0], stream=s):
+        run_decode(pool, q, bt, cl, ctx, 2, ws, out=out_d)
+    with torch.cuda.graph(graphs[1], stream=s):
+        ops.paged_prefill_kv8(qp, *pool, cu, cl, bt, 4, inv_sqrt(128), 200, 3000, blocks, ws, out=out_p)
+    for _ in range(2):
+        for order in ((0, 1), (1, 0)):
+            for i in order:
+                out_d.zero_()
+                out_p.zero_()
+                graphs[i].replay()
+                if i == 0:
+                    assert_close(out_d, want, tol)
+                else:
+                    assert torch.equal(out_p, want_p)
+            assert_close(run_decode(bpool, bq, bbt, bcl, big_ctx, 8, ws), bwant, btol)
+    del graphs
+    assert ops.device_status() == 0
+
+
+def test_side_stream_and_append_then_decode_chain(device):
+    # One step as a server runs it: prompts appended and attended, then 20 tokens one by one,
+    # all on a side stream, against the plain forms on the same codes.
+    H, Hq, d = 2, 8, 128
+    lens = [37, 5, 64]
+    bt, nb = make_tables([c + 20 for c in lens], 16, 40)
+    for fmt in FMTS:
+        g = gen_of(device, 41)
+        pool = random_pool(nb, H, 16, d, fmt, g, device)
+        ws = ops.Workspace()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            k, v = (torch.randn((sum(lens), H, d), device=device, generator=g).to(torch.bfloat16) for _ in "kv")
+            q = torch.randn((sum(lens), Hq, d), device=device, generator=g).to(torch.bfloat16)
+            run_append(pool, k, v, bt, lens, lens, device)
+            out = run_prefill(pool, q, bt, lens, lens, H, device, ws=ws)
+        side.synchronize()
+        want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), lens, lens, 4,
+                                  inv_sqrt(d), 2.0 ** -8)
+        assert_close(out, want, tol)
+        ctx = list(lens)
+        for _ in range(20):
+            ctx = [c + 1 for c in ctx]
+            with torch.cuda.stream(side):
+                k, v = (torch.randn((3, H, d), device=device, generator=g).to(torch.bfloat16) for _ in "kv")
+                q = torch.randn((3, Hq, d), device=device, generator=g).to(torch.bfloat16)
+                run_append(pool, k, v, bt, ctx, [1] * 3, device, one=True)
+                out = run_decode(pool, q, i32(bt, device), i32(ctx, device), ctx, H, ws)
+            side.synchronize()
+            want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [1] * 3, 4,
+                                      inv_sqrt(d), U16)
+            assert_close(out, want, tol)
+        assert ops.device_status() == 0
+
+
+def test_blocks_are_copied_with_their_scales(device):
+    # Copy-on-write of an 8-bit block with fa_copy_blocks: slabs as bf16 of half the head_dim,
+    # scales as f32 layers of one element.
+    pool = random_pool(12, 2, 16, 128, torch.float8_e4m3fn, gen_of(device, 42), device)
+    before = clone(pool)
+    pairs = i32([[3, 7], [0, 11]], device)
+    half = [c.view(torch.bfloat16) for c in pool[:2]]
+    ops.copy_blocks([half[0]], [half[1]], pairs)
+    ops.copy_blocks([pool[2][:, :, None, None]], [pool[3][:, :, None, None]], pairs)
+    for now, was in zip(pool, before):
+        now, was = [t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (now, was)]
+        assert torch.equal(now[7], was[3]) and torch.equal(now[11], was[0])
+        assert torch.equal(now[:7], was[:7])
+
+
+def test_refusals(device):
+    ctx = [40, 50]
+    pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, ctx, 43)
+    ws = ops.Workspace()
+    k = torch.zeros((2, 2, 128), device=device, dtype=torch.bfloat16)
+    bad = [
+        lambda: ops.paged_decode_kv8(q, *pool, bt, cl, 3, 0.1, 50, ws),                       # n_rep
+        lambda: ops.paged_decode_kv8(q, *pool, bt, cl, 4, 0.1, 65, ws),                       # table too short
+        lambda: ops.paged_decode_kv8(q, *pool, bt, cl, 4, math.nan, 50, ws),
+        lambda: ops.paged_decode_kv8(q[:, :, :64], *pool, bt, cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q.double(), *pool, bt, cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q.cpu(), *pool, bt, cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q, *pool, bt.long(), cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q, *pool, bt[:1], cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q, pool[0], pool[1], pool[2].double(), pool[3], bt, cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q, pool[0].view(torch.uint8), *pool[1:], bt, cl, 4, 0.1, 50, ws),
+        lambda: ops.paged_decode_kv8(q, *pool, bt, cl, 4, 0.1, 50, ws, out=q[:1]),
+        lambda: ops.paged_append_kv8(*pool, k, k[:1], bt, cl),
+        lambda: ops.paged_append_kv8(*pool, k[:1], k[:1], bt, cl),
+        lambda: ops.paged_append_kv8(*pool, k, k, bt, cl, i32([0, 1], device)),
+        lambda: ops.paged_append_kv8(*pool, k.transpose(1, 2), k.transpose(1, 2), bt, cl),
+        lambda: ops.paged_prefill_kv8(q, *pool, i32([0, 1], device), cl, bt, 4, 0.1, 1, 50, 9, ws),
+        lambda: ops.paged_prefill_kv8(q, *pool, i32([0, 1, 2], device), cl, bt, 4, 0.1, 60, 50, 9, ws),
+        lambda: ops.paged_prefill_kv8(q, *pool, i32([0, 0, 2], device), cl, bt, 4, 0.1, 2, 50, -1, ws),
+        lambda: ops.paged_prefill_kv8(q, *pool, i32([0, 0, 2], device), cl, bt, 4, 0.1, 2, 50, 9, None),
+    ]
+    for call in bad:
+        with pytest.raises(FlourAttnError):
+            call()
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
