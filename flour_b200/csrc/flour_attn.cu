@@ -963,6 +963,34 @@ fa_status launch_generic8(const fa_kv8_layer *L, const void *q, void *out, int32
   });
 }
 
+// ---- log probabilities ------------------------------------------------------------------------
+
+constexpr int kLpPartTile = fa::kLpPartThreads * fa::kLpPartLogits;
+constexpr int kLpPartCtasPerSm = 12;
+constexpr int kLpSmallTile = fa::kLpSmallThreads * fa::kLpPartLogits;
+
+template <typename T>
+fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t stream, const char *who) {
+  // 15 more logits: a row that does not start on 16 bytes fills its first vector partly.
+  const int64_t span = int64_t(p.vocab) + 15;
+  if (span <= kLpSmallTile)
+    return launch_pdl(who, fa::logprobs_part_kernel<T, fa::kLpSmallThreads>, dim3(unsigned(rows)),
+                      fa::kLpSmallThreads, 0, stream, 1, p);
+  const int64_t ranks = (span + kLpPartTile - 1) / kLpPartTile;
+  if (ranks <= fa::kLpMaxCluster && rows * ranks <= kLpPartCtasPerSm * int64_t(sm_count())) {
+    auto kern = fa::logprobs_part_kernel<T, fa::kLpPartThreads>;
+    if (ranks > 8) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return fail(FA_ECUDA, "%s: cluster attribute: %s", who, cudaGetErrorString(e));
+    }
+    return launch_pdl(who, kern, dim3(unsigned(rows * ranks)), fa::kLpPartThreads, 0, stream, int(ranks), p);
+  }
+  int split = 1;  // few rows too long for registers
+  while (split < 8 && int64_t(rows) * split * 2 <= int64_t(sm_count()) * 3) split *= 2;
+  return launch_pdl(who, fa::logprobs_stream_kernel<T>, dim3(unsigned(rows * split)), fa::kLpStreamThreads, 0,
+                    stream, split, p);
+}
+
 // Whether the tcgen05 prefill serves a call, over a copy of the cache in the query type.
 bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float scale, const void *q,
                         const void *out, int num_seqs, int32_t total_blocks) {
@@ -1581,9 +1609,19 @@ fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const 
     grid = dim3(unsigned((total_q + fa::kAppendChunk - 1) / fa::kAppendChunk),
                 unsigned((per_run + fa::kAppendWarps - 1) / fa::kAppendWarps));
   }
+  // The vector form reads rows of 16 bytes and writes 8.
+  const int per16 = 16 / dtype_size(dtype);
+  const bool vec = layer->block_size == 16 && (layer->head_dim == 64 || layer->head_dim == 128) &&
+                   aligned(key, 16) && aligned(value, 16) && key_stride_token % per16 == 0 &&
+                   key_stride_head % per16 == 0 && value_stride_token % per16 == 0 &&
+                   value_stride_head % per16 == 0 && aligned(layer->k_cache, 8) && aligned(layer->v_cache, 8);
   return with_types8(dtype, layer->dtype, [&](auto t, auto f) {
-    return launch_pdl(who, fa::kv8_append_kernel<decltype(t), decltype(f)>, grid, fa::kAppendThreads, 0,
-                      reinterpret_cast<cudaStream_t>(stream), 1, p);
+    using T = decltype(t);
+    using F = decltype(f);
+    auto kern = !vec                    ? fa::kv8_append_kernel<T, F, 0>
+                : layer->head_dim == 64 ? fa::kv8_append_kernel<T, F, 64>
+                                        : fa::kv8_append_kernel<T, F, 128>;
+    return launch_pdl(who, kern, grid, fa::kAppendThreads, 0, reinterpret_cast<cudaStream_t>(stream), 1, p);
   });
 }
 
@@ -1694,20 +1732,11 @@ fa_status fa_token_logprobs(const void *logits, int32_t dtype, int64_t row_strid
   p.top_logprobs = top_logprobs_out;
   p.vocab = vocab;
   p.top_k = top_k;
-  // CTAs per row: as many as fill the GPU, each with a tile of the row or more.
-  int ranks = 1;
-  while (ranks < fa::kLpMaxCluster && int64_t(num_rows) * ranks * 2 <= int64_t(sm_count()) * 4 &&
-         vocab / (ranks * 2) >= fa::kLpThreads * fa::kLpTile / 2)
-    ranks *= 2;
-  const dim3 grid(unsigned(num_rows * ranks));
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case FA_F32:
-      return launch_pdl(who, fa::token_logprobs_kernel<float>, grid, fa::kLpThreads, 0, st, ranks, p);
-    case FA_BF16:
-      return launch_pdl(who, fa::token_logprobs_kernel<__nv_bfloat16>, grid, fa::kLpThreads, 0, st, ranks, p);
-    default:
-      return launch_pdl(who, fa::token_logprobs_kernel<__half>, grid, fa::kLpThreads, 0, st, ranks, p);
+    case FA_F32: return launch_logprobs<float>(p, num_rows, st, who);
+    case FA_BF16: return launch_logprobs<__nv_bfloat16>(p, num_rows, st, who);
+    default: return launch_logprobs<__half>(p, num_rows, st, who);
   }
 }
 

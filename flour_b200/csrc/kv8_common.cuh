@@ -166,6 +166,92 @@ __device__ __forceinline__ bool append_run(const Kv8AppendParams &p, const Kv8Ru
   return bad;
 }
 
+// The same for block_size 16, head_dim D of 64 or 128 and 16-byte aligned rows: the run's rows are
+// loaded at once, 8 values a lane and row (4 KB of bf16 a warp in flight at D = 128), and stay in
+// registers between the maximum and the rounding. Magnitudes are compared as integers, two 16-bit
+// ones an instruction; a run with an infinity or NaN (the largest patterns) takes append_run.
+template <typename T, class F, int D>
+__device__ __forceinline__ bool append_run_vec(const Kv8AppendParams &p, const Kv8Run &r, int h, int kv) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, PASSES = 16 / ROWS, W = sizeof(T) * 2;
+  const int lane = threadIdx.x & 31, row = lane / LANES, col = lane % LANES * 8;
+  const T *x = static_cast<const T *>(p.x[kv]) + int64_t(r.tok0) * p.stride_t[kv] +
+               int64_t(h) * p.stride_h[kv] + col;
+  uint8_t *page = p.cache[kv] + (size_t(r.id) * p.num_kv_heads + h) * (16 * D) + col;
+  float *sc = p.scale[kv] + size_t(r.id) * p.num_kv_heads + h;
+  const float before = *sc;
+  uint32_t v[PASSES][W];  // 8 values of a row
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+#pragma unroll
+    for (int q = 0; q < W / 4; ++q) {
+      uint4 t = make_uint4(0u, 0u, 0u, 0u);
+      if (i * ROWS + row < r.n)
+        t = __ldcs(reinterpret_cast<const uint4 *>(x + int64_t(i * ROWS + row) * p.stride_t[kv]) + q);
+      v[i][4 * q] = t.x;
+      v[i][4 * q + 1] = t.y;
+      v[i][4 * q + 2] = t.z;
+      v[i][4 * q + 3] = t.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      if constexpr (sizeof(T) == 4) mx = max(mx, v[i][q] & 0x7fffffffu);
+      else mx = __vmaxu2(mx, v[i][q] & 0x7fff7fffu);
+    }
+  if constexpr (sizeof(T) == 2) mx = max(mx & 0xffffu, mx >> 16);
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  float amax;
+  bool fin;
+  if constexpr (sizeof(T) == 4) {
+    amax = __uint_as_float(mx);
+    fin = mx < 0x7f800000u;
+  } else {
+    amax = unpack2<T>(mx).x;
+    fin = mx < (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
+  }
+  if (!fin) return append_run<T, F>(p, r, h, kv);
+  float move;
+  const float after = append_scale<F>(amax, before, r.row0 > 0, move), inv = 1.f / after;
+  if (move != 1.f) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int o = i * ROWS + row;
+      if (o < r.row0) {
+        uint2 *at = reinterpret_cast<uint2 *>(page + o * D);
+        uint2 b = *at;
+        uint32_t lo, hi;
+        unpack4<F>(b.x, lo, hi);
+        float2 f0 = f16x2_to_f2(lo), f1 = f16x2_to_f2(hi);
+        b.x = to_bytes2<F>(f0.x * move, f0.y * move) | to_bytes2<F>(f1.x * move, f1.y * move) << 16;
+        unpack4<F>(b.y, lo, hi);
+        f0 = f16x2_to_f2(lo);
+        f1 = f16x2_to_f2(hi);
+        b.y = to_bytes2<F>(f0.x * move, f0.y * move) | to_bytes2<F>(f1.x * move, f1.y * move) << 16;
+        *at = b;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    uint32_t b[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float2 f;
+      if constexpr (sizeof(T) == 4) f = make_float2(__uint_as_float(v[i][2 * q]), __uint_as_float(v[i][2 * q + 1]));
+      else f = unpack2<T>(v[i][q]);
+      b[q] = to_bytes2<F>(f.x * inv, f.y * inv);
+    }
+    if (i * ROWS + row < r.n)
+      *reinterpret_cast<uint2 *>(page + (r.row0 + i * ROWS + row) * D) =
+          make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+  }
+  if (lane == 0) *sc = after;
+  return false;
+}
+
 // Tokens [16 c, 16 c + 16) of the packed batch: the runs that begin there, in `runs` (each token
 // that is its sequence's first or its block's first begins one). Called by the first 16 threads
 // of a warp with `cu` in shared or global memory.
@@ -210,8 +296,13 @@ __device__ __forceinline__ int append_runs(const Kv8AppendParams &p, const int32
 // its warps take (run, head, K | V) units. A run belongs to one warp, so the scale of a block is
 // read, grown and written by one owner, and no order of the warps changes a result.
 // One-token form: a unit is (sequence, head, K | V), with nothing to search.
-template <typename T, class F>
+// D: 64 or 128 for the vector form, 0 for any shape.
+template <typename T, class F, int D>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendParams p) {
+  auto append = [&](const Kv8Run &r, int h, int kv) {
+    if constexpr (D > 0) return append_run_vec<T, F, D>(p, r, h, kv);
+    else return append_run<T, F>(p, r, h, kv);
+  };
   __shared__ Kv8Run runs[kAppendChunk];
   __shared__ int s_n;
   __shared__ int32_t s_cu[kAppendCuSmem];
@@ -235,7 +326,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
       return;
     }
     const Kv8Run r{id, (L - 1) % p.block_size, 1, s};
-    bad = append_run<T, F>(p, r, hk >> 1, hk & 1);
+    bad = append(r, hk >> 1, hk & 1);
   } else {
     const int32_t *cu = p.cu_seqlens_q;
     if (p.num_seqs < kAppendCuSmem) {
@@ -251,7 +342,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     const int units = s_n * per_run;
     for (int u = blockIdx.y * kAppendWarps + warp; u < units; u += gridDim.y * kAppendWarps) {
       const int hk = u % per_run;
-      bad |= append_run<T, F>(p, runs[u / per_run], hk >> 1, hk & 1);
+      bad |= append(runs[u / per_run], hk >> 1, hk & 1);
     }
   }
   if (bad) report(FA_DEVERR_VALUE);

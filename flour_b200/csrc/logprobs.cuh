@@ -5,19 +5,19 @@
 // and the k tokens of highest logit, ties to the lower index. A logit of -inf is a token that a
 // mask took out: it has probability 0, adds nothing, and is not listed.
 //
-// One pass over the row. A row is one cluster of 1 to 8 CTAs (more for few rows), each takes a
-// contiguous part, and rank 0 joins the parts over distributed shared memory: no workspace, no
-// atomics, one launch, and one order of every sum.
+// A row is read once, by one cluster of up to 16 CTAs; rank 0 joins the parts that the others
+// write into its shared memory. No workspace, no atomics between CTAs, one launch, and one order of
+// every sum. Two kernels:
+//   part    each CTA's part of the row fits its registers (32 logits a thread): few rows, where
+//           latency counts;
+//   stream  each CTA walks its part in tiles, the next one's loads in flight: many rows.
 //
-// A thread holds a tile of 32 logits in registers (16-byte loads, all in flight together), then
-// takes the tile's maximum, rescales its running Z and W = sum e^(x - m)(x - m) only where the
-// maximum grew, and adds the tile.
-//
-// Top k. Each warp keeps the best 32 it has seen as sorted 64-bit keys (ordered float bits, then
-// the complement of the index), one to a lane. From the first tile's 32 lane maxima it takes the
-// k-th largest: at least k logits are no smaller, so it bounds the k-th largest from below, and
-// only about 1.5 k of the tile's 1024 logits pass. Passing logits are gathered 32 at a time, sorted
-// and merged across the lanes; the list's k-th key is the bound of the next tile.
+// Top k without sorting the row. Among n groups that cover the logits, at least k maxima, hence at
+// least k logits, are >= the k-th largest group maximum: a lower bound of the k-th largest logit.
+// With 32 groups (lanes of a warp, or half warps of a CTA) one bitonic sort over the lanes of a
+// warp gives it, and of the random logits about 32 ln(32 / (32 - k)) pass, 31 for k = 20. What
+// passes is gathered and sorted as 64-bit keys: the float's bits in order, then the complement of
+// the index.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -26,11 +26,12 @@
 
 namespace fa {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpTile = 32;       // logits per thread and tile
 constexpr int kLpMaxTop = 32;
-constexpr int kLpMaxCluster = 8;
+constexpr int kLpMaxCluster = 16;    // 16 CTAs a cluster is opt-in; 8 without
+constexpr int kLpPartLogits = 32;    // a thread's logits in the part kernel
+constexpr int kLpPartThreads = 512;
+constexpr int kLpSmallThreads = 128; // vocabularies that fit one CTA of this size
+constexpr int kLpStreamThreads = 256;
 
 struct LogprobParams {
   const void *logits;        // row r at r * row_stride elements
@@ -54,10 +55,6 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
   return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-  return __shfl_xor_sync(0xffffffffu, v, m);
-}
-
 // Bitonic sort of one key per lane, largest first.
 __device__ __forceinline__ uint64_t warp_sort(uint64_t v) {
   const int lane = threadIdx.x & 31;
@@ -65,29 +62,14 @@ __device__ __forceinline__ uint64_t warp_sort(uint64_t v) {
   for (int k = 2; k <= 32; k <<= 1) {
 #pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
-      const uint64_t w = shfl_xor64(v, j);
+      const uint64_t w = __shfl_xor_sync(0xffffffffu, v, j);
       const bool larger = ((lane & j) == 0) == ((lane & k) == 0);  // this lane keeps the larger
       v = (v > w) == larger ? v : w;
     }
   }
   return v;
 }
-
-// The 32 largest of two descending lists, descending.
-__device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b) {
-  const int lane = threadIdx.x & 31;
-  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  uint64_t v = a > r ? a : r;  // bitonic
-#pragma unroll
-  for (int j = 16; j > 0; j >>= 1) {
-    const uint64_t w = shfl_xor64(v, j);
-    v = (v > w) == ((lane & j) == 0) ? v : w;
-  }
-  return v;
-}
-
-// Largest 32 floats of a warp (one a lane) in order; used for the first bound alone.
-__device__ __forceinline__ float warp_sort_f(float v) {
+__device__ __forceinline__ float warp_sort(float v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1) {
@@ -101,245 +83,462 @@ __device__ __forceinline__ float warp_sort_f(float v) {
   return v;
 }
 
-// (m, Z, W) of two parts of a row. m = -inf marks a part without a finite logit.
+// The 32 largest of two descending lists, descending.
+__device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b) {
+  const int lane = threadIdx.x & 31;
+  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  uint64_t v = a > r ? a : r;  // bitonic
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const uint64_t w = __shfl_xor_sync(0xffffffffu, v, j);
+    v = (v > w) == ((lane & j) == 0) ? v : w;
+  }
+  return v;
+}
+
+// Two f32 operations an instruction.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// A part of a row: m its largest logit, z = sum e^(x - m), w = sum e^(x - m) (x - m). A part
+// without a finite logit has m = -inf, z = 0. A NaN logit makes z NaN, for good.
 struct LpState {
   float m, z, w;
 };
+
+// e^(x - m') = e^(x - m) e^(m - m'):  z' = c z,  w' = c (w + (m - m') z).
 __device__ __forceinline__ void lp_shift(LpState &a, float m) {
-  // e^(x - m') = e^(x - m) e^(m - m'): Z' = c Z, W' = c (W + (m - m') Z).
   const float d = a.m - m;
   const float c = ex2(d * kLog2e);
   if (a.m != neg_inf()) {
     const float w = c * fmaf(d, a.z, a.w);
     a.z *= c;
-    a.w = c > 0.f ? w : a.z;  // c = 0: nothing is left of the part, and d Z may have overflowed
+    a.w = c > 0.f ? w : a.z;  // c = 0: nothing is left of the part, and d z may have overflowed
   }
   a.m = m;
 }
 __device__ __forceinline__ LpState lp_join(LpState a, LpState b) {
   const float m = fmaxf(a.m, b.m);
-  if (m == neg_inf()) return LpState{m, a.z + b.z, a.w + b.w};
-  lp_shift(a, m);
-  lp_shift(b, m);
+  if (m != neg_inf()) {
+    lp_shift(a, m);
+    lp_shift(b, m);
+  }
   return LpState{m, a.z + b.z, a.w + b.w};
 }
+// Join over the lanes of a warp; both partners of a step add the lower lane's part first, so that
+// every lane ends with the same bits.
+__device__ __forceinline__ LpState lp_warp_join(LpState st) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const LpState b{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.z, o),
+                    __shfl_xor_sync(0xffffffffu, st.w, o)};
+    st = (lane & o) ? lp_join(b, st) : lp_join(st, b);
+  }
+  return st;
+}
+
+// z and w of N logits against m >= all of them (m may be -inf: then nothing but NaN counts).
+template <int N>
+__device__ __forceinline__ void lp_sums(const float (&f)[N], float m, float &z, float &w) {
+  if (m == neg_inf()) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (f[j] != f[j]) z = f[j];
+    return;
+  }
+  const uint64_t nm = f2_pack(-m, -m), l2e = f2_pack(kLog2e, kLog2e);
+  uint64_t za[2] = {0, 0}, wa[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const uint64_t d = f2_add(f2_pack(f[j], f[j + 1]), nm);
+    const float2 s = f2_unpack(f2_mul(d, l2e));
+    const uint64_t e = f2_pack(ex2(s.x), ex2(s.y));
+    za[(j >> 1) & 1] = f2_add(za[(j >> 1) & 1], e);
+    wa[(j >> 1) & 1] = f2_fma(e, d, wa[(j >> 1) & 1]);
+  }
+  const float2 zz = f2_unpack(f2_add(za[0], za[1])), ww = f2_unpack(f2_add(wa[0], wa[1]));
+  float ws = ww.x + ww.y;
+  if (ws != ws) {  // a masked logit's 0 * -inf (or a NaN, which z has seen): once more, with care
+    ws = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = f[j] - m;
+      ws = fmaf(ex2(d * kLog2e), fmaxf(d, -1e30f), ws);
+    }
+  }
+  z += zz.x + zz.y;
+  w += ws;
+}
+
+// A row as 16-byte vectors from the aligned address at or below its start: vector v holds logits
+// v * VE - off and on.
+template <typename T> struct LpRow {
+  static constexpr int VE = 16 / sizeof(T);
+  const T *x;
+  const uint4 *xv;
+  int off, vocab;
+  int64_t nv;
+  __device__ __forceinline__ LpRow(const LogprobParams &p, int64_t row) {
+    x = static_cast<const T *>(p.logits) + row * p.row_stride;
+    off = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    xv = reinterpret_cast<const uint4 *>(x - off);
+    vocab = p.vocab;
+    nv = (int64_t(vocab) + off + VE - 1) / VE;
+  }
+  // Vector v of a part that ends at v1; -inf past it. The row's first and last vectors may hold
+  // its neighbours' logits too and are read element by element.
+  __device__ __forceinline__ uint4 load(int64_t v, int64_t v1) const {
+    const int64_t e0 = v * VE - off;
+    if (v < v1 && e0 >= 0 && e0 + VE <= vocab) return __ldcs(xv + v);
+    alignas(16) T e[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      e[j] = (v < v1 && e0 + j >= 0 && e0 + j < vocab) ? x[e0 + j] : Elem<T>::from_f(neg_inf());
+    return *reinterpret_cast<const uint4 *>(e);
+  }
+  __device__ __forceinline__ int index(int64_t v) const { return int(v * VE - off); }
+};
+
+template <typename T, int NV>
+__device__ __forceinline__ void lp_floats(const uint4 (&raw)[NV], float (&f)[NV * 16 / sizeof(T)]) {
+  constexpr int VE = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        f[i * VE + j] = __uint_as_float(w[j]);
+      } else {
+        const float2 t = unpack2<T>(w[j]);
+        f[i * VE + 2 * j] = t.x;
+        f[i * VE + 2 * j + 1] = t.y;
+      }
+    }
+  }
+}
+
+// A warp's best 32 logits so far, one key to a lane in order, and the candidates gathered since.
+struct LpList {
+  uint64_t mine = 0;             // this lane's key
+  uint64_t bound = 0;            // only larger keys can be among the best k
+  float fbound = -3.402823466e38f;  // its value; no -inf passes
+  int n = 0;                     // gathered (warp-uniform)
+  uint64_t *cand;                // shared, 64 of this warp
+
+  __device__ __forceinline__ void at_least(float v) {  // k logits are >= v
+    if (v >= fbound) {
+      bound = (lp_key(v, 0) & 0xffffffff00000000ull) - 1;
+      fbound = v;
+    }
+  }
+  __device__ __forceinline__ void flush(int count, int k) {  // count <= 32
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    mine = warp_merge(mine, warp_sort(lane < count ? cand[lane] : 0));
+    const uint64_t kth = __shfl_sync(0xffffffffu, mine, k - 1);
+    if (kth > bound) {
+      bound = kth;
+      fbound = lp_value(kth);
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void offer(bool in, float v, int idx, int k) {
+    const int lane = threadIdx.x & 31;
+    if (!__any_sync(0xffffffffu, in)) return;
+    const uint64_t key = lp_key(v, idx);
+    const uint32_t mask = __ballot_sync(0xffffffffu, in && key > bound);
+    if (in && key > bound) cand[n + __popc(mask & ((1u << lane) - 1u))] = key;
+    n += __popc(mask);
+    if (n >= 32) {
+      flush(32, k);
+      n -= 32;
+      if (lane < n) cand[lane] = cand[lane + 32];
+      __syncwarp();
+    }
+  }
+};
 
 struct LpPart {
   LpState s;
   uint64_t top[kLpMaxTop];
 };
 
+// Shared by both kernels once a CTA's part is known to its warp 0 (st in every lane, top one key a
+// lane): ranks > 0 write theirs to rank 0 and leave; rank 0 joins all and writes the row's results.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LogprobParams p) {
+__device__ __forceinline__ void lp_finish(const LogprobParams &p, const T *x, int64_t row, LpState st,
+                                          uint64_t top, LpPart *s_parts) {
   namespace cg = cooperative_groups;
-  constexpr int VE = 16 / sizeof(T);      // logits per 16-byte vector
-  constexpr int NV = kLpTile / VE;        // vectors per thread and tile
-  __shared__ LpState s_state[kLpWarps];
-  __shared__ uint64_t s_top[kLpWarps][32];
-  __shared__ uint64_t s_new[kLpWarps][64];  // gathered candidates of a warp
-  __shared__ LpPart s_part;
-  __shared__ LpPart s_parts[kLpMaxCluster];
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x / ranks;
-  const int V = p.vocab, K = p.top_k;
-  if (tid == 0) pdl_trigger();
-  pdl_wait();
-
-  // The row as 16-byte vectors from the aligned address at or below its start: vector v holds
-  // logits v * VE - off .. + VE, the first and last may hold others' too and are read by element.
-  const T *x = static_cast<const T *>(p.logits) + row * p.row_stride;
-  const int off = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const uint4 *xv = reinterpret_cast<const uint4 *>(x - off);
-  const int64_t nv = (int64_t(V) + off + VE - 1) / VE;
-  const int64_t per = (nv + ranks - 1) / ranks;
-  const int64_t v0 = rank * per, v1 = min(nv, v0 + per);
-
-  LpState st{neg_inf(), 0.f, 0.f};
-  uint64_t list = 0;           // this lane's entry of the warp's best 32
-  uint64_t bound = 0;          // only larger keys may enter the best k
-  float fbound = neg_inf();    // its value
-  int n_new = 0;               // gathered candidates (warp-uniform)
-  uint64_t *const cand = s_new[warp];
-
-  auto flush = [&](int n) {  // merge the first n (<= 32) gathered candidates
-    __syncwarp();
-    const uint64_t c = warp_sort(lane < n ? cand[lane] : 0);
-    list = warp_merge(list, c);
-    bound = max(bound, __shfl_sync(0xffffffffu, list, K - 1));
-    fbound = bound ? lp_value(bound) : neg_inf();
-    __syncwarp();
-  };
-
-  bool first = true;
-  for (int64_t vt = v0; vt < v1; vt += int64_t(kLpThreads) * NV) {
-    // ---- load a tile: vector vt + i * 256 + tid -----------------------------------------------
-    uint4 raw[NV];
-    float f[kLpTile];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t v = vt + i * kLpThreads + tid;
-      const int64_t e0 = v * VE - off;
-      if (v < v1 && e0 >= 0 && e0 + VE <= V) {
-        raw[i] = __ldcs(xv + v);
-      } else {
-        // Outside the part, or an edge vector of the row: element by element, -inf elsewhere.
-        T e[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j)
-          e[j] = (v < v1 && e0 + j >= 0 && e0 + j < V) ? x[e0 + j] : Elem<T>::from_f(neg_inf());
-        raw[i] = *reinterpret_cast<const uint4 *>(e);
-      }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int K = p.top_k;
+  if (ranks > 1) {
+    // The first barrier phase (arrived at on entry) says that rank 0 runs, so its memory may be
+    // written; the second that every part is there.
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 0) {
+      LpPart *q = cluster.map_shared_rank(s_parts, 0) + rank;
+      q->top[lane] = top;
+      if (lane == 0) q->s = st;
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 4) {
-          f[i * VE + j] = __uint_as_float(w[j]);
-        } else {
-          const float2 t2 = unpack2<T>(w[j]);
-          f[i * VE + 2 * j] = t2.x;
-          f[i * VE + 2 * j + 1] = t2.y;
-        }
-      }
-    }
-    // ---- softmax sums ---------------------------------------------------------------------------
-    float tm = f[0];
-#pragma unroll
-    for (int j = 1; j < kLpTile; ++j) tm = fmaxf(tm, f[j]);
-    if (tm > st.m) lp_shift(st, tm);
-    const float m = st.m == neg_inf() ? 0.f : st.m;
-#pragma unroll
-    for (int j = 0; j < kLpTile; ++j) {
-      const float d = f[j] - m;
-      const float e = ex2(d * kLog2e);
-      st.z += e;
-      st.w = fmaf(e, fmaxf(d, -1e30f), st.w);  // e = 0 where d = -inf, and 0 * -inf is not 0
-    }
-    // ---- candidates -------------------------------------------------------------------------------
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
     if (K > 0) {
-      if (first) {
-        // At least K of the lane maxima, so at least K logits, are >= their K-th largest. Equal
-        // ones enter too (the key just below the value at the highest index).
-        const float kth = __shfl_sync(0xffffffffu, warp_sort_f(tm), K - 1);
-        if (kth > neg_inf()) {
-          bound = (lp_key(kth, 0) & 0xffffffff00000000ull) - 1;
-          fbound = kth;
-        }
-        first = false;
+      for (int n = kLpMaxCluster / 2; n > 0; n >>= 1) {
+        for (int i = warp; i < n; i += warps)
+          if (i + n < ranks)
+            s_parts[i].top[lane] = warp_merge(s_parts[i].top[lane], s_parts[i + n].top[lane]);
+        __syncthreads();
       }
-      if (__any_sync(0xffffffffu, tm >= fbound && tm > neg_inf())) {
+    }
+    if (warp != 0) return;
+    top = s_parts[0].top[lane];
+    st = lp_warp_join(lane < ranks ? s_parts[lane].s : LpState{neg_inf(), 0.f, 0.f});
+  }
+  if (warp != 0) return;
+  // A NaN or +inf logit makes z NaN and with it everything said of the row. A row without a
+  // finite logit says that nothing can come: -inf for any token, no alternatives, entropy 0.
+  const bool bad = st.z != st.z || st.m == -neg_inf();
+  const bool none = st.m == neg_inf();
+  const float ln_z = none ? 0.f : logf(st.z);
+  const float nan = __int_as_float(0x7fc00000);
+  if (lane == 0) {
+    if (p.token_ids) {
+      const int32_t t = p.token_ids[row];
+      float lp = 0.f;
+      if (t < -1 || t >= p.vocab) {
+        report(FA_DEVERR_TOKEN);
+        lp = nan;
+      } else if (t >= 0) {
+        lp = bad ? nan : none ? neg_inf() : (Elem<T>::to_f(x[t]) - st.m) - ln_z;
+      }
+      p.logprobs[row] = lp;
+    }
+    if (p.entropy) p.entropy[row] = bad ? nan : none ? 0.f : fmaxf(ln_z - st.w / st.z, 0.f);
+  }
+  if (lane < K) {
+    const bool has = top != 0 && !bad;
+    p.top_ids[row * K + lane] = has ? int32_t(0xffffffffu - uint32_t(top)) : -1;
+    p.top_logprobs[row * K + lane] = bad ? nan : has ? (lp_value(top) - st.m) - ln_z : neg_inf();
+  }
+}
+
+__device__ __forceinline__ void lp_cluster_arrive() {
+  if (cooperative_groups::this_cluster().num_blocks() > 1)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+
+// ---- part kernel --------------------------------------------------------------------------------
+// Every thread keeps its logits (vector i * THREADS + tid of the CTA's part) in registers.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(const LogprobParams p) {
+  using Row = LpRow<T>;
+  constexpr int VE = Row::VE, NV = kLpPartLogits / VE, WARPS = THREADS / 32;
+  constexpr int PER_GROUP = THREADS / 32;  // threads of one of the 32 groups
+  constexpr int CAP = WARPS * 64;          // gathered candidates; more: each warp filters its own
+  __shared__ float s_max[32];
+  __shared__ float2 s_sum[WARPS];
+  __shared__ uint64_t s_cand[CAP];
+  __shared__ uint64_t s_top[WARPS][32];
+  __shared__ LpPart s_parts[kLpMaxCluster];
+  __shared__ int s_n;
+  const int ranks = int(cooperative_groups::this_cluster().num_blocks());
+  const int rank = int(cooperative_groups::this_cluster().block_rank());
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.top_k;
+  lp_cluster_arrive();
+  if (tid == 0) {
+    pdl_trigger();
+    s_n = 0;
+  }
+  pdl_wait();
+  const int64_t row = blockIdx.x / ranks;
+  const Row r(p, row);
+  const int64_t per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
+  uint4 raw[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float vm = f[i * VE];
+  for (int i = 0; i < NV; ++i) raw[i] = r.load(v0 + i * THREADS + tid, v1);
+  float f[kLpPartLogits];
+  lp_floats<T>(raw, f);
+  float gm[kLpPartLogits / 8];  // maxima of eights
 #pragma unroll
-          for (int j = 1; j < VE; ++j) vm = fmaxf(vm, f[i * VE + j]);
-          if (!__any_sync(0xffffffffu, vm >= fbound && vm > neg_inf())) continue;
-          const int e0 = int((vt + i * kLpThreads + tid) * VE - off);
+  for (int g = 0; g < kLpPartLogits / 8; ++g) {
+    gm[g] = f[8 * g];
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            const float v = f[i * VE + j];
-            const uint64_t key = lp_key(v, e0 + j);
-            const bool in = v > neg_inf() && key > bound;
-            const uint32_t mask = __ballot_sync(0xffffffffu, in);
-            if (mask) {
-              if (in) cand[n_new + __popc(mask & ((1u << lane) - 1u))] = key;
-              n_new += __popc(mask);
-              if (n_new >= 32) {
-                flush(32);
-                n_new -= 32;
-                if (lane < n_new) cand[lane] = cand[lane + 32];
-                __syncwarp();
-              }
-            }
+    for (int j = 1; j < 8; ++j) gm[g] = fmaxf(gm[g], f[8 * g + j]);
+  }
+  const float tm = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+  float m = tm;
+#pragma unroll
+  for (int o = 1; o < PER_GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane % PER_GROUP == 0) s_max[tid / PER_GROUP] = fmaxf(m, neg_inf());  // all NaN: -inf
+  __syncthreads();
+
+  // Each warp by itself: the part's maximum and the bound of its k-th largest.
+  const float sorted = warp_sort(s_max[lane]);
+  m = __shfl_sync(0xffffffffu, sorted, 0);
+  if (K > 0 && m > neg_inf()) {
+    const float bound = fmaxf(__shfl_sync(0xffffffffu, sorted, K - 1), -3.402823466e38f);
+    if (tm >= bound) {
+#pragma unroll
+      for (int g = 0; g < kLpPartLogits / 8; ++g) {
+        if (!(gm[g] >= bound)) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (f[8 * g + j] >= bound) {
+            const int at = atomicAdd(&s_n, 1);
+            const int e = 8 * g + j;
+            if (at < CAP)
+              s_cand[at] = lp_key(f[e], r.index(v0 + (e / VE) * THREADS + tid) + e % VE);
           }
         }
       }
     }
   }
-  if (K > 0 && n_new > 0) flush(n_new);
-
-  // ---- join the warps, then the cluster ------------------------------------------------------------
+  float z = 0.f, w = 0.f;
+  lp_sums(f, m, z, w);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const LpState b{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.z, o),
-                    __shfl_xor_sync(0xffffffffu, st.w, o)};
-    // Both partners must compute the same sum: the lower lane's part first.
-    st = (lane & o) ? lp_join(b, st) : lp_join(st, b);
+    z += __shfl_xor_sync(0xffffffffu, z, o);
+    w += __shfl_xor_sync(0xffffffffu, w, o);
   }
+  if (lane == 0) s_sum[warp] = make_float2(z, w);
+  __syncthreads();
+
+  const int n = s_n;
+  uint64_t top = 0;
+  if (n > CAP) {  // many equal logits: the warps' own lists, which drop ties past the k-th
+    LpList list;
+    list.cand = s_cand + warp * 64;
+    __syncthreads();  // everyone has read s_n; s_cand is rewritten
+    list.at_least(__shfl_sync(0xffffffffu, warp_sort(fmaxf(tm, neg_inf())), K - 1));
+#pragma unroll
+    for (int e = 0; e < kLpPartLogits; ++e)
+      list.offer(f[e] >= list.fbound, f[e], r.index(v0 + (e / VE) * THREADS + tid) + e % VE, K);
+    if (list.n > 0) list.flush(list.n, K);
+    s_top[warp][lane] = list.mine;
+    __syncthreads();
+    if (warp == 0)
+      for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
+  } else if (warp == 0) {
+    for (int i = 0; i < n; i += 32) {
+      const uint64_t c = warp_sort(i + lane < n ? s_cand[i + lane] : 0);
+      top = i ? warp_merge(top, c) : c;
+    }
+  }
+  LpState st{m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    st.z += s_sum[i].x;
+    st.w += s_sum[i].y;
+  }
+  lp_finish<T>(p, r.x, row, st, top, s_parts);
+}
+
+// ---- stream kernel ------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kLpStreamThreads, 3) logprobs_stream_kernel(const LogprobParams p) {
+  using Row = LpRow<T>;
+  constexpr int VE = Row::VE, NV = 4, N = NV * VE;  // 64 bytes a thread and tile
+  constexpr int THREADS = kLpStreamThreads, WARPS = THREADS / 32;
+  __shared__ LpState s_state[WARPS];
+  __shared__ uint64_t s_top[WARPS][32];
+  __shared__ uint64_t s_cand[WARPS][64];
+  __shared__ LpPart s_parts[kLpMaxCluster];
+  const int ranks = int(cooperative_groups::this_cluster().num_blocks());
+  const int rank = int(cooperative_groups::this_cluster().block_rank());
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.top_k;
+  lp_cluster_arrive();
+  if (tid == 0) pdl_trigger();
+  pdl_wait();
+  const int64_t row = blockIdx.x / ranks;
+  const Row r(p, row);
+  const int64_t per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
+  LpState st{neg_inf(), 0.f, 0.f};
+  LpList list;
+  list.cand = s_cand[warp];
+  uint4 raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) raw[i] = r.load(v0 + i * THREADS + tid, v1);
+  for (int64_t vt = v0; vt < v1; vt += THREADS * NV) {
+    float f[N];
+    lp_floats<T>(raw, f);
+    if (vt + THREADS * NV < v1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) raw[i] = r.load(vt + (NV + i) * THREADS + tid, v1);
+    }
+    float gm[N / 8];
+#pragma unroll
+    for (int g = 0; g < N / 8; ++g) {
+      gm[g] = f[8 * g];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) gm[g] = fmaxf(gm[g], f[8 * g + j]);
+    }
+    float tm = gm[0];
+#pragma unroll
+    for (int g = 1; g < N / 8; ++g) tm = fmaxf(tm, gm[g]);
+    tm = fmaxf(tm, neg_inf());  // all NaN: -inf
+    if (tm > st.m) lp_shift(st, tm);
+    lp_sums(f, st.m, st.z, st.w);
+    if (K > 0) {
+      if (vt == v0) list.at_least(__shfl_sync(0xffffffffu, warp_sort(tm), K - 1));
+      if (__any_sync(0xffffffffu, tm >= list.fbound)) {
+#pragma unroll
+        for (int g = 0; g < N / 8; ++g) {
+          if (!__any_sync(0xffffffffu, gm[g] >= list.fbound)) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int e = 8 * g + j;
+            list.offer(f[e] >= list.fbound, f[e], r.index(vt + (e / VE) * THREADS + tid) + e % VE, K);
+          }
+        }
+        if (vt == v0 && list.n > 0) {  // the first tile's k-th is a far better bound
+          list.flush(list.n, K);
+          list.n = 0;
+        }
+      }
+    }
+  }
+  if (K > 0 && list.n > 0) list.flush(list.n, K);
+  st = lp_warp_join(st);
   if (lane == 0) s_state[warp] = st;
-  s_top[warp][lane] = list;
+  s_top[warp][lane] = list.mine;
   __syncthreads();
   if (K > 0) {
 #pragma unroll
-    for (int n = kLpWarps / 2; n > 0; n >>= 1) {
+    for (int n = WARPS / 2; n > 0; n >>= 1) {
       if (warp < n) s_top[warp][lane] = warp_merge(s_top[warp][lane], s_top[warp + n][lane]);
       __syncthreads();
     }
   }
-  if (warp == 0) {
-    s_part.top[lane] = s_top[0][lane];
-    if (lane == 0) {
-      LpState a = s_state[0];
-      for (int w = 1; w < kLpWarps; ++w) a = lp_join(a, s_state[w]);
-      s_part.s = a;
-    }
-  }
-  __syncthreads();
-  if (ranks > 1) {
-    cluster.sync();  // every rank's part is written
-    if (rank == 0) {
-      for (int r = warp; r < ranks; r += kLpWarps) {
-        const LpPart *q = cluster.map_shared_rank(&s_part, r);
-        s_parts[r].top[lane] = q->top[lane];
-        if (lane == 0) s_parts[r].s = q->s;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        uint64_t best = s_parts[0].top[lane];
-        LpState a = s_parts[0].s;
-        for (int r = 1; r < ranks; ++r) {
-          if (K > 0) best = warp_merge(best, s_parts[r].top[lane]);
-          a = lp_join(a, s_parts[r].s);
-        }
-        s_part.top[lane] = best;
-        if (lane == 0) s_part.s = a;
-      }
-    }
-    cluster.sync();  // no rank leaves while its shared memory is being read
-  }
-  if (rank != 0 || warp != 0) return;
-  __syncwarp();
-  const LpState a = s_part.s;
-  // A NaN or +inf logit makes Z NaN and with it everything said of the row. A row without a
-  // finite logit says that nothing can come: -inf for any token, no alternatives, entropy 0.
-  const bool none = a.m == neg_inf() && a.z == 0.f;
-  const float ln_z = none ? 0.f : logf(a.z);
-  const float nan = __int_as_float(0x7fc00000);
-  const bool bad = !(a.z == a.z) || a.m == -neg_inf();
-  if (lane == 0) {
-    if (p.token_ids) {
-      const int32_t t = p.token_ids[row];
-      float lp = 0.f;
-      if (t < -1 || t >= V) {
-        report(FA_DEVERR_TOKEN);
-        lp = nan;
-      } else if (t >= 0) {
-        lp = bad ? nan : none ? neg_inf() : (Elem<T>::to_f(x[t]) - a.m) - ln_z;
-      }
-      p.logprobs[row] = lp;
-    }
-    if (p.entropy) p.entropy[row] = bad ? nan : none ? 0.f : fmaxf(ln_z - a.w / a.z, 0.f);
-  }
-  if (lane < K) {
-    const uint64_t key = s_part.top[lane];
-    const bool has = key != 0 && !bad;
-    p.top_ids[row * K + lane] = has ? int32_t(0xffffffffu - uint32_t(key)) : -1;
-    p.top_logprobs[row * K + lane] = bad ? nan : has ? (lp_value(key) - a.m) - ln_z : neg_inf();
-  }
+  st = lp_warp_join(lane < WARPS ? s_state[lane] : LpState{neg_inf(), 0.f, 0.f});
+  lp_finish<T>(p, r.x, row, st, s_top[0][lane], s_parts);
 }
 
 }  // namespace fa
