@@ -966,7 +966,7 @@ fa_status launch_generic8(const fa_kv8_layer *L, const void *q, void *out, int32
 // ---- log probabilities ------------------------------------------------------------------------
 
 constexpr int kLpPartTile = fa::kLpPartThreads * fa::kLpPartLogits;
-constexpr int kLpPartCtasPerSm = 12;
+constexpr int kLpPartCtasPerSm = 2;
 constexpr int kLpSmallTile = fa::kLpSmallThreads * fa::kLpPartLogits;
 
 template <typename T>
@@ -986,7 +986,7 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     return launch_pdl(who, kern, dim3(unsigned(rows * ranks)), fa::kLpPartThreads, 0, stream, int(ranks), p);
   }
   int split = 1;  // few rows too long for registers
-  while (split < 8 && int64_t(rows) * split * 2 <= int64_t(sm_count()) * 3) split *= 2;
+  while (split < 8 && int64_t(rows) * split * 2 <= int64_t(sm_count()) * 4) split *= 2;
   return launch_pdl(who, fa::logprobs_stream_kernel<T>, dim3(unsigned(rows * split)), fa::kLpStreamThreads, 0,
                     stream, split, p);
 }

@@ -161,20 +161,39 @@ __device__ __forceinline__ LpState lp_warp_join(LpState st) {
   return st;
 }
 
-// z and w of N logits against m >= all of them (m may be -inf: then nothing but NaN counts).
-template <int N>
-__device__ __forceinline__ void lp_sums(const float (&f)[N], float m, float &z, float &w) {
+// Logits e, e + 1 of the vectors `raw` (e even and constant once unrolled).
+template <typename T, int NV>
+__device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
+  constexpr int VE = 16 / sizeof(T);
+  const uint4 &v = raw[e / VE];
+  const int i = e % VE;
+  if constexpr (sizeof(T) == 4)
+    return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                  : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  else
+    return unpack2<T>(i == 0 ? v.x : i == 2 ? v.y : i == 4 ? v.z : v.w);
+}
+
+// z and w of the logits in `raw` against m >= all of them (m may be -inf: then nothing but NaN
+// counts).
+template <typename T, int NV>
+__device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &z, float &w) {
+  constexpr int N = NV * 16 / sizeof(T);
   if (m == neg_inf()) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (f[j] != f[j]) z = f[j];
+    for (int j = 0; j < N; j += 2) {
+      const float2 x = lp_pair<T>(raw, j);
+      if (x.x != x.x) z = x.x;
+      if (x.y != x.y) z = x.y;
+    }
     return;
   }
   const uint64_t nm = f2_pack(-m, -m), l2e = f2_pack(kLog2e, kLog2e);
   uint64_t za[2] = {0, 0}, wa[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
-    const uint64_t d = f2_add(f2_pack(f[j], f[j + 1]), nm);
+    const float2 x = lp_pair<T>(raw, j);
+    const uint64_t d = f2_add(f2_pack(x.x, x.y), nm);
     const float2 s = f2_unpack(f2_mul(d, l2e));
     const uint64_t e = f2_pack(ex2(s.x), ex2(s.y));
     za[(j >> 1) & 1] = f2_add(za[(j >> 1) & 1], e);
@@ -185,9 +204,11 @@ __device__ __forceinline__ void lp_sums(const float (&f)[N], float m, float &z, 
   if (ws != ws) {  // a masked logit's 0 * -inf (or a NaN, which z has seen): once more, with care
     ws = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = f[j] - m;
-      ws = fmaf(ex2(d * kLog2e), fmaxf(d, -1e30f), ws);
+    for (int j = 0; j < N; j += 2) {
+      const float2 x = lp_pair<T>(raw, j);
+      const float d0 = x.x - m, d1 = x.y - m;
+      ws = fmaf(ex2(d0 * kLog2e), fmaxf(d0, -1e30f), ws);
+      ws = fmaf(ex2(d1 * kLog2e), fmaxf(d1, -1e30f), ws);
     }
   }
   z += zz.x + zz.y;
@@ -221,67 +242,112 @@ template <typename T> struct LpRow {
     return *reinterpret_cast<const uint4 *>(e);
   }
   __device__ __forceinline__ int index(int64_t v) const { return int(v * VE - off); }
+  __device__ __forceinline__ float at(int i) const { return Elem<T>::to_f(x[i]); }
 };
 
+// Maxima of eight logits each, and of all; -inf where there is no number. 16-bit ones are compared
+// two at a time.
 template <typename T, int NV>
-__device__ __forceinline__ void lp_floats(const uint4 (&raw)[NV], float (&f)[NV * 16 / sizeof(T)]) {
-  constexpr int VE = 16 / sizeof(T);
+__device__ __forceinline__ float lp_maxima(const uint4 (&raw)[NV], float (&gm)[NV * 2 / sizeof(T)]) {
+  constexpr int G = NV * 2 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+  for (int g = 0; g < G; ++g) {
+    if constexpr (sizeof(T) == 2) {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2 *w = reinterpret_cast<const T2 *>(&raw[g]);
+      const T2 m2 = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      const float2 m = unpack2<T>(*reinterpret_cast<const uint32_t *>(&m2));
+      gm[g] = fmaxf(fmaxf(m.x, m.y), neg_inf());
+    } else {
+      float m = neg_inf();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        f[i * VE + j] = __uint_as_float(w[j]);
-      } else {
-        const float2 t = unpack2<T>(w[j]);
-        f[i * VE + 2 * j] = t.x;
-        f[i * VE + 2 * j + 1] = t.y;
+      for (int j = 0; j < 8; j += 2) {
+        const float2 x = lp_pair<T>(raw, 8 * g + j);
+        m = fmaxf(m, fmaxf(x.x, x.y));
       }
+      gm[g] = m;
     }
   }
+  float tm = gm[0];
+#pragma unroll
+  for (int g = 1; g < G; ++g) tm = fmaxf(tm, gm[g]);
+  return tm;
+}
+
+// The warp's list `mine` with its n <= 32 gathered candidates. Out of line: one copy of the sort.
+__device__ __noinline__ uint64_t lp_take(uint64_t mine, const uint64_t *cand, int n) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  mine = warp_merge(mine, warp_sort(lane < n ? cand[lane] : 0));
+  __syncwarp();
+  return mine;
 }
 
 // A warp's best 32 logits so far, one key to a lane in order, and the candidates gathered since.
 struct LpList {
-  uint64_t mine = 0;             // this lane's key
-  uint64_t bound = 0;            // only larger keys can be among the best k
+  uint64_t mine = 0;                // this lane's key
+  uint64_t bound = 0;               // only larger keys can be among the best k
   float fbound = -3.402823466e38f;  // its value; no -inf passes
-  int n = 0;                     // gathered (warp-uniform)
-  uint64_t *cand;                // shared, 64 of this warp
+  int n = 0;                        // gathered (warp-uniform)
+  uint64_t *cand;                   // shared, 64 of this warp
 
   __device__ __forceinline__ void at_least(float v) {  // k logits are >= v
-    if (v >= fbound) {
+    if (v > fbound) {
       bound = (lp_key(v, 0) & 0xffffffff00000000ull) - 1;
       fbound = v;
     }
   }
-  __device__ __forceinline__ void flush(int count, int k) {  // count <= 32
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    mine = warp_merge(mine, warp_sort(lane < count ? cand[lane] : 0));
+  __device__ __forceinline__ void flush(int count, int k) {
+    mine = lp_take(mine, cand, count);
     const uint64_t kth = __shfl_sync(0xffffffffu, mine, k - 1);
     if (kth > bound) {
       bound = kth;
       fbound = lp_value(kth);
     }
-    __syncwarp();
   }
-  __device__ __forceinline__ void offer(bool in, float v, int idx, int k) {
+  // Gathers the logits of a tile that pass the bound. hits: one bit per logit of this lane, bit e
+  // for logit e % VE of vector v0 + (e / VE) * step; they are read again from the row.
+  template <class Row>
+  __device__ __forceinline__ void gather(uint32_t hits, const Row &r, int64_t v0, int step, int k) {
     const int lane = threadIdx.x & 31;
-    if (!__any_sync(0xffffffffu, in)) return;
-    const uint64_t key = lp_key(v, idx);
-    const uint32_t mask = __ballot_sync(0xffffffffu, in && key > bound);
-    if (in && key > bound) cand[n + __popc(mask & ((1u << lane) - 1u))] = key;
-    n += __popc(mask);
-    if (n >= 32) {
-      flush(32, k);
-      n -= 32;
-      if (lane < n) cand[lane] = cand[lane + 32];
-      __syncwarp();
+    while (__any_sync(0xffffffffu, hits != 0)) {
+      uint64_t key = 0;
+      if (hits) {
+        const int e = __ffs(hits) - 1;
+        hits &= hits - 1;
+        const int idx = r.index(v0 + int64_t(e / Row::VE) * step) + e % Row::VE;
+        key = lp_key(r.at(idx), idx);
+      }
+      const uint32_t mask = __ballot_sync(0xffffffffu, key > bound);
+      if (key > bound) cand[n + __popc(mask & ((1u << lane) - 1u))] = key;
+      n += __popc(mask);
+      if (n >= 32) {
+        flush(32, k);
+        n -= 32;
+        if (lane < n) cand[lane] = cand[lane + 32];
+        __syncwarp();
+      }
     }
   }
 };
+
+// Bits of the logits that are >= bound, by eights that hold one.
+template <typename T, int NV>
+__device__ __forceinline__ uint32_t lp_hits(const uint4 (&raw)[NV], const float (&gm)[NV * 2 / sizeof(T)],
+                                            float bound) {
+  uint32_t hits = 0;
+#pragma unroll
+  for (int g = 0; g < NV * 2 / int(sizeof(T)); ++g) {
+    if (!__any_sync(0xffffffffu, gm[g] >= bound)) continue;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float2 x = lp_pair<T>(raw, 8 * g + j);
+      if (x.x >= bound) hits |= 1u << (8 * g + j);
+      if (x.y >= bound) hits |= 2u << (8 * g + j);
+    }
+  }
+  return hits;
+}
 
 struct LpPart {
   LpState s;
@@ -384,20 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   uint4 raw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) raw[i] = r.load(v0 + i * THREADS + tid, v1);
-  float f[kLpPartLogits];
-  lp_floats<T>(raw, f);
-  float gm[kLpPartLogits / 8];  // maxima of eights
-#pragma unroll
-  for (int g = 0; g < kLpPartLogits / 8; ++g) {
-    gm[g] = f[8 * g];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) gm[g] = fmaxf(gm[g], f[8 * g + j]);
-  }
-  const float tm = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+  float gm[kLpPartLogits / 8];
+  const float tm = lp_maxima<T>(raw, gm);
   float m = tm;
 #pragma unroll
   for (int o = 1; o < PER_GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane % PER_GROUP == 0) s_max[tid / PER_GROUP] = fmaxf(m, neg_inf());  // all NaN: -inf
+  if (lane % PER_GROUP == 0) s_max[tid / PER_GROUP] = m;
   __syncthreads();
 
   // Each warp by itself: the part's maximum and the bound of its k-th largest.
@@ -405,24 +463,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   m = __shfl_sync(0xffffffffu, sorted, 0);
   if (K > 0 && m > neg_inf()) {
     const float bound = fmaxf(__shfl_sync(0xffffffffu, sorted, K - 1), -3.402823466e38f);
-    if (tm >= bound) {
-#pragma unroll
-      for (int g = 0; g < kLpPartLogits / 8; ++g) {
-        if (!(gm[g] >= bound)) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (f[8 * g + j] >= bound) {
-            const int at = atomicAdd(&s_n, 1);
-            const int e = 8 * g + j;
-            if (at < CAP)
-              s_cand[at] = lp_key(f[e], r.index(v0 + (e / VE) * THREADS + tid) + e % VE);
-          }
-        }
-      }
+    uint32_t hits = lp_hits<T>(raw, gm, bound);
+    while (hits) {
+      const int e = __ffs(hits) - 1;
+      hits &= hits - 1;
+      const int idx = r.index(v0 + (e / VE) * THREADS + tid) + e % VE;
+      const int at = atomicAdd(&s_n, 1);
+      if (at < CAP) s_cand[at] = lp_key(r.at(idx), idx);
     }
   }
   float z = 0.f, w = 0.f;
-  lp_sums(f, m, z, w);
+  lp_sums<T>(raw, m, z, w);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -437,10 +488,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     LpList list;
     list.cand = s_cand + warp * 64;
     __syncthreads();  // everyone has read s_n; s_cand is rewritten
-    list.at_least(__shfl_sync(0xffffffffu, warp_sort(fmaxf(tm, neg_inf())), K - 1));
-#pragma unroll
-    for (int e = 0; e < kLpPartLogits; ++e)
-      list.offer(f[e] >= list.fbound, f[e], r.index(v0 + (e / VE) * THREADS + tid) + e % VE, K);
+    list.at_least(__shfl_sync(0xffffffffu, warp_sort(tm), K - 1));
+    list.gather(lp_hits<T>(raw, gm, list.fbound), r, v0 + tid, THREADS, K);
     if (list.n > 0) list.flush(list.n, K);
     s_top[warp][lane] = list.mine;
     __syncthreads();
@@ -462,12 +511,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
 }
 
 // ---- stream kernel ------------------------------------------------------------------------------
+// Tiles of 64 bytes a thread, the next one in flight. The 32 groups of the CTA (eight lanes each)
+// keep their running maxima in shared memory, and the warps take a new bound from them after tiles
+// 1, 2, 4, 8, ...: without a barrier but the first, for maxima that a warp sees too early are still
+// a lower bound. About 32 ln(32 / (32 - k)) / 8 logits a warp pass in each doubling.
 template <typename T>
-__global__ void __launch_bounds__(kLpStreamThreads, 3) logprobs_stream_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(const LogprobParams p) {
   using Row = LpRow<T>;
-  constexpr int VE = Row::VE, NV = 4, N = NV * VE;  // 64 bytes a thread and tile
+  constexpr int VE = Row::VE, NV = 4, N = NV * VE;
   constexpr int THREADS = kLpStreamThreads, WARPS = THREADS / 32;
   __shared__ LpState s_state[WARPS];
+  __shared__ volatile float s_max[32];
   __shared__ uint64_t s_top[WARPS][32];
   __shared__ uint64_t s_cand[WARPS][64];
   __shared__ LpPart s_parts[kLpMaxCluster];
@@ -483,46 +537,34 @@ __global__ void __launch_bounds__(kLpStreamThreads, 3) logprobs_stream_kernel(co
   LpState st{neg_inf(), 0.f, 0.f};
   LpList list;
   list.cand = s_cand[warp];
-  uint4 raw[NV];
+  uint4 next[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) raw[i] = r.load(v0 + i * THREADS + tid, v1);
-  for (int64_t vt = v0; vt < v1; vt += THREADS * NV) {
-    float f[N];
-    lp_floats<T>(raw, f);
+  for (int i = 0; i < NV; ++i) next[i] = r.load(v0 + i * THREADS + tid, v1);
+  int tile = 0;
+  for (int64_t vt = v0; vt < v1; vt += THREADS * NV, ++tile) {
+    uint4 raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = next[i];
     if (vt + THREADS * NV < v1) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) raw[i] = r.load(vt + (NV + i) * THREADS + tid, v1);
+      for (int i = 0; i < NV; ++i) next[i] = r.load(vt + (NV + i) * THREADS + tid, v1);
     }
     float gm[N / 8];
-#pragma unroll
-    for (int g = 0; g < N / 8; ++g) {
-      gm[g] = f[8 * g];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) gm[g] = fmaxf(gm[g], f[8 * g + j]);
-    }
-    float tm = gm[0];
-#pragma unroll
-    for (int g = 1; g < N / 8; ++g) tm = fmaxf(tm, gm[g]);
-    tm = fmaxf(tm, neg_inf());  // all NaN: -inf
+    const float tm = lp_maxima<T>(raw, gm);
     if (tm > st.m) lp_shift(st, tm);
-    lp_sums(f, st.m, st.z, st.w);
+    lp_sums<T>(raw, st.m, st.z, st.w);
     if (K > 0) {
-      if (vt == v0) list.at_least(__shfl_sync(0xffffffffu, warp_sort(tm), K - 1));
-      if (__any_sync(0xffffffffu, tm >= list.fbound)) {
+      if ((tile & (tile + 1)) == 0) {
+        float m = st.m;
 #pragma unroll
-        for (int g = 0; g < N / 8; ++g) {
-          if (!__any_sync(0xffffffffu, gm[g] >= list.fbound)) continue;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int e = 8 * g + j;
-            list.offer(f[e] >= list.fbound, f[e], r.index(vt + (e / VE) * THREADS + tid) + e % VE, K);
-          }
-        }
-        if (vt == v0 && list.n > 0) {  // the first tile's k-th is a far better bound
-          list.flush(list.n, K);
-          list.n = 0;
-        }
+        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane % 8 == 0) s_max[tid / 8] = m;
+        if (tile == 0) __syncthreads();
+        __syncwarp();
+        list.at_least(__shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
       }
+      if (__any_sync(0xffffffffu, tm >= list.fbound))
+        list.gather(lp_hits<T>(raw, gm, list.fbound), r, vt + tid, THREADS, K);
     }
   }
   if (K > 0 && list.n > 0) list.flush(list.n, K);
