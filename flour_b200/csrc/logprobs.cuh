@@ -96,33 +96,6 @@ __device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b) {
   return v;
 }
 
-// Two f32 operations an instruction.
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // A part of a row: m its largest logit, z = sum e^(x - m), w = sum e^(x - m) (x - m). A part
 // without a finite logit has m = -inf, z = 0. A NaN logit makes z NaN, for good.
 struct LpState {
@@ -175,7 +148,8 @@ __device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
 }
 
 // z and w of the logits in `raw` against m >= all of them (m may be -inf: then nothing but NaN
-// counts).
+// counts). Four operations a logit: with L = log2(e), M = m L rounded and r = m L - M (one fma, so
+// exact), s = x L - M is one fma, e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r leaves the sums.
 template <typename T, int NV>
 __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &z, float &w) {
   constexpr int N = NV * 16 / sizeof(T);
@@ -188,30 +162,34 @@ __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &
     }
     return;
   }
-  const uint64_t nm = f2_pack(-m, -m), l2e = f2_pack(kLog2e, kLog2e);
-  uint64_t za[2] = {0, 0}, wa[2] = {0, 0};
+  const float M = m * kLog2e, r = fmaf(m, kLog2e, -M);
+  float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
     const float2 x = lp_pair<T>(raw, j);
-    const uint64_t d = f2_add(f2_pack(x.x, x.y), nm);
-    const float2 s = f2_unpack(f2_mul(d, l2e));
-    const uint64_t e = f2_pack(ex2(s.x), ex2(s.y));
-    za[(j >> 1) & 1] = f2_add(za[(j >> 1) & 1], e);
-    wa[(j >> 1) & 1] = f2_fma(e, d, wa[(j >> 1) & 1]);
+    const float s0 = fmaf(x.x, kLog2e, -M), s1 = fmaf(x.y, kLog2e, -M);
+    const float e0 = ex2(s0), e1 = ex2(s1);
+    z0 += e0;
+    z1 += e1;
+    w0 = fmaf(e0, s0, w0);
+    w1 = fmaf(e1, s1, w1);
   }
-  const float2 zz = f2_unpack(f2_add(za[0], za[1])), ww = f2_unpack(f2_add(wa[0], wa[1]));
-  float ws = ww.x + ww.y;
-  if (ws != ws) {  // a masked logit's 0 * -inf (or a NaN, which z has seen): once more, with care
-    ws = 0.f;
+  const float back = ex2(-r);
+  float zs = (z0 + z1) * back, ws = fmaf(-r, z0 + z1, w0 + w1) * (back * 0.693147180559945f);
+  // A masked logit's 0 * -inf, a NaN, or logits too large for M: once more, with care.
+  if (ws != ws) {
+    zs = ws = 0.f;
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       const float2 x = lp_pair<T>(raw, j);
       const float d0 = x.x - m, d1 = x.y - m;
-      ws = fmaf(ex2(d0 * kLog2e), fmaxf(d0, -1e30f), ws);
-      ws = fmaf(ex2(d1 * kLog2e), fmaxf(d1, -1e30f), ws);
+      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
+      zs += e0 + e1;
+      ws = fmaf(e0, fmaxf(d0, -1e30f), ws);
+      ws = fmaf(e1, fmaxf(d1, -1e30f), ws);
     }
   }
-  z += zz.x + zz.y;
+  z += zs;
   w += ws;
 }
 
@@ -240,6 +218,18 @@ template <typename T> struct LpRow {
     for (int j = 0; j < VE; ++j)
       e[j] = (v < v1 && e0 + j >= 0 && e0 + j < vocab) ? x[e0 + j] : Elem<T>::from_f(neg_inf());
     return *reinterpret_cast<const uint4 *>(e);
+  }
+  // Vectors v, v + step, ... v + (NV - 1) step of this thread, where first .. last bound those of
+  // all threads: one check for a tile inside the row.
+  template <int NV>
+  __device__ __forceinline__ void load_tile(uint4 (&raw)[NV], int64_t first, int64_t v, int step, int64_t v1) const {
+    if (first >= (off ? 1 : 0) && first + int64_t(step) * NV <= min(v1, (int64_t(vocab) + off) / VE)) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) raw[i] = __ldcs(xv + v + i * step);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) raw[i] = load(v + i * step, v1);
+    }
   }
   __device__ __forceinline__ int index(int64_t v) const { return int(v * VE - off); }
   __device__ __forceinline__ float at(int i) const { return Elem<T>::to_f(x[i]); }
@@ -448,8 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   const Row r(p, row);
   const int64_t per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
   uint4 raw[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) raw[i] = r.load(v0 + i * THREADS + tid, v1);
+  r.load_tile(raw, v0, v0 + tid, THREADS, v1);
   float gm[kLpPartLogits / 8];
   const float tm = lp_maxima<T>(raw, gm);
   float m = tm;
@@ -538,17 +527,14 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
   LpList list;
   list.cand = s_cand[warp];
   uint4 next[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) next[i] = r.load(v0 + i * THREADS + tid, v1);
+  r.load_tile(next, v0, v0 + tid, THREADS, v1);
   int tile = 0;
   for (int64_t vt = v0; vt < v1; vt += THREADS * NV, ++tile) {
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = next[i];
-    if (vt + THREADS * NV < v1) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) next[i] = r.load(vt + (NV + i) * THREADS + tid, v1);
-    }
+    if (vt + THREADS * NV < v1)
+      r.load_tile(next, vt + THREADS * NV, vt + THREADS * NV + tid, THREADS, v1);
     float gm[N / 8];
     const float tm = lp_maxima<T>(raw, gm);
     if (tm > st.m) lp_shift(st, tm);
