@@ -1721,7 +1721,8 @@ fa_status fa_token_logprobs(const void *logits, int32_t dtype, int64_t row_strid
   if (num_rows > 1 && row_stride < vocab)
     return fail(FA_EINVAL, "%s: row_stride %lld < vocab %d", who, (long long)row_stride, vocab);
   if (!aligned(logits, dtype_size(dtype))) return fail(FA_EINVAL, "%s: misaligned logits", who);
-  if (num_rows > INT32_MAX / fa::kLpMaxCluster) return fail(FA_EUNSUPPORTED, "%s: %d rows", who, num_rows);
+  if (num_rows > INT32_MAX / fa::kLpMaxCluster || vocab > (1 << 30))
+    return fail(FA_EUNSUPPORTED, "%s: %d rows of %d", who, num_rows, vocab);
   fa::LogprobParams p{};
   p.logits = logits;
   p.row_stride = row_stride;

@@ -162,7 +162,8 @@ __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &
     }
     return;
   }
-  const float M = m * kLog2e, r = fmaf(m, kLog2e, -M);
+  const float M = m * kLog2e;
+  const float r = fmaf(m, kLog2e, -M);
   float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
@@ -193,37 +194,41 @@ __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &
   w += ws;
 }
 
+// Logits e0 .. e0 + 15 bytes of x[0 .. end), -inf outside. Out of line: few vectors take it.
+template <typename T> __device__ __noinline__ uint4 lp_edge(const T *x, int e0, int end) {
+  constexpr int VE = 16 / sizeof(T);
+  alignas(16) T e[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j) e[j] = (e0 + j >= 0 && e0 + j < end) ? x[e0 + j] : Elem<T>::from_f(neg_inf());
+  return *reinterpret_cast<const uint4 *>(e);
+}
+
 // A row as 16-byte vectors from the aligned address at or below its start: vector v holds logits
 // v * VE - off and on.
 template <typename T> struct LpRow {
   static constexpr int VE = 16 / sizeof(T);
   const T *x;
   const uint4 *xv;
-  int off, vocab;
-  int64_t nv;
+  int off, vocab, nv;
   __device__ __forceinline__ LpRow(const LogprobParams &p, int64_t row) {
     x = static_cast<const T *>(p.logits) + row * p.row_stride;
     off = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     xv = reinterpret_cast<const uint4 *>(x - off);
     vocab = p.vocab;
-    nv = (int64_t(vocab) + off + VE - 1) / VE;
+    nv = (vocab + off + VE - 1) / VE;
   }
   // Vector v of a part that ends at v1; -inf past it. The row's first and last vectors may hold
   // its neighbours' logits too and are read element by element.
-  __device__ __forceinline__ uint4 load(int64_t v, int64_t v1) const {
-    const int64_t e0 = v * VE - off;
+  __device__ __forceinline__ uint4 load(int v, int v1) const {
+    const int e0 = v * VE - off;
     if (v < v1 && e0 >= 0 && e0 + VE <= vocab) return __ldcs(xv + v);
-    alignas(16) T e[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j)
-      e[j] = (v < v1 && e0 + j >= 0 && e0 + j < vocab) ? x[e0 + j] : Elem<T>::from_f(neg_inf());
-    return *reinterpret_cast<const uint4 *>(e);
+    return lp_edge<T>(x, e0, v < v1 ? vocab : 0);
   }
   // Vectors v, v + step, ... v + (NV - 1) step of this thread, where first .. last bound those of
   // all threads: one check for a tile inside the row.
   template <int NV>
-  __device__ __forceinline__ void load_tile(uint4 (&raw)[NV], int64_t first, int64_t v, int step, int64_t v1) const {
-    if (first >= (off ? 1 : 0) && first + int64_t(step) * NV <= min(v1, (int64_t(vocab) + off) / VE)) {
+  __device__ __forceinline__ void load_tile(uint4 (&raw)[NV], int first, int v, int step, int v1) const {
+    if (first >= (off ? 1 : 0) && first + step * NV <= min(v1, (vocab + off) / VE)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) raw[i] = __ldcs(xv + v + i * step);
     } else {
@@ -231,8 +236,44 @@ template <typename T> struct LpRow {
       for (int i = 0; i < NV; ++i) raw[i] = load(v + i * step, v1);
     }
   }
-  __device__ __forceinline__ int index(int64_t v) const { return int(v * VE - off); }
-  __device__ __forceinline__ float at(int i) const { return Elem<T>::to_f(x[i]); }
+  __device__ __forceinline__ int index(int v) const { return v * VE - off; }
+};
+
+// Logit e of the vectors, e at run time: selects, no memory.
+template <typename T, int NV>
+__device__ __forceinline__ float lp_pick(const uint4 (&raw)[NV], int e) {
+  constexpr int VE = 16 / sizeof(T);
+  uint4 v = raw[0];
+#pragma unroll
+  for (int i = 1; i < NV; ++i)
+    if (e / VE == i) v = raw[i];
+  const int b = e % VE * sizeof(T);  // byte in the vector
+  const uint32_t w = b < 8 ? (b < 4 ? v.x : v.y) : (b < 12 ? v.z : v.w);
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else return (b & 2) ? unpack2<T>(w).y : unpack2<T>(w).x;
+}
+
+// The same through shared memory, for the loop that has no registers to spare: a lane writes its
+// vectors to places of its own and reads one logit back.
+template <typename T, int NV> struct LpStash {
+  T *mine;  // 16-byte places 512 bytes apart
+  __device__ __forceinline__ LpStash(uint4 *warp_base, const uint4 (&raw)[NV]) {
+    uint4 *at = warp_base + (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) at[32 * i] = raw[i];
+    mine = reinterpret_cast<T *>(at);
+  }
+  __device__ __forceinline__ uint4 vector(int i) const {
+    return *reinterpret_cast<const uint4 *>(mine + i * (32 * 16 / int(sizeof(T))));
+  }
+  __device__ __forceinline__ float operator()(int e) const {
+    constexpr int VE = 16 / sizeof(T);
+    return Elem<T>::to_f(mine[(e / VE) * (32 * VE) + e % VE]);
+  }
+};
+template <typename T, int NV> struct LpPicked {
+  const uint4 (&raw)[NV];
+  __device__ __forceinline__ float operator()(int e) const { return lp_pick<T>(raw, e); }
 };
 
 // Maxima of eight logits each, and of all; -inf where there is no number. 16-bit ones are compared
@@ -279,6 +320,7 @@ struct LpList {
   uint64_t bound = 0;               // only larger keys can be among the best k
   float fbound = -3.402823466e38f;  // its value; no -inf passes
   int n = 0;                        // gathered (warp-uniform)
+  bool listed = false;              // the bound is a key of the list
   uint64_t *cand;                   // shared, 64 of this warp
 
   __device__ __forceinline__ void at_least(float v) {  // k logits are >= v
@@ -293,20 +335,21 @@ struct LpList {
     if (kth > bound) {
       bound = kth;
       fbound = lp_value(kth);
+      listed = true;
     }
   }
   // Gathers the logits of a tile that pass the bound. hits: one bit per logit of this lane, bit e
-  // for logit e % VE of vector v0 + (e / VE) * step; they are read again from the row.
-  template <class Row>
-  __device__ __forceinline__ void gather(uint32_t hits, const Row &r, int64_t v0, int step, int k) {
+  // for logit e % VE of vector v0 + (e / VE) * step.
+  template <class Value, class Row>
+  __device__ __forceinline__ void gather(uint32_t hits, const Value &value, const Row &r, int v0, int step, int k) {
     const int lane = threadIdx.x & 31;
     while (__any_sync(0xffffffffu, hits != 0)) {
       uint64_t key = 0;
       if (hits) {
         const int e = __ffs(hits) - 1;
         hits &= hits - 1;
-        const int idx = r.index(v0 + int64_t(e / Row::VE) * step) + e % Row::VE;
-        key = lp_key(r.at(idx), idx);
+        const int idx = r.index(v0 + e / Row::VE * step) + e % Row::VE;
+        key = lp_key(value(e), idx);
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, key > bound);
       if (key > bound) cand[n + __popc(mask & ((1u << lane) - 1u))] = key;
@@ -337,6 +380,56 @@ __device__ __forceinline__ uint32_t lp_hits(const uint4 (&raw)[NV], const float 
     }
   }
   return hits;
+}
+
+// The CTA's candidates: keys of the logits that passed the bound when their tile was read. One
+// that comes when the pool is full is counted only, and the row's part is read again with lists.
+constexpr int kLpPool = 1024;
+struct LpPool {
+  uint64_t key[kLpPool];
+  int n;
+};
+
+// Each lane takes its hits one by one: a short loop, for unrolled updates miss the instruction cache.
+template <class Value, class Row>
+__device__ __forceinline__ void lp_pool_add(LpPool &pool, uint32_t hits, const Value &value, const Row &r,
+                                            int v0, int step) {
+#pragma unroll 1
+  while (hits) {
+    const int e = __ffs(hits) - 1;
+    hits &= hits - 1;
+    const int at = atomicAdd(&pool.n, 1);
+    const int idx = r.index(v0 + e / Row::VE * step) + e % Row::VE;
+    if (at < kLpPool) pool.key[at] = lp_key(value(e), idx);
+  }
+}
+
+// The best 32 of the pool, one key to a lane of warp 0. Each warp sorts every WARPS-th run of 32.
+template <int WARPS>
+__device__ __forceinline__ uint64_t lp_pool_top(const LpPool &pool, int n, uint64_t (&s_top)[WARPS][32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint64_t top = 0;
+  for (int i = 32 * warp; i < n; i += 32 * WARPS) {
+    const uint64_t c = warp_sort(i + lane < n ? pool.key[i + lane] : 0);
+    top = i == 32 * warp ? c : warp_merge(top, c);
+  }
+  const int lists = min(WARPS, (n + 31) / 32);
+  if (lists <= 1) return top;
+  s_top[warp][lane] = top;
+  for (int h = WARPS / 2; h > 0; h >>= 1) {
+    __syncthreads();
+    if (warp < h && warp + h < lists) {
+      top = warp_merge(top, s_top[warp + h][lane]);
+      s_top[warp][lane] = top;
+    }
+  }
+  return top;
+}
+
+// The next float above x (finite).
+__device__ __forceinline__ float lp_above(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return __uint_as_float(b >> 31 ? b - 1 : b + 1);
 }
 
 struct LpPart {
@@ -418,25 +511,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   using Row = LpRow<T>;
   constexpr int VE = Row::VE, NV = kLpPartLogits / VE, WARPS = THREADS / 32;
   constexpr int PER_GROUP = THREADS / 32;  // threads of one of the 32 groups
-  constexpr int CAP = WARPS * 64;          // gathered candidates; more: each warp filters its own
   __shared__ float s_max[32];
   __shared__ float2 s_sum[WARPS];
-  __shared__ uint64_t s_cand[CAP];
+  __shared__ LpPool s_pool;
   __shared__ uint64_t s_top[WARPS][32];
   __shared__ LpPart s_parts[kLpMaxCluster];
-  __shared__ int s_n;
   const int ranks = int(cooperative_groups::this_cluster().num_blocks());
   const int rank = int(cooperative_groups::this_cluster().block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.top_k;
   lp_cluster_arrive();
   if (tid == 0) {
     pdl_trigger();
-    s_n = 0;
+    s_pool.n = 0;
   }
   pdl_wait();
   const int64_t row = blockIdx.x / ranks;
   const Row r(p, row);
-  const int64_t per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
+  const int per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
   uint4 raw[NV];
   r.load_tile(raw, v0, v0 + tid, THREADS, v1);
   float gm[kLpPartLogits / 8];
@@ -448,18 +539,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   __syncthreads();
 
   // Each warp by itself: the part's maximum and the bound of its k-th largest.
-  const float sorted = warp_sort(s_max[lane]);
-  m = __shfl_sync(0xffffffffu, sorted, 0);
-  if (K > 0 && m > neg_inf()) {
+  m = s_max[lane];
+  if (K > 0) {
+    const float sorted = warp_sort(m);
+    m = __shfl_sync(0xffffffffu, sorted, 0);
     const float bound = fmaxf(__shfl_sync(0xffffffffu, sorted, K - 1), -3.402823466e38f);
-    uint32_t hits = lp_hits<T>(raw, gm, bound);
-    while (hits) {
-      const int e = __ffs(hits) - 1;
-      hits &= hits - 1;
-      const int idx = r.index(v0 + (e / VE) * THREADS + tid) + e % VE;
-      const int at = atomicAdd(&s_n, 1);
-      if (at < CAP) s_cand[at] = lp_key(r.at(idx), idx);
-    }
+    lp_pool_add(s_pool, lp_hits<T>(raw, gm, bound), LpPicked<T, NV>{raw}, r, v0 + tid, THREADS);
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
   float z = 0.f, w = 0.f;
   lp_sums<T>(raw, m, z, w);
@@ -471,24 +559,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   if (lane == 0) s_sum[warp] = make_float2(z, w);
   __syncthreads();
 
-  const int n = s_n;
+  const int n = s_pool.n;
   uint64_t top = 0;
-  if (n > CAP) {  // many equal logits: the warps' own lists, which drop ties past the k-th
+  if (n > kLpPool) {  // many equal logits: the warps' own lists, which drop ties past the k-th
+    static_assert(WARPS * 64 <= kLpPool, "the lists' candidates reuse the pool");
     LpList list;
-    list.cand = s_cand + warp * 64;
-    __syncthreads();  // everyone has read s_n; s_cand is rewritten
+    list.cand = s_pool.key + warp * 64;
     list.at_least(__shfl_sync(0xffffffffu, warp_sort(tm), K - 1));
-    list.gather(lp_hits<T>(raw, gm, list.fbound), r, v0 + tid, THREADS, K);
+    list.gather(lp_hits<T>(raw, gm, list.fbound), LpPicked<T, NV>{raw}, r, v0 + tid, THREADS, K);
     if (list.n > 0) list.flush(list.n, K);
     s_top[warp][lane] = list.mine;
     __syncthreads();
     if (warp == 0)
       for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
-  } else if (warp == 0) {
-    for (int i = 0; i < n; i += 32) {
-      const uint64_t c = warp_sort(i + lane < n ? s_cand[i + lane] : 0);
-      top = i ? warp_merge(top, c) : c;
-    }
+  } else {
+    top = lp_pool_top<WARPS>(s_pool, n, s_top);
   }
   LpState st{m, 0.f, 0.f};
 #pragma unroll
@@ -499,11 +584,36 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   lp_finish<T>(p, r.x, row, st, top, s_parts);
 }
 
+// A part once more, with a list a warp (the pool was too small). Out of line: its registers are not
+// the streaming loop's.
+template <typename T>
+__device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, float bound, uint64_t *cand,
+                                           uint4 *stash, int K) {
+  constexpr int THREADS = kLpStreamThreads, NV = 4;
+  const int tid = threadIdx.x;
+  LpList list;
+  list.cand = cand;
+  list.at_least(bound);
+  for (int vt = v0; vt < v1; vt += THREADS * NV) {
+    uint4 raw[NV];
+    r.load_tile(raw, vt, vt + tid, THREADS, v1);
+    float gm[NV * 2 / sizeof(T)];
+    lp_maxima<T>(raw, gm);
+    // A key already in the list has a lower index than any of this tile: equal logits are out.
+    const float pass = list.listed ? lp_above(list.fbound) : list.fbound;
+    const uint32_t hits = lp_hits<T>(raw, gm, pass);
+    list.gather(hits, LpStash<T, NV>(stash, raw), r, vt + tid, THREADS, K);
+  }
+  if (list.n > 0) list.flush(list.n, K);
+  return list.mine;
+}
+
 // ---- stream kernel ------------------------------------------------------------------------------
 // Tiles of 64 bytes a thread, the next one in flight. The 32 groups of the CTA (eight lanes each)
 // keep their running maxima in shared memory, and the warps take a new bound from them after tiles
 // 1, 2, 4, 8, ...: without a barrier but the first, for maxima that a warp sees too early are still
-// a lower bound. About 32 ln(32 / (32 - k)) / 8 logits a warp pass in each doubling.
+// a lower bound. About 32 ln(32 / (32 - k)) logits pass in each doubling. Where more than the pool
+// holds pass (ascending rows, many equal logits) the part is read a second time, with a list a warp.
 template <typename T>
 __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(const LogprobParams p) {
   using Row = LpRow<T>;
@@ -511,25 +621,28 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
   constexpr int THREADS = kLpStreamThreads, WARPS = THREADS / 32;
   __shared__ LpState s_state[WARPS];
   __shared__ volatile float s_max[32];
+  __shared__ uint4 s_stash[WARPS][NV * 32];
+  __shared__ LpPool s_pool;
   __shared__ uint64_t s_top[WARPS][32];
-  __shared__ uint64_t s_cand[WARPS][64];
   __shared__ LpPart s_parts[kLpMaxCluster];
   const int ranks = int(cooperative_groups::this_cluster().num_blocks());
   const int rank = int(cooperative_groups::this_cluster().block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.top_k;
   lp_cluster_arrive();
-  if (tid == 0) pdl_trigger();
+  if (tid == 0) {
+    pdl_trigger();
+    s_pool.n = 0;
+  }
   pdl_wait();
   const int64_t row = blockIdx.x / ranks;
   const Row r(p, row);
-  const int64_t per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
+  const int per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
   LpState st{neg_inf(), 0.f, 0.f};
-  LpList list;
-  list.cand = s_cand[warp];
+  float bound = -3.402823466e38f;  // no -inf passes
   uint4 next[NV];
   r.load_tile(next, v0, v0 + tid, THREADS, v1);
   int tile = 0;
-  for (int64_t vt = v0; vt < v1; vt += THREADS * NV, ++tile) {
+  for (int vt = v0; vt < v1; vt += THREADS * NV, ++tile) {
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = next[i];
@@ -547,26 +660,40 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
         if (lane % 8 == 0) s_max[tid / 8] = m;
         if (tile == 0) __syncthreads();
         __syncwarp();
-        list.at_least(__shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
+        bound = fmaxf(bound, __shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
       }
-      if (__any_sync(0xffffffffu, tm >= list.fbound))
-        list.gather(lp_hits<T>(raw, gm, list.fbound), r, vt + tid, THREADS, K);
+      if (__any_sync(0xffffffffu, tm >= bound)) {
+        const LpStash<T, NV> stash(s_stash[warp], raw);
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+          const uint4 one[1] = {stash.vector(i)};
+          uint32_t hits = 0;
+#pragma unroll
+          for (int j = 0; j < VE; j += 2) {
+            const float2 x = lp_pair<T>(one, j);
+            if (x.x >= bound) hits |= 1u << j;
+            if (x.y >= bound) hits |= 2u << j;
+          }
+          lp_pool_add(s_pool, hits, LpPicked<T, 1>{one}, r, vt + tid + i * THREADS, 0);
+        }
+      }
     }
   }
-  if (K > 0 && list.n > 0) list.flush(list.n, K);
   st = lp_warp_join(st);
   if (lane == 0) s_state[warp] = st;
-  s_top[warp][lane] = list.mine;
   __syncthreads();
-  if (K > 0) {
-#pragma unroll
-    for (int n = WARPS / 2; n > 0; n >>= 1) {
-      if (warp < n) s_top[warp][lane] = warp_merge(s_top[warp][lane], s_top[warp + n][lane]);
-      __syncthreads();
-    }
+  const int n = s_pool.n;
+  uint64_t top = 0;
+  if (n > kLpPool) {
+    s_top[warp][lane] = lp_reread<T>(r, v0, v1, bound, s_pool.key + warp * 64, s_stash[warp], K);
+    __syncthreads();
+    if (warp == 0)
+      for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
+  } else {
+    top = lp_pool_top<WARPS>(s_pool, n, s_top);
   }
   st = lp_warp_join(lane < WARPS ? s_state[lane] : LpState{neg_inf(), 0.f, 0.f});
-  lp_finish<T>(p, r.x, row, st, s_top[0][lane], s_parts);
+  lp_finish<T>(p, r.x, row, st, top, s_parts);
 }
 
 }  // namespace fa
