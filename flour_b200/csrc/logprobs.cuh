@@ -239,71 +239,67 @@ template <typename T> struct LpRow {
   __device__ __forceinline__ int index(int v) const { return v * VE - off; }
 };
 
-// Logit e of the vectors, e at run time: selects, no memory.
+// The largest logit of each vector, and of all; -inf where there is no number. 16-bit ones are
+// compared two at a time.
 template <typename T, int NV>
-__device__ __forceinline__ float lp_pick(const uint4 (&raw)[NV], int e) {
-  constexpr int VE = 16 / sizeof(T);
-  uint4 v = raw[0];
+__device__ __forceinline__ float lp_maxima(const uint4 (&raw)[NV], float (&vm)[NV]) {
+  float tm = neg_inf();
 #pragma unroll
-  for (int i = 1; i < NV; ++i)
-    if (e / VE == i) v = raw[i];
-  const int b = e % VE * sizeof(T);  // byte in the vector
-  const uint32_t w = b < 8 ? (b < 4 ? v.x : v.y) : (b < 12 ? v.z : v.w);
-  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
-  else return (b & 2) ? unpack2<T>(w).y : unpack2<T>(w).x;
-}
-
-// The same through shared memory, for the loop that has no registers to spare: a lane writes its
-// vectors to places of its own and reads one logit back.
-template <typename T, int NV> struct LpStash {
-  T *mine;  // 16-byte places 512 bytes apart
-  __device__ __forceinline__ LpStash(uint4 *warp_base, const uint4 (&raw)[NV]) {
-    uint4 *at = warp_base + (threadIdx.x & 31);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) at[32 * i] = raw[i];
-    mine = reinterpret_cast<T *>(at);
-  }
-  __device__ __forceinline__ uint4 vector(int i) const {
-    return *reinterpret_cast<const uint4 *>(mine + i * (32 * 16 / int(sizeof(T))));
-  }
-  __device__ __forceinline__ float operator()(int e) const {
-    constexpr int VE = 16 / sizeof(T);
-    return Elem<T>::to_f(mine[(e / VE) * (32 * VE) + e % VE]);
-  }
-};
-template <typename T, int NV> struct LpPicked {
-  const uint4 (&raw)[NV];
-  __device__ __forceinline__ float operator()(int e) const { return lp_pick<T>(raw, e); }
-};
-
-// Maxima of eight logits each, and of all; -inf where there is no number. 16-bit ones are compared
-// two at a time.
-template <typename T, int NV>
-__device__ __forceinline__ float lp_maxima(const uint4 (&raw)[NV], float (&gm)[NV * 2 / sizeof(T)]) {
-  constexpr int G = NV * 2 / sizeof(T);
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
+  for (int i = 0; i < NV; ++i) {
     if constexpr (sizeof(T) == 2) {
       using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-      const T2 *w = reinterpret_cast<const T2 *>(&raw[g]);
+      const T2 *w = reinterpret_cast<const T2 *>(&raw[i]);
       const T2 m2 = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
       const float2 m = unpack2<T>(*reinterpret_cast<const uint32_t *>(&m2));
-      gm[g] = fmaxf(fmaxf(m.x, m.y), neg_inf());
+      vm[i] = fmaxf(m.x, m.y);
     } else {
-      float m = neg_inf();
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float2 x = lp_pair<T>(raw, 8 * g + j);
-        m = fmaxf(m, fmaxf(x.x, x.y));
-      }
-      gm[g] = m;
+      const float2 a = lp_pair<T>(raw, i * 4), b = lp_pair<T>(raw, i * 4 + 2);
+      vm[i] = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
     }
+    tm = fmaxf(tm, vm[i]);
   }
-  float tm = gm[0];
-#pragma unroll
-  for (int g = 1; g < G; ++g) tm = fmaxf(tm, gm[g]);
   return tm;
 }
+
+// This lane's logits that are >= bound, one at a time. Short loops over selected registers: updates
+// unrolled over the tile miss the instruction cache, and few tiles take them.
+template <typename T, int NV> struct LpHits {
+  static constexpr int VE = 16 / sizeof(T);
+  uint32_t vecs = 0, bits = 0;  // vectors not yet looked at, hits in the current one
+  uint4 one[1];
+  int vec = 0;
+  __device__ __forceinline__ LpHits(const float (&vm)[NV], float bound) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (vm[i] >= bound) vecs |= 1u << i;
+  }
+  // The next hit: its value and number e (logit e % VE of vector e / VE); false when there is none.
+  __device__ __forceinline__ bool next(const uint4 (&raw)[NV], float bound, float &x, int &e) {
+    if (bits == 0) {
+      if (vecs == 0) return false;
+      vec = __ffs(vecs) - 1;
+      vecs &= vecs - 1;
+      one[0] = raw[0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i)
+        if (vec == i) one[0] = raw[i];
+#pragma unroll
+      for (int j = 0; j < VE; j += 2) {
+        const float2 p = lp_pair<T>(one, j);
+        if (p.x >= bound) bits |= 1u << j;
+        if (p.y >= bound) bits |= 2u << j;
+      }
+    }
+    const int j = __ffs(bits) - 1;  // a vector's maximum is a hit
+    bits &= bits - 1;
+    e = vec * VE + j;
+    const int b = j * int(sizeof(T));
+    const uint32_t w = b < 8 ? (b < 4 ? one[0].x : one[0].y) : (b < 12 ? one[0].z : one[0].w);
+    if constexpr (sizeof(T) == 4) x = __uint_as_float(w);
+    else x = (b & 2) ? unpack2<T>(w).y : unpack2<T>(w).x;
+    return true;
+  }
+};
 
 // The warp's list `mine` with its n <= 32 gathered candidates. Out of line: one copy of the sort.
 __device__ __noinline__ uint64_t lp_take(uint64_t mine, const uint64_t *cand, int n) {
@@ -338,19 +334,19 @@ struct LpList {
       listed = true;
     }
   }
-  // Gathers the logits of a tile that pass the bound. hits: one bit per logit of this lane, bit e
-  // for logit e % VE of vector v0 + (e / VE) * step.
-  template <class Value, class Row>
-  __device__ __forceinline__ void gather(uint32_t hits, const Value &value, const Row &r, int v0, int step, int k) {
+  // Gathers the logits of a tile that are >= pass. Logit e is e % VE of vector v0 + e / VE * step.
+  template <typename T, int NV>
+  __device__ __forceinline__ void gather(const uint4 (&raw)[NV], const float (&vm)[NV], float pass,
+                                         const LpRow<T> &r, int v0, int step, int k) {
     const int lane = threadIdx.x & 31;
-    while (__any_sync(0xffffffffu, hits != 0)) {
+    LpHits<T, NV> hits(vm, pass);
+    while (true) {
+      float x;
+      int e;
       uint64_t key = 0;
-      if (hits) {
-        const int e = __ffs(hits) - 1;
-        hits &= hits - 1;
-        const int idx = r.index(v0 + e / Row::VE * step) + e % Row::VE;
-        key = lp_key(value(e), idx);
-      }
+      const bool has = hits.next(raw, pass, x, e);
+      if (has) key = lp_key(x, r.index(v0 + e / LpRow<T>::VE * step) + e % LpRow<T>::VE);
+      if (!__any_sync(0xffffffffu, has)) break;
       const uint32_t mask = __ballot_sync(0xffffffffu, key > bound);
       if (key > bound) cand[n + __popc(mask & ((1u << lane) - 1u))] = key;
       n += __popc(mask);
@@ -364,24 +360,6 @@ struct LpList {
   }
 };
 
-// Bits of the logits that are >= bound, by eights that hold one.
-template <typename T, int NV>
-__device__ __forceinline__ uint32_t lp_hits(const uint4 (&raw)[NV], const float (&gm)[NV * 2 / sizeof(T)],
-                                            float bound) {
-  uint32_t hits = 0;
-#pragma unroll
-  for (int g = 0; g < NV * 2 / int(sizeof(T)); ++g) {
-    if (!__any_sync(0xffffffffu, gm[g] >= bound)) continue;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float2 x = lp_pair<T>(raw, 8 * g + j);
-      if (x.x >= bound) hits |= 1u << (8 * g + j);
-      if (x.y >= bound) hits |= 2u << (8 * g + j);
-    }
-  }
-  return hits;
-}
-
 // The CTA's candidates: keys of the logits that passed the bound when their tile was read. One
 // that comes when the pool is full is counted only, and the row's part is read again with lists.
 constexpr int kLpPool = 1024;
@@ -390,17 +368,17 @@ struct LpPool {
   int n;
 };
 
-// Each lane takes its hits one by one: a short loop, for unrolled updates miss the instruction cache.
-template <class Value, class Row>
-__device__ __forceinline__ void lp_pool_add(LpPool &pool, uint32_t hits, const Value &value, const Row &r,
-                                            int v0, int step) {
+template <typename T, int NV>
+__device__ __forceinline__ void lp_pool_add(LpPool &pool, const uint4 (&raw)[NV], const float (&vm)[NV],
+                                            float bound, const LpRow<T> &r, int v0, int step) {
+  LpHits<T, NV> hits(vm, bound);
+  float x;
+  int e;
 #pragma unroll 1
-  while (hits) {
-    const int e = __ffs(hits) - 1;
-    hits &= hits - 1;
+  while (hits.next(raw, bound, x, e)) {
     const int at = atomicAdd(&pool.n, 1);
-    const int idx = r.index(v0 + e / Row::VE * step) + e % Row::VE;
-    if (at < kLpPool) pool.key[at] = lp_key(value(e), idx);
+    if (at < kLpPool)
+      pool.key[at] = lp_key(x, r.index(v0 + e / LpRow<T>::VE * step) + e % LpRow<T>::VE);
   }
 }
 
@@ -530,8 +508,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
   const int per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
   uint4 raw[NV];
   r.load_tile(raw, v0, v0 + tid, THREADS, v1);
-  float gm[kLpPartLogits / 8];
-  const float tm = lp_maxima<T>(raw, gm);
+  float vm[NV];
+  const float tm = lp_maxima<T>(raw, vm);
   float m = tm;
 #pragma unroll
   for (int o = 1; o < PER_GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -544,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     const float sorted = warp_sort(m);
     m = __shfl_sync(0xffffffffu, sorted, 0);
     const float bound = fmaxf(__shfl_sync(0xffffffffu, sorted, K - 1), -3.402823466e38f);
-    lp_pool_add(s_pool, lp_hits<T>(raw, gm, bound), LpPicked<T, NV>{raw}, r, v0 + tid, THREADS);
+    lp_pool_add(s_pool, raw, vm, bound, r, v0 + tid, THREADS);
   } else {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -566,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     LpList list;
     list.cand = s_pool.key + warp * 64;
     list.at_least(__shfl_sync(0xffffffffu, warp_sort(tm), K - 1));
-    list.gather(lp_hits<T>(raw, gm, list.fbound), LpPicked<T, NV>{raw}, r, v0 + tid, THREADS, K);
+    list.gather(raw, vm, list.fbound, r, v0 + tid, THREADS, K);
     if (list.n > 0) list.flush(list.n, K);
     s_top[warp][lane] = list.mine;
     __syncthreads();
@@ -588,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
 // the streaming loop's.
 template <typename T>
 __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, float bound, uint64_t *cand,
-                                           uint4 *stash, int K) {
+                                           int K) {
   constexpr int THREADS = kLpStreamThreads, NV = 4;
   const int tid = threadIdx.x;
   LpList list;
@@ -597,12 +575,10 @@ __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, flo
   for (int vt = v0; vt < v1; vt += THREADS * NV) {
     uint4 raw[NV];
     r.load_tile(raw, vt, vt + tid, THREADS, v1);
-    float gm[NV * 2 / sizeof(T)];
-    lp_maxima<T>(raw, gm);
+    float vm[NV];
+    lp_maxima<T>(raw, vm);
     // A key already in the list has a lower index than any of this tile: equal logits are out.
-    const float pass = list.listed ? lp_above(list.fbound) : list.fbound;
-    const uint32_t hits = lp_hits<T>(raw, gm, pass);
-    list.gather(hits, LpStash<T, NV>(stash, raw), r, vt + tid, THREADS, K);
+    list.gather(raw, vm, list.listed ? lp_above(list.fbound) : list.fbound, r, vt + tid, THREADS, K);
   }
   if (list.n > 0) list.flush(list.n, K);
   return list.mine;
@@ -617,11 +593,10 @@ __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, flo
 template <typename T>
 __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(const LogprobParams p) {
   using Row = LpRow<T>;
-  constexpr int VE = Row::VE, NV = 4, N = NV * VE;
+  constexpr int NV = 4;
   constexpr int THREADS = kLpStreamThreads, WARPS = THREADS / 32;
   __shared__ LpState s_state[WARPS];
   __shared__ volatile float s_max[32];
-  __shared__ uint4 s_stash[WARPS][NV * 32];
   __shared__ LpPool s_pool;
   __shared__ uint64_t s_top[WARPS][32];
   __shared__ LpPart s_parts[kLpMaxCluster];
@@ -648,10 +623,9 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
     for (int i = 0; i < NV; ++i) raw[i] = next[i];
     if (vt + THREADS * NV < v1)
       r.load_tile(next, vt + THREADS * NV, vt + THREADS * NV + tid, THREADS, v1);
-    float gm[N / 8];
-    const float tm = lp_maxima<T>(raw, gm);
+    float vm[NV];
+    const float tm = lp_maxima<T>(raw, vm);
     if (tm > st.m) lp_shift(st, tm);
-    lp_sums<T>(raw, st.m, st.z, st.w);
     if (K > 0) {
       if ((tile & (tile + 1)) == 0) {
         float m = st.m;
@@ -662,22 +636,9 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
         __syncwarp();
         bound = fmaxf(bound, __shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
       }
-      if (__any_sync(0xffffffffu, tm >= bound)) {
-        const LpStash<T, NV> stash(s_stash[warp], raw);
-#pragma unroll 1
-        for (int i = 0; i < NV; ++i) {
-          const uint4 one[1] = {stash.vector(i)};
-          uint32_t hits = 0;
-#pragma unroll
-          for (int j = 0; j < VE; j += 2) {
-            const float2 x = lp_pair<T>(one, j);
-            if (x.x >= bound) hits |= 1u << j;
-            if (x.y >= bound) hits |= 2u << j;
-          }
-          lp_pool_add(s_pool, hits, LpPicked<T, 1>{one}, r, vt + tid + i * THREADS, 0);
-        }
-      }
+      if (tm >= bound) lp_pool_add(s_pool, raw, vm, bound, r, vt + tid, THREADS);
     }
+    lp_sums<T>(raw, st.m, st.z, st.w);
   }
   st = lp_warp_join(st);
   if (lane == 0) s_state[warp] = st;
@@ -685,7 +646,7 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
   const int n = s_pool.n;
   uint64_t top = 0;
   if (n > kLpPool) {
-    s_top[warp][lane] = lp_reread<T>(r, v0, v1, bound, s_pool.key + warp * 64, s_stash[warp], K);
+    s_top[warp][lane] = lp_reread<T>(r, v0, v1, bound, s_pool.key + warp * 64, K);
     __syncthreads();
     if (warp == 0)
       for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
