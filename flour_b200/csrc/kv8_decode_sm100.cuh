@@ -51,8 +51,13 @@ struct Kv8DecodeSmem {
                 "reduction scratch must fit in the ring");
 };
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  mma16816<__half>(c, a, b0, b1);
+// c = a b (no accumulator to clear first).
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 template <typename T, class F, int HD, int NSTAGE>
@@ -179,19 +184,24 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   const int l_xor = HD == 128 ? (l_tok & 7) : ((l_tok >> 1) & 3);
   auto at = [&](int c) { return uint32_t(l_tok * HD + (((c + l_hi) ^ l_xor) << 4)); };
 
+  // Two accumulators, so that a page's products are two chains of CH / 2.
   auto scores = [&](uint32_t kb, float (&c)[4]) {
-    c[0] = c[1] = c[2] = c[3] = 0.f;
+    float d[4];
 #pragma unroll
     for (int ch = 0; ch < CH; ch += 2) {
       uint32_t r[4], a[4];
       ldsm_x4(kb + at(ch), r);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        unpack4<F>(r[2 * e], a[0], a[2]);
-        unpack4<F>(r[2 * e + 1], a[1], a[3]);
-        mma_f16(c, a, qb[ch + e][0], qb[ch + e][1]);
-      }
+      unpack4<F>(r[0], a[0], a[2]);
+      unpack4<F>(r[1], a[1], a[3]);
+      if (ch == 0) mma_f16_zero(c, a, qb[ch][0], qb[ch][1]);
+      else mma16816<__half>(c, a, qb[ch][0], qb[ch][1]);
+      unpack4<F>(r[2], a[0], a[2]);
+      unpack4<F>(r[3], a[1], a[3]);
+      if (ch == 0) mma_f16_zero(d, a, qb[ch + 1][0], qb[ch + 1][1]);
+      else mma16816<__half>(d, a, qb[ch + 1][0], qb[ch + 1][1]);
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] += d[e];
   };
   // Scaled scores of a page whose first token is tok0; tokens past the context are -inf.
   auto finish = [&](float (&c)[4], float ks, int tok0) {
@@ -211,20 +221,23 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
       break;
     }
     const int j = 2 * (warp + i * kDecodeWarps);
-    const bool two = j + 1 < npg;
     const int tok0 = (pg0 + j) * kPage;
     const uint32_t kb = ring + st * S::kStageBytes, vb = kb + 2 * S::kPageBytes;
-    const float vs0 = s_vs[j], vs1 = two ? s_vs[j + 1] : vs0;
+    const bool two = j + 1 < npg;
+    if (ctx - tok0 < 2 * kPage) {
+      // The context ends in this step, the warp's last. What lies behind its last token (another
+      // owner's bytes, or a page that was not loaded) may be e4m3's NaN, which a probability of 0
+      // would not mask: clear those rows of V.
+      for (int x = (ctx - tok0) * (HD / 16) + lane; x < 2 * kPage * (HD / 16); x += 32)
+        *reinterpret_cast<uint4 *>(smem + (vb - smem_u32(smem)) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+    }
 
     float ca[4], cb[4];
     scores(kb, ca);
+    scores(kb + S::kPageBytes, cb);
     finish(ca, s_ks[j], tok0);
-    if (two) {
-      scores(kb + S::kPageBytes, cb);
-      finish(cb, s_ks[j + 1], tok0 + kPage);
-    } else {
-      cb[0] = cb[1] = cb[2] = cb[3] = neg_inf();
-    }
+    finish(cb, s_ks[j + 1], tok0 + kPage);
     float bm0 = fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]));
     float bm1 = fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]));
 #pragma unroll
@@ -232,76 +245,73 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
       bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, x));
       bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, x));
     }
-    const float mn0 = fmaxf(m0, bm0), mn1 = fmaxf(m1, bm1);
-    const float c0 = ex2(m0 - mn0), c1 = ex2(m1 - mn1);
+    if (__any_sync(0xffffffffu, bm0 > m0 || bm1 > m1)) {  // few steps raise a maximum late in a context
+      const float mn0 = fmaxf(m0, bm0), mn1 = fmaxf(m1, bm1);
+      const float c0 = ex2(m0 - mn0), c1 = ex2(m1 - mn1);
+      l0 *= c0;
+      l1 *= c1;
+      m0 = mn0;
+      m1 = mn1;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        o[c][0] *= c0;
+        o[c][1] *= c1;
+        o[c][2] *= c0;
+        o[c][3] *= c1;
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      ca[e] = ex2(ca[e] - (e & 1 ? mn1 : mn0));
-      cb[e] = ex2(cb[e] - (e & 1 ? mn1 : mn0));
+      ca[e] = ex2(ca[e] - (e & 1 ? m1 : m0));
+      cb[e] = ex2(cb[e] - (e & 1 ? m1 : m0));
     }
-    l0 = l0 * c0 + ((ca[0] + ca[2]) + (cb[0] + cb[2]));
-    l1 = l1 * c1 + ((ca[1] + ca[3]) + (cb[1] + cb[3]));
-    m0 = mn0;
-    m1 = mn1;
-    const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0], ca[1]));
-    const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2], ca[3]));
-    const uint32_t pb0 = movmatrix_t(pack2<__half>(cb[0], cb[1]));
-    const uint32_t pb1 = movmatrix_t(pack2<__half>(cb[2], cb[3]));
-    // Bytes behind the last token may be anything; an e4m3 NaN there would survive p = 0.
-    const int live = ctx - tok0;  // of this step's 32 tokens
-    const bool tail = std::is_same<F, E4m3>::value && live < 2 * kPage;
-    const bool same = vs0 == vs1;
-    auto keep = [&](int tok) {  // byte mask of tokens tok, tok + 1
-      return (tok < live ? 0x0000ffffu : 0u) | (tok + 1 < live ? 0xffff0000u : 0u);
-    };
+    l0 += (ca[0] + ca[2]) + (cb[0] + cb[2]);
+    l1 += (ca[1] + ca[3]) + (cb[1] + cb[3]);
+    // V's scales: the larger multiplies the step's product, the other page's probabilities take the
+    // ratio (a power of two for scales of one append history, and then exact).
+    const float vs0 = s_vs[j], vs1 = two ? s_vs[j + 1] : vs0;
+    const float vs = fmaxf(vs0, vs1);
+    const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.2e-38f;
+    const float inv = vs > 0.f ? 1.f / vs : 0.f;  // both scales 0: nothing to add
+    const float ra = apart ? 1.f : vs0 * inv, rb = apart ? 0.f : vs1 * inv;
+    const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0] * ra, ca[1] * ra));
+    const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2] * ra, ca[3] * ra));
+    const uint32_t pb0 = movmatrix_t(pack2<__half>(cb[0] * rb, cb[1] * rb));
+    const uint32_t pb1 = movmatrix_t(pack2<__half>(cb[2] * rb, cb[3] * rb));
+    // o += (P_a V_a + P_b V_b) factor
+    auto values = [&](uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, float factor) {
 #pragma unroll
-    for (int ch = 0; ch < CH; ch += 2) {
-      float ta[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      uint32_t r[4], a[4];
-      ldsm_x4_t(vb + at(ch), r);
-      if (tail) {
+      for (int ch = 0; ch < CH; ch += 2) {
+        float ta[2][4];
+        uint32_t ra4[4], rb4[4], a[4];
+        ldsm_x4_t(vb + at(ch), ra4);
+        ldsm_x4_t(vb + S::kPageBytes + at(ch), rb4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] &= keep(2 * t + (e & 1) * 8);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        unpack4_t<F>(r[2 * e], a[0], a[1]);
-        unpack4_t<F>(r[2 * e + 1], a[2], a[3]);
-        mma_f16(ta[e], a, pa0, pa1);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        o[ch + e][0] *= c0;
-        o[ch + e][1] *= c1;
-        o[ch + e][2] *= c0;
-        o[ch + e][3] *= c1;
-      }
-      if (!same) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            o[ch + e][q] = fmaf(ta[e][q], vs0, o[ch + e][q]);
-            ta[e][q] = 0.f;
-          }
-      }
-      if (two) {
-        ldsm_x4_t(vb + S::kPageBytes + at(ch), r);
-        if (tail) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] &= keep(kPage + 2 * t + (e & 1) * 8);
+        for (int e = 0; e < 2; ++e) {
+          unpack4_t<F>(ra4[2 * e], a[0], a[1]);
+          unpack4_t<F>(ra4[2 * e + 1], a[2], a[3]);
+          mma_f16_zero(ta[e], a, a0, a1);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          unpack4_t<F>(r[2 * e], a[0], a[1]);
-          unpack4_t<F>(r[2 * e + 1], a[2], a[3]);
-          mma_f16(ta[e], a, pb0, pb1);
+          unpack4_t<F>(rb4[2 * e], a[0], a[1]);
+          unpack4_t<F>(rb4[2 * e + 1], a[2], a[3]);
+          mma16816<__half>(ta[e], a, b0, b1);
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q], factor, o[ch + e][q]);
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q], vs1, o[ch + e][q]);
+    };
+    if (!apart) {
+      values(pa0, pa1, pb0, pb1, vs);
+    } else {  // more than a factor 64 between the pages: one after the other
+#pragma unroll 1
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t q0 = movmatrix_t(pack2<__half>(cb[0], cb[1])), q1 = movmatrix_t(pack2<__half>(cb[2], cb[3]));
+        values(x ? 0u : pa0, x ? 0u : pa1, x ? q0 : 0u, x ? q1 : 0u, x ? vs1 : vs0);
+      }
     }
     __syncwarp();
     if (lane == 0 && i + NSTAGE < n_my) issue(i + NSTAGE);

@@ -288,7 +288,7 @@ FA_API fa_status fa_paged_prefill(const fa_kv_layer *layer, const void *query, v
  *
  * One layer: K and V slabs of bytes [num_blocks, num_kv_heads, block_size, head_dim], laid out
  * like the 16-bit pool's, and for each an f32 scale per (block, KV head). A value is
- * byte * scale. Attention takes any finite scales (a cache quantised elsewhere); those that
+ * byte * scale. Attention takes any finite scales >= 0 (a cache quantised elsewhere); those that
  * fa_paged_append_kv8 writes are powers of two. Blocks are copied, exported and shared like any
  * block, with their scales: fa_copy_blocks takes the slabs as a 16-bit layer of head_dim / 2 and
  * the scales as an FA_F32 layer of block_size 1 and head_dim 1. */
