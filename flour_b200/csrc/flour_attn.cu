@@ -858,74 +858,98 @@ bool decode8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, const vo
   return (dtype == FA_BF16 || dtype == FA_F16) && L->block_size == fa::kPage &&
          (L->head_dim == 64 || L->head_dim == 128) && n_rep >= 1 && n_rep <= 8 &&
          int64_t(L->num_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
-         aligned(L->k_cache, 16) && aligned(L->v_cache, 16) && aligned(q, 8) && aligned(out, 2);
+         aligned(L->k_cache, 16) && aligned(L->v_cache, 16) && aligned(q, 8) && aligned(out, 8);
 }
 
 constexpr int kKv8Stages = 2;
 
 template <typename T, class F, int HD>
-fa_status launch_decode8_t(const fa::DecodeParams &p, const fa::Kv8Cache &c, const CUtensorMap &tk,
+fa_status launch_decode8_t(const fa::Kv8DecodeParams &p, int grid, const CUtensorMap &tk,
                            const CUtensorMap &tv, cudaStream_t stream) {
   using S = fa::Kv8DecodeSmem<HD, kKv8Stages>;
   auto kern = fa::kv8_decode_kernel<T, F, HD, kKv8Stages>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAlloc);
   if (e != cudaSuccess)
     return fail(FA_ECUDA, "paged_decode_kv8: set smem attribute: %s", cudaGetErrorString(e));
-  return launch_pdl("paged_decode_kv8", kern, dim3(p.max_splits, p.num_kv_heads, p.num_seqs),
-                    fa::kDecodeThreads, S::kAlloc, stream, 1, p, c, tk, tv);
+  return launch_pdl("paged_decode_kv8", kern, dim3(grid), fa::kDecodeThreads, S::kAlloc, stream, 1, p, tk, tv);
+}
+
+// CTAs of one launch: three per SM, fewer where even the longest possible batch has fewer ranges.
+// Sequences of one launch: as many as the kernel's prefix sums hold, and as their pairs fit 30 bits.
+struct Decode8Plan {
+  int seqs, grid;
+};
+Decode8Plan plan_decode8(int num_seqs, int num_kv_heads, int max_context_len) {
+  const int64_t pairs = int64_t(num_kv_heads) * ((max_context_len + 2 * fa::kPage - 1) / (2 * fa::kPage));
+  Decode8Plan d;
+  d.seqs = int(std::min<int64_t>(std::min(num_seqs, fa::kKv8MaxSeqs),
+                                 std::max<int64_t>(1, (int64_t(1) << 30) / std::max<int64_t>(1, pairs))));
+  const int64_t cta = fa::kDecodeWarps * fa::kKv8MinPairs;
+  d.grid = int(std::max<int64_t>(1, std::min<int64_t>(3 * sm_count(), (d.seqs * pairs + cta - 1) / cta)));
+  return d;
+}
+
+struct Decode8Workspace {
+  size_t lse_off, o_off, bytes;  // tickets at 0
+};
+Decode8Workspace decode8_workspace_layout(int num_heads, int num_kv_heads, int head_dim, const Decode8Plan &d) {
+  auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
+  Decode8Workspace w;
+  const size_t rows = size_t(d.grid) * fa::kKv8Pieces * (num_heads / num_kv_heads);
+  w.lse_off = r256(size_t(d.seqs) * num_kv_heads * 4);
+  w.o_off = w.lse_off + r256(rows * 4);
+  w.bytes = w.o_off + rows * head_dim * 4;
+  return w;
 }
 
 fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *ctx,
                          const int32_t *tables, int max_blocks, int num_seqs, int num_heads, int n_rep,
                          int max_context_len, float scale, void *ws, size_t ws_bytes, cudaStream_t stream) {
-  DecodePlan plan;
-  if (!plan_decode(num_seqs, L->num_kv_heads, max_context_len, &plan))
-    return fail(FA_EUNSUPPORTED, "paged_decode_kv8: context of %d tokens needs more than %d splits",
-                max_context_len, fa::kDecodeMaxSplits);
-  const DecodeWorkspace w =
-      decode_workspace_layout(num_seqs, num_heads, L->num_kv_heads, L->head_dim, plan);
-  if (w.bytes > 0) {
-    if (!ws) return fail(FA_EINVAL, "paged_decode_kv8: workspace is NULL but %zu bytes are needed", w.bytes);
-    if (ws_bytes < w.bytes)
-      return fail(FA_ERANGE, "paged_decode_kv8: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
-    if (!aligned(ws, 256)) return fail(FA_EINVAL, "paged_decode_kv8: workspace must be 256-byte aligned");
-    if (fa_status s = zero_stale_tickets(ws, w.lse_off, stream); s != FA_OK) return s;
-  }
-  fa::DecodeParams p{};
-  p.q = q;
-  p.out = out;
-  p.context_lens = ctx;
-  p.block_tables = tables;
+  const Decode8Plan plan = plan_decode8(num_seqs, L->num_kv_heads, max_context_len);
+  const Decode8Workspace w = decode8_workspace_layout(num_heads, L->num_kv_heads, L->head_dim, plan);
+  if (!ws) return fail(FA_EINVAL, "paged_decode_kv8: workspace is NULL but %zu bytes are needed", w.bytes);
+  if (ws_bytes < w.bytes)
+    return fail(FA_ERANGE, "paged_decode_kv8: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
+  if (!aligned(ws, 256)) return fail(FA_EINVAL, "paged_decode_kv8: workspace must be 256-byte aligned");
+  if (fa_status s = zero_stale_tickets(ws, w.lse_off, stream); s != FA_OK) return s;
+  fa::Kv8DecodeParams p{};
   char *wsb = static_cast<char *>(ws);
-  p.counters = w.bytes ? reinterpret_cast<int32_t *>(wsb + w.counters_off) : nullptr;
-  p.part_lse = w.bytes ? reinterpret_cast<float *>(wsb + w.lse_off) : nullptr;
-  p.part_o = w.bytes ? reinterpret_cast<float *>(wsb + w.o_off) : nullptr;
+  p.tickets = reinterpret_cast<int32_t *>(wsb);
+  p.piece_lse = reinterpret_cast<float *>(wsb + w.lse_off);
+  p.pieces = reinterpret_cast<float *>(wsb + w.o_off);
+  p.k_scale = L->k_scale;
+  p.v_scale = L->v_scale;
   p.max_blocks_per_seq = max_blocks;
-  p.num_seqs = num_seqs;
   p.num_heads = num_heads;
   p.num_kv_heads = L->num_kv_heads;
   p.n_rep = n_rep;
   p.num_blocks = L->num_blocks;
-  p.pages_per_split = plan.pages_per_split;
-  p.max_splits = plan.max_splits;
   p.max_context_len = max_context_len;
   p.scale_log2 = scale * fa::kLog2e;
-  p.scale = scale;
-  const fa::Kv8Cache c{L->k_scale, L->v_scale};
   const int64_t rows = int64_t(L->num_blocks) * L->num_kv_heads * L->block_size;
   CUtensorMap tk, tv;
   if (fa_status s = make_page8_map(&tk, L->k_cache, rows, L->head_dim); s != FA_OK) return s;
   if (fa_status s = make_page8_map(&tv, L->v_cache, rows, L->head_dim); s != FA_OK) return s;
-  return with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
-    using T = decltype(t);
-    using F = decltype(f);
-    if constexpr (sizeof(T) == 2) {
-      if (L->head_dim == 128) return launch_decode8_t<T, F, 128>(p, c, tk, tv, stream);
-      return launch_decode8_t<T, F, 64>(p, c, tk, tv, stream);
-    } else {
-      return fail(FA_EUNSUPPORTED, "paged_decode_kv8: f32 queries take the generic kernel");
-    }
-  });
+  const size_t row_bytes = size_t(num_heads) * L->head_dim * 2;
+  for (int s0 = 0; s0 < num_seqs; s0 += plan.seqs) {
+    p.num_seqs = std::min(plan.seqs, num_seqs - s0);
+    p.q = static_cast<const char *>(q) + s0 * row_bytes;
+    p.out = static_cast<char *>(out) + s0 * row_bytes;
+    p.context_lens = ctx + s0;
+    p.block_tables = tables + size_t(s0) * max_blocks;
+    const fa_status st = with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
+      using T = decltype(t);
+      using F = decltype(f);
+      if constexpr (sizeof(T) == 2) {
+        if (L->head_dim == 128) return launch_decode8_t<T, F, 128>(p, plan.grid, tk, tv, stream);
+        return launch_decode8_t<T, F, 64>(p, plan.grid, tk, tv, stream);
+      } else {
+        return fail(FA_EUNSUPPORTED, "paged_decode_kv8: f32 queries take the generic kernel");
+      }
+    });
+    if (st != FA_OK) return st;
+  }
+  return ok();
 }
 
 fa_status launch_generic8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *cu,
@@ -1627,7 +1651,12 @@ fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const 
 
 size_t fa_paged_decode_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                           int32_t head_dim, int32_t max_context_len) {
-  return fa_paged_attention_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len, 1);
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context_len <= 0 ||
+      num_heads % num_kv_heads != 0)
+    return 0;
+  return decode8_workspace_layout(num_heads, num_kv_heads, head_dim,
+                                  plan_decode8(num_seqs, num_kv_heads, max_context_len))
+      .bytes;
 }
 
 fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void *out, int32_t dtype,

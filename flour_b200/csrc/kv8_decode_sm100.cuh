@@ -5,10 +5,18 @@
 //
 // with k_j, v_j the bytes and ks(j), vs(j) the scales of position j's block and KV head.
 //
-// The split into (split, kv head, sequence) CTAs, the per-warp TMA rings, the online softmax and
-// the ticketed merge are those of the 16-bit decode (decode_sm100.cuh); half the bytes per token
-// leave half the time per token, so a ring step is two pages (32 tokens: one max, one exchange
-// over the lanes and one rescale of the accumulators for both).
+// Work. A step is a pair of pages (32 tokens) of one (sequence, KV head): one maximum, one exchange
+// over the lanes for both. All pairs of the batch, in order of (sequence, KV head, page), are cut
+// into equal contiguous ranges, one per warp, three CTAs of four warps per SM; a warp streams its
+// range through a ring of its own, across the ends of sequences, with no barrier to wait at. So
+// every SM has the same bytes to read whatever the lengths, and the latencies of a start (lengths,
+// block table, first bytes) are paid once a launch and not once a split: half the bytes of a
+// 16-bit cache leave half the time to hide them in. (The 16-bit decode's grid of splits measured
+// 63 us for 64 contexts of U[512, 4096] and 58 us for 59 of U[1, 6438]; see the figures below.)
+// A (sequence, KV head) that ends inside one range is written by its warp; the others leave pieces
+// (O / l, log2-sum-exp) in the workspace, which the CTA joins when its warps are done, and the last
+// CTA of a (sequence, KV head) to finish (a ticket, no waiting) joins the CTAs' pieces. The ranges
+// follow from the lengths alone, so results do not depend on timing.
 //
 // Bytes become f16 in registers, exactly (e4m3 and int8 are subsets of f16), and feed
 // mma.sync m16n8k16 with f32 accumulation:
@@ -20,9 +28,9 @@
 // q is divided by a power of two that brings each head's largest |q| into [1, 2), so that bf16
 // queries fit f16 (a value 2^-24 below its head's largest is lost, as it is in an f32 sum of this
 // length), and the factor returns with the score's scale. P is rounded to f16, which loses 8 times
-// less than the bf16 of the 16-bit decode. The scale of K multiplies a score in f32; the scale
-// of V multiplies the page's product in f32, two pages of one scale (powers of two: the usual
-// case) share an accumulator.
+// less than the bf16 of the 16-bit decode. The scale of K multiplies a score in f32; the larger of
+// the pair's two scales of V multiplies its product in f32, and the other page's probabilities take
+// the ratio (a power of two for scales of the append, and then exact).
 #pragma once
 
 #include "decode_sm100.cuh"
@@ -30,25 +38,49 @@
 
 namespace fa {
 
-struct Kv8Cache {
-  const float *k_scale;  // [num_blocks, num_kv_heads]
+constexpr int kKv8MaxSeqs = 384;   // sequences per launch (prefix sums and lengths in shared memory)
+constexpr int kKv8MinPairs = 4;    // a warp's range is at least this long
+constexpr int kKv8Direct = 8;      // CTAs that may share an item before each joins its own pieces
+constexpr int kKv8Pieces = 10;     // of a CTA in the workspace: 4 warps x (first, last), then its own two
+
+struct Kv8DecodeParams {
+  const void *q;                 // [num_seqs, num_heads, HD]
+  void *out;
+  const int32_t *context_lens;
+  const int32_t *block_tables;
+  const float *k_scale;          // [num_blocks, num_kv_heads]
   const float *v_scale;
+  int32_t *tickets;              // [num_seqs * num_kv_heads], zero between launches
+  float *pieces;                 // [gridDim.x][kKv8Pieces][n_rep][HD]
+  float *piece_lse;              // [gridDim.x][kKv8Pieces][n_rep]
+  int32_t max_blocks_per_seq;
+  int32_t num_seqs;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t n_rep;
+  int32_t num_blocks;
+  int32_t max_context_len;
+  float scale_log2;              // scale * log2(e)
+};
+
+// What a warp needs of 32 pairs of its range, filled ahead by one lane each.
+struct Kv8Window {
+  int32_t row[2][32];  // of the slab viewed as [rows, HD]; second page: -1 if the context ends before
+  float ks[2][32], vs[2][32];
 };
 
 template <int HD, int NSTAGE>
 struct Kv8DecodeSmem {
   static constexpr int kPageBytes = kPage * HD;               // K (or V) of one page
-  static constexpr int kStageBytes = 4 * kPageBytes;          // K, K, V, V of a step's two pages
+  static constexpr int kStageBytes = 4 * kPageBytes;          // K, K, V, V of a pair
   static constexpr int kRingBytes = kDecodeWarps * NSTAGE * kStageBytes;
-  static constexpr int kIdsOff = kRingBytes;
-  static constexpr int kKsOff = kIdsOff + kDecodeMaxPagesPerSplit * 4;
-  static constexpr int kVsOff = kKsOff + kDecodeMaxPagesPerSplit * 4;
-  static constexpr int kBarOff = kVsOff + kDecodeMaxPagesPerSplit * 4;
-  static constexpr int kFlagOff = kBarOff + kDecodeWarps * NSTAGE * 8;
-  static constexpr int kAlloc = kFlagOff + 16 + 1024;  // slack to align the base to 1024 B
-  static constexpr int kRedStride = HD + 4;            // reduction scratch over the drained ring
-  static_assert(kDecodeWarps * 8 * (kRedStride + 2) * 4 + 8 * kDecodeMaxSplits * 4 <= kRingBytes,
-                "reduction scratch must fit in the ring");
+  static constexpr int kWinOff = kRingBytes;
+  static constexpr int kOffsOff = kWinOff + kDecodeWarps * 2 * int(sizeof(Kv8Window));
+  static constexpr int kCtxOff = kOffsOff + (kKv8MaxSeqs + 4) * 4;
+  static constexpr int kBarOff = kCtxOff + kKv8MaxSeqs * 4;
+  static constexpr int kMiscOff = kBarOff + kDecodeWarps * NSTAGE * 8;
+  static constexpr int kAlloc = kMiscOff + 128 + 1024;  // slack to align the base to 1024 B
+  static_assert(3 * (kAlloc + 1024) <= 228 * 1024, "three CTAs per SM");
 };
 
 // c = a b (no accumulator to clear first).
@@ -62,121 +94,143 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint32_t (&a)[
 
 template <typename T, class F, int HD, int NSTAGE>
 __global__ void __launch_bounds__(kDecodeThreads, 3)
-    kv8_decode_kernel(const __grid_constant__ DecodeParams p, const Kv8Cache sc,
-                      const __grid_constant__ CUtensorMap tm_k,
+    kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v) {
   using S = Kv8DecodeSmem<HD, NSTAGE>;
   constexpr int CH = HD / 16;  // 16-byte chunks of a row = k16 steps of S = m16 tiles of O
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~uintptr_t(1023));
-  int32_t *s_ids = reinterpret_cast<int32_t *>(smem + S::kIdsOff);
-  float *s_ks = reinterpret_cast<float *>(smem + S::kKsOff);
-  float *s_vs = reinterpret_cast<float *>(smem + S::kVsOff);
+  Kv8Window *s_win = reinterpret_cast<Kv8Window *>(smem + S::kWinOff);
+  int32_t *offs = reinterpret_cast<int32_t *>(smem + S::kOffsOff);  // pairs of sequences < s
+  int32_t *s_ctx = reinterpret_cast<int32_t *>(smem + S::kCtxOff);
   uint64_t *s_bar = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
-  int32_t *s_flag = reinterpret_cast<int32_t *>(smem + S::kFlagOff);
+  int32_t *s_misc = reinterpret_cast<int32_t *>(smem + S::kMiscOff);  // scan sums, piece items, flag
 
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int n_rep = p.n_rep;
-  if (tid == 0) pdl_trigger();
-  pdl_wait();
-
-  const int ctx = p.context_lens[b];
-  if (ctx < 1 || ctx > p.max_context_len || int64_t(ctx) > int64_t(p.max_blocks_per_seq) * kPage) {
-    if (split == 0) {
-      if (tid == 0) report(FA_DEVERR_CONTEXT);
-      for (int x = tid; x < n_rep * HD; x += kDecodeThreads)
-        store_out<T>(p, b, kvh * n_rep + x / HD, HD, x % HD, 0.f);
-    }
-    return;
-  }
-  const int n_pages = (ctx + kPage - 1) / kPage;
-  const int n_splits = (n_pages + p.pages_per_split - 1) / p.pages_per_split;
-  if (split >= n_splits) return;
-  const int pg0 = split * p.pages_per_split;
-  const int npg = min(n_pages, pg0 + p.pages_per_split) - pg0;
-
+  const int n_rep = p.n_rep, H = p.num_kv_heads;
   if (tid == 0) {
+    pdl_trigger();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
 #pragma unroll
     for (int i = 0; i < kDecodeWarps * NSTAGE; ++i) mbar_init(smem_u32(&s_bar[i]), 1);
     fence_mbar_init();
   }
-  const int32_t *table = p.block_tables + size_t(b) * p.max_blocks_per_seq + pg0;
-  bool bad = false;
-  for (int i = tid; i < npg; i += kDecodeThreads) {
-    int id = table[i];
-    if (uint32_t(id) >= uint32_t(p.num_blocks)) { bad = true; id = 0; }
-    s_ids[i] = id;
-  }
-  if (bad) report(FA_DEVERR_BLOCK_ID);
-  __syncthreads();
+  pdl_wait();
 
-  // ---- per-warp stream of page pairs --------------------------------------------------------
-  const int n_pairs = (npg + 1) / 2;
-  const int n_my = n_pairs > warp ? (n_pairs - warp + kDecodeWarps - 1) / kDecodeWarps : 0;
+  // ---- prefix sums of the sequences' pairs; 128 sequences a turn ------------------------------
+  for (int s0 = 0, carry = 0; s0 < p.num_seqs; s0 += kDecodeThreads) {
+    const int s = s0 + tid;
+    int n = 0;
+    if (s < p.num_seqs) {
+      const int ctx = p.context_lens[s];
+      const bool ok = ctx >= 1 && ctx <= p.max_context_len &&
+                      int64_t(ctx) <= int64_t(p.max_blocks_per_seq) * kPage;
+      n = ok ? (ctx + 2 * kPage - 1) / (2 * kPage) : 0;
+      s_ctx[s] = ctx;
+      if (!ok && s % int(gridDim.x) == int(blockIdx.x)) {
+        // Nothing valid to attend to: one CTA zeroes the sequence's heads and reports.
+        report(FA_DEVERR_CONTEXT);
+        T *o = static_cast<T *>(p.out) + size_t(s) * p.num_heads * HD;
+        for (int x = 0; x < p.num_heads * HD; ++x) o[x] = Elem<T>::from_f(0.f);
+      }
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_misc[warp] = incl;
+    __syncthreads();
+    int base = carry, sum = carry;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      if (w < warp) base += s_misc[w];
+      sum += s_misc[w];
+    }
+    if (s < p.num_seqs) offs[s + 1] = base + incl;
+    carry = sum;
+    __syncthreads();
+  }
+  if (tid == 0) offs[0] = 0;
+  __syncthreads();
+  const int total = offs[p.num_seqs] * H;
+  const int workers = int(gridDim.x) * kDecodeWarps;
+  const int ppw = max(kKv8MinPairs, (total + workers - 1) / workers);  // pairs per warp
+  const int c0 = int(blockIdx.x) * (kDecodeWarps * ppw);
+  if (c0 >= total) return;
+  const int c1 = min(total, c0 + kDecodeWarps * ppw);
+  const int w0 = min(total, c0 + warp * ppw), n_my = min(total, w0 + ppw) - w0;
+
+  // Pair f of the flattened batch: its sequence, KV head, number in the (sequence, KV head) item.
+  struct Pair {
+    int s, kvh, j, of;
+  };
+  auto find = [&](int f) {
+    int lo = 0, hi = p.num_seqs;  // last s with H * offs[s] <= f (of those with pairs)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (offs[mid] * H <= f) lo = mid; else hi = mid;
+    }
+    const int np = offs[lo + 1] - offs[lo], rem = f - offs[lo] * H;
+    return Pair{lo, rem / np, rem % np, np};
+  };
+
+  // ---- this warp's stream -----------------------------------------------------------------------
   const uint32_t ring = smem_u32(smem) + warp * NSTAGE * S::kStageBytes;
   const uint32_t bar0 = smem_u32(&s_bar[warp * NSTAGE]);
   const uint64_t policy = policy_evict_first();
+  Kv8Window *win = s_win + warp * 2;
 
-  auto issue = [&](int i) {
-    const int st = i % NSTAGE, j = 2 * (warp + i * kDecodeWarps);
-    const uint32_t dst = ring + st * S::kStageBytes, bar = bar0 + st * 8;
-    const int n = min(2, npg - j);
-    mbar_arrive_expect_tx(bar, n * 2 * S::kPageBytes);
-    for (int x = 0; x < n; ++x) {
-      const int row = (s_ids[j + x] * p.num_kv_heads + kvh) * kPage;
-      tma_load_2d_hint(dst + x * S::kPageBytes, &tm_k, bar, 0, row, policy);
-      tma_load_2d_hint(dst + (2 + x) * S::kPageBytes, &tm_v, bar, 0, row, policy);
+  // Rows of window w go to shared memory at once; scales follow (fill_scales), behind the first loads.
+  int fill_at0 = 0, fill_at1 = 0;
+  auto fill_rows = [&](int w) {
+    const int i = 32 * w + lane;
+    if (i < n_my) {
+      const Pair pr = find(w0 + i);
+      const int32_t *table = p.block_tables + size_t(pr.s) * p.max_blocks_per_seq + 2 * pr.j;
+      const bool two = (2 * pr.j + 1) * kPage < s_ctx[pr.s];
+      int id0 = table[0], id1 = two ? table[1] : 0;
+      if (uint32_t(id0) >= uint32_t(p.num_blocks) || uint32_t(id1) >= uint32_t(p.num_blocks)) {
+        report(FA_DEVERR_BLOCK_ID);  // such a block is read as block 0
+        if (uint32_t(id0) >= uint32_t(p.num_blocks)) id0 = 0;
+        if (uint32_t(id1) >= uint32_t(p.num_blocks)) id1 = 0;
+      }
+      fill_at0 = id0 * H + pr.kvh;
+      fill_at1 = two ? id1 * H + pr.kvh : fill_at0;
+      win[w & 1].row[0][lane] = fill_at0 * kPage;
+      win[w & 1].row[1][lane] = two ? fill_at1 * kPage : -1;
     }
+    __syncwarp();
   };
-  if (lane == 0)
-    for (int i = 0; i < NSTAGE && i < n_my; ++i) issue(i);
-  // Scales arrive while the first pages do.
-  for (int i = tid; i < npg; i += kDecodeThreads) {
-    const size_t at = size_t(s_ids[i]) * p.num_kv_heads + kvh;
-    s_ks[i] = sc.k_scale[at];
-    s_vs[i] = sc.v_scale[at];
-  }
-
-  // Q^T fragments (n = head g): k = 2t, 2t+1 <-> dims 4t, 4t+1 of the chunk, k + 8 <-> dims + 2.
-  uint32_t qb[CH][2];
-  float f0, f1;  // score factors of heads 2t, 2t+1
-  {
-    const T *qrow = static_cast<const T *>(p.q) + (size_t(b) * p.num_heads + kvh * n_rep + g) * HD;
-    float2 v[CH][2];
-    float amax = 0.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      uint2 raw = make_uint2(0u, 0u);
-      if (g < n_rep) raw = *reinterpret_cast<const uint2 *>(qrow + c * 16 + 4 * t);
-      v[c][0] = unpack2<T>(raw.x);
-      v[c][1] = unpack2<T>(raw.y);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) amax = fmaxf(amax, fmaxf(fabsf(v[c][e].x), fabsf(v[c][e].y)));
+  auto fill_scales = [&](int w) {
+    if (32 * w + lane < n_my) {
+      win[w & 1].ks[0][lane] = p.k_scale[fill_at0];
+      win[w & 1].ks[1][lane] = p.k_scale[fill_at1];
+      win[w & 1].vs[0][lane] = p.v_scale[fill_at0];
+      win[w & 1].vs[1][lane] = p.v_scale[fill_at1];
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // 2^floor(log2 amax), kept where its reciprocal is a normal number too.
-    const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 3u), 251u);
-    const float up = __uint_as_float(ex << 23), down = __uint_as_float((254u - ex) << 23);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) qb[c][e] = pack2<__half>(v[c][e].x * down, v[c][e].y * down);
-    // Lane 4 h holds head h's factor.
-    f0 = __shfl_sync(0xffffffffu, up, 8 * t) * p.scale_log2;
-    f1 = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
+    __syncwarp();
+  };
+  auto issue = [&](int i) {
+    const Kv8Window &w = win[(i >> 5) & 1];
+    const int st = i % NSTAGE, r0 = w.row[0][i & 31], r1 = w.row[1][i & 31];
+    const uint32_t dst = ring + st * S::kStageBytes, bar = bar0 + st * 8;
+    mbar_arrive_expect_tx(bar, (r1 >= 0 ? 4 : 2) * S::kPageBytes);
+    tma_load_2d_hint(dst, &tm_k, bar, 0, r0, policy);
+    if (r1 >= 0) tma_load_2d_hint(dst + S::kPageBytes, &tm_k, bar, 0, r1, policy);
+    tma_load_2d_hint(dst + 2 * S::kPageBytes, &tm_v, bar, 0, r0, policy);
+    if (r1 >= 0) tma_load_2d_hint(dst + 3 * S::kPageBytes, &tm_v, bar, 0, r1, policy);
+  };
+  if (n_my > 0) {
+    fill_rows(0);
+    if (lane == 0)
+      for (int i = 0; i < NSTAGE && i < n_my; ++i) issue(i);
+    fill_scales(0);
   }
-  __syncthreads();  // scales are in shared memory
-
-  float m0 = neg_inf(), m1 = neg_inf(), l0 = 0.f, l1 = 0.f;  // heads 2t, 2t+1
-  float o[CH][4];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
 
   // This lane's ldmatrix row (token) and its swizzled chunk: 128-byte rows xor the chunk with
   // row & 7, 64-byte rows with (row >> 1) & 3.
@@ -184,231 +238,358 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   const int l_xor = HD == 128 ? (l_tok & 7) : ((l_tok >> 1) & 3);
   auto at = [&](int c) { return uint32_t(l_tok * HD + (((c + l_hi) ^ l_xor) << 4)); };
 
-  // Two accumulators, so that a page's products are two chains of CH / 2.
-  auto scores = [&](uint32_t kb, float (&c)[4]) {
-    float d[4];
-#pragma unroll
-    for (int ch = 0; ch < CH; ch += 2) {
-      uint32_t r[4], a[4];
-      ldsm_x4(kb + at(ch), r);
-      unpack4<F>(r[0], a[0], a[2]);
-      unpack4<F>(r[1], a[1], a[3]);
-      if (ch == 0) mma_f16_zero(c, a, qb[ch][0], qb[ch][1]);
-      else mma16816<__half>(c, a, qb[ch][0], qb[ch][1]);
-      unpack4<F>(r[2], a[0], a[2]);
-      unpack4<F>(r[3], a[1], a[3]);
-      if (ch == 0) mma_f16_zero(d, a, qb[ch + 1][0], qb[ch + 1][1]);
-      else mma16816<__half>(d, a, qb[ch + 1][0], qb[ch + 1][1]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] += d[e];
-  };
-  // Scaled scores of a page whose first token is tok0; tokens past the context are -inf.
-  auto finish = [&](float (&c)[4], float ks, int tok0) {
-    const float a0 = f0 * ks, a1 = f1 * ks;
-    const bool v0 = tok0 + g < ctx, v1 = tok0 + g + 8 < ctx;
-    c[0] = v0 ? c[0] * a0 : neg_inf();
-    c[1] = v0 ? c[1] * a1 : neg_inf();
-    c[2] = v1 ? c[2] * a0 : neg_inf();
-    c[3] = v1 ? c[3] * a1 : neg_inf();
-  };
+  int pieces[2] = {-1, -1};  // items of this warp's first and last piece
+  bool dead = false;         // a wait gave up: nothing more is loaded or computed
+  Pair pr = n_my > 0 ? find(w0) : Pair{};
+  for (int i = 0; i < n_my;) {
+    // ---- a segment: this warp's part of one (sequence, KV head) ------------------------------
+    const int seg = min(pr.of - pr.j, n_my - i);
+    const int ctx = s_ctx[pr.s];
+    const int hq0 = pr.kvh * n_rep;
 
-  int timed_out_at = -1;
-  for (int i = 0; i < n_my; ++i) {
-    const int st = i % NSTAGE;
-    if (!__all_sync(0xffffffffu, mbar_wait(bar0 + st * 8, (i / NSTAGE) & 1))) {
-      timed_out_at = i;
-      break;
-    }
-    const int j = 2 * (warp + i * kDecodeWarps);
-    const int tok0 = (pg0 + j) * kPage;
-    const uint32_t kb = ring + st * S::kStageBytes, vb = kb + 2 * S::kPageBytes;
-    const bool two = j + 1 < npg;
-    if (ctx - tok0 < 2 * kPage) {
-      // The context ends in this step, the warp's last. What lies behind its last token (another
-      // owner's bytes, or a page that was not loaded) may be e4m3's NaN, which a probability of 0
-      // would not mask: clear those rows of V.
-      for (int x = (ctx - tok0) * (HD / 16) + lane; x < 2 * kPage * (HD / 16); x += 32)
-        *reinterpret_cast<uint4 *>(smem + (vb - smem_u32(smem)) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-      __syncwarp();
-    }
-
-    float ca[4], cb[4];
-    scores(kb, ca);
-    scores(kb + S::kPageBytes, cb);
-    finish(ca, s_ks[j], tok0);
-    finish(cb, s_ks[j + 1], tok0 + kPage);
-    float bm0 = fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]));
-    float bm1 = fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]));
+    // Q^T fragments (n = head g): k = 2t, 2t+1 <-> dims 4t, 4t+1 of the chunk, k + 8 <-> dims + 2.
+    uint32_t qb[CH][2];
+    float f0, f1;  // score factors of heads 2t, 2t+1
+    {
+      const T *qrow = static_cast<const T *>(p.q) + (size_t(pr.s) * p.num_heads + hq0 + g) * HD;
+      uint2 raw[CH];
+      float amax = 0.f;
 #pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, x));
-      bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, x));
-    }
-    if (__any_sync(0xffffffffu, bm0 > m0 || bm1 > m1)) {  // few steps raise a maximum late in a context
-      const float mn0 = fmaxf(m0, bm0), mn1 = fmaxf(m1, bm1);
-      const float c0 = ex2(m0 - mn0), c1 = ex2(m1 - mn1);
-      l0 *= c0;
-      l1 *= c1;
-      m0 = mn0;
-      m1 = mn1;
+      for (int c = 0; c < CH; ++c)
+        raw[c] = g < n_rep ? *reinterpret_cast<const uint2 *>(qrow + c * 16 + 4 * t) : make_uint2(0u, 0u);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        o[c][0] *= c0;
-        o[c][1] *= c1;
-        o[c][2] *= c0;
-        o[c][3] *= c1;
+        const float2 a = unpack2<T>(raw[c].x), b = unpack2<T>(raw[c].y);
+        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
       }
-    }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // 2^floor(log2 amax), kept where its reciprocal is a normal number too.
+      const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 3u), 251u);
+      const float up = __uint_as_float(ex << 23), down = __uint_as_float((254u - ex) << 23);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      ca[e] = ex2(ca[e] - (e & 1 ? m1 : m0));
-      cb[e] = ex2(cb[e] - (e & 1 ? m1 : m0));
+      for (int c = 0; c < CH; ++c) {
+        const float2 a = unpack2<T>(raw[c].x), b = unpack2<T>(raw[c].y);
+        qb[c][0] = pack2<__half>(a.x * down, a.y * down);
+        qb[c][1] = pack2<__half>(b.x * down, b.y * down);
+      }
+      // Lane 4 h holds head h's factor.
+      f0 = __shfl_sync(0xffffffffu, up, 8 * t) * p.scale_log2;
+      f1 = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
     }
-    l0 += (ca[0] + ca[2]) + (cb[0] + cb[2]);
-    l1 += (ca[1] + ca[3]) + (cb[1] + cb[3]);
-    // V's scales: the larger multiplies the step's product, the other page's probabilities take the
-    // ratio (a power of two for scales of one append history, and then exact).
-    const float vs0 = s_vs[j], vs1 = two ? s_vs[j + 1] : vs0;
-    const float vs = fmaxf(vs0, vs1);
-    const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.2e-38f;
-    const float inv = vs > 0.f ? 1.f / vs : 0.f;  // both scales 0: nothing to add
-    const float ra = apart ? 1.f : vs0 * inv, rb = apart ? 0.f : vs1 * inv;
-    const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0] * ra, ca[1] * ra));
-    const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2] * ra, ca[3] * ra));
-    const uint32_t pb0 = movmatrix_t(pack2<__half>(cb[0] * rb, cb[1] * rb));
-    const uint32_t pb1 = movmatrix_t(pack2<__half>(cb[2] * rb, cb[3] * rb));
-    // o += (P_a V_a + P_b V_b) factor
-    auto values = [&](uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, float factor) {
+    Pair next{};
+    if (i + seg < n_my) {  // the next segment's queries, on their way while this one is worked on
+      next = find(w0 + i + seg);
+      const char *at = reinterpret_cast<const char *>(static_cast<const T *>(p.q) +
+                                                      (size_t(next.s) * p.num_heads + next.kvh * n_rep) * HD);
+      if (lane * 128 < n_rep * HD * 2) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + lane * 128));
+    }
+    float m0 = neg_inf(), m1 = neg_inf(), l0 = 0.f, l1 = 0.f;  // heads 2t, 2t+1
+    float o[CH][4];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+
+    // Two accumulators, so that a page's products are two chains of CH / 2.
+    auto scores = [&](uint32_t kb, float (&c)[4]) {
+      float d[4];
 #pragma unroll
       for (int ch = 0; ch < CH; ch += 2) {
-        float ta[2][4];
-        uint32_t ra4[4], rb4[4], a[4];
-        ldsm_x4_t(vb + at(ch), ra4);
-        ldsm_x4_t(vb + S::kPageBytes + at(ch), rb4);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          unpack4_t<F>(ra4[2 * e], a[0], a[1]);
-          unpack4_t<F>(ra4[2 * e + 1], a[2], a[3]);
-          mma_f16_zero(ta[e], a, a0, a1);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          unpack4_t<F>(rb4[2 * e], a[0], a[1]);
-          unpack4_t<F>(rb4[2 * e + 1], a[2], a[3]);
-          mma16816<__half>(ta[e], a, b0, b1);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q], factor, o[ch + e][q]);
+        uint32_t r[4], a[4];
+        ldsm_x4(kb + at(ch), r);
+        unpack4<F>(r[0], a[0], a[2]);
+        unpack4<F>(r[1], a[1], a[3]);
+        if (ch == 0) mma_f16_zero(c, a, qb[ch][0], qb[ch][1]);
+        else mma16816<__half>(c, a, qb[ch][0], qb[ch][1]);
+        unpack4<F>(r[2], a[0], a[2]);
+        unpack4<F>(r[3], a[1], a[3]);
+        if (ch == 0) mma_f16_zero(d, a, qb[ch + 1][0], qb[ch + 1][1]);
+        else mma16816<__half>(d, a, qb[ch + 1][0], qb[ch + 1][1]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] += d[e];
     };
-    if (!apart) {
-      values(pa0, pa1, pb0, pb1, vs);
-    } else {  // more than a factor 64 between the pages: one after the other
+    // Scaled scores of a page whose first token is tok0; tokens past the context are -inf.
+    auto finish = [&](float (&c)[4], float ks, int tok0) {
+      const float a0 = f0 * ks, a1 = f1 * ks;
+      const bool v0 = tok0 + g < ctx, v1 = tok0 + g + 8 < ctx;
+      c[0] = v0 ? c[0] * a0 : neg_inf();
+      c[1] = v0 ? c[1] * a1 : neg_inf();
+      c[2] = v1 ? c[2] * a0 : neg_inf();
+      c[3] = v1 ? c[3] * a1 : neg_inf();
+    };
+
+    for (const int end = i + seg; i < end; ++i) {
+      if ((i & 31) == 0 && i + 32 < n_my) {  // the next window, while this one is worked on
+        fill_rows((i >> 5) + 1);
+        fill_scales((i >> 5) + 1);
+      }
+      const int st = i % NSTAGE;
+      // Warp-uniform outcome: every lane polls (bounded), and the warp goes on together.
+      if (!dead && !__all_sync(0xffffffffu, mbar_wait(bar0 + st * 8, (i / NSTAGE) & 1))) {
+        if (lane == 0) report(FA_DEVERR_TIMEOUT);
+        for (int j = i + 1; j < n_my && j < i + NSTAGE; ++j)  // drain the loads in flight
+          mbar_wait(bar0 + (j % NSTAGE) * 8, (j / NSTAGE) & 1);
+        dead = true;
+      }
+      if (dead) continue;
+      const Kv8Window &w = win[(i >> 5) & 1];
+      const int e32 = i & 31;
+      const int tok0 = (pr.j + seg - (end - i)) * (2 * kPage);
+      const uint32_t kb = ring + st * S::kStageBytes, vb = kb + 2 * S::kPageBytes;
+      if (ctx - tok0 < 2 * kPage) {
+        // The context ends in this pair. What lies behind its last token (another owner's bytes, or
+        // a page that was not loaded) may be e4m3's NaN, which a probability of 0 would not mask:
+        // clear those rows of V, and order the stores before the ring's next load into them.
+        for (int x = (ctx - tok0) * (HD / 16) + lane; x < 2 * kPage * (HD / 16); x += 32)
+          *reinterpret_cast<uint4 *>(smem + (vb - smem_u32(smem)) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+
+      float ca[4], cb[4];
+      scores(kb, ca);
+      scores(kb + S::kPageBytes, cb);
+      finish(ca, w.ks[0][e32], tok0);
+      finish(cb, w.ks[1][e32], tok0 + kPage);
+      float bm0 = fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]));
+      float bm1 = fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]));
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, x));
+        bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, x));
+      }
+      if (__any_sync(0xffffffffu, bm0 > m0 || bm1 > m1)) {  // few steps raise a maximum late in a context
+        const float mn0 = fmaxf(m0, bm0), mn1 = fmaxf(m1, bm1);
+        const float r0 = ex2(m0 - mn0), r1 = ex2(m1 - mn1);
+        l0 *= r0;
+        l1 *= r1;
+        m0 = mn0;
+        m1 = mn1;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          o[c][0] *= r0;
+          o[c][1] *= r1;
+          o[c][2] *= r0;
+          o[c][3] *= r1;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ca[e] = ex2(ca[e] - (e & 1 ? m1 : m0));
+        cb[e] = ex2(cb[e] - (e & 1 ? m1 : m0));
+      }
+      l0 += (ca[0] + ca[2]) + (cb[0] + cb[2]);
+      l1 += (ca[1] + ca[3]) + (cb[1] + cb[3]);
+      const float vs0 = w.vs[0][e32], vs1 = w.vs[1][e32];
+      const float vs = fmaxf(vs0, vs1);
+      const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.2e-38f;
+      const float inv = vs > 0.f ? 1.f / vs : 0.f;  // both scales 0: nothing to add
+      const float ra = apart ? 1.f : vs0 * inv, rb = apart ? 0.f : vs1 * inv;
+      const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0] * ra, ca[1] * ra));
+      const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2] * ra, ca[3] * ra));
+      const uint32_t pb0 = movmatrix_t(pack2<__half>(cb[0] * rb, cb[1] * rb));
+      const uint32_t pb1 = movmatrix_t(pack2<__half>(cb[2] * rb, cb[3] * rb));
+      // o += (P_a V_a + P_b V_b) factor
+      auto values = [&](uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, float factor) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ch += 2) {
+          float ta[2][4];
+          uint32_t ra4[4], rb4[4], a[4];
+          ldsm_x4_t(vb + at(ch), ra4);
+          ldsm_x4_t(vb + S::kPageBytes + at(ch), rb4);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            unpack4_t<F>(ra4[2 * e], a[0], a[1]);
+            unpack4_t<F>(ra4[2 * e + 1], a[2], a[3]);
+            mma_f16_zero(ta[e], a, a0, a1);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            unpack4_t<F>(rb4[2 * e], a[0], a[1]);
+            unpack4_t<F>(rb4[2 * e + 1], a[2], a[3]);
+            mma16816<__half>(ta[e], a, b0, b1);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q], factor, o[ch + e][q]);
+        }
+      };
+      if (!apart) {
+        values(pa0, pa1, pb0, pb1, vs);
+      } else {  // more than a factor 64 between the pages: one after the other
 #pragma unroll 1
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t q0 = movmatrix_t(pack2<__half>(cb[0], cb[1])), q1 = movmatrix_t(pack2<__half>(cb[2], cb[3]));
-        values(x ? 0u : pa0, x ? 0u : pa1, x ? q0 : 0u, x ? q1 : 0u, x ? vs1 : vs0);
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t q0 = movmatrix_t(pack2<__half>(cb[0], cb[1]));
+          const uint32_t q1 = movmatrix_t(pack2<__half>(cb[2], cb[3]));
+          values(x ? 0u : pa0, x ? 0u : pa1, x ? q0 : 0u, x ? q1 : 0u, x ? vs1 : vs0);
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && i + NSTAGE < n_my) issue(i + NSTAGE);
+    }
+
+    // ---- the segment's end: the output, or a piece ---------------------------------------------
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    const float i0 = 1.f / l0, i1 = 1.f / l1;
+    if (seg == pr.of) {
+      T *out = static_cast<T *>(p.out) + (size_t(pr.s) * p.num_heads + hq0) * HD + 2 * g;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (2 * t < n_rep)
+          *reinterpret_cast<uint32_t *>(out + (2 * t) * HD + c * 16) = pack2<T>(o[c][0] * i0, o[c][2] * i0);
+        if (2 * t + 1 < n_rep)
+          *reinterpret_cast<uint32_t *>(out + (2 * t + 1) * HD + c * 16) = pack2<T>(o[c][1] * i1, o[c][3] * i1);
+      }
+    } else {
+      const int which = i == seg ? 0 : 1;  // the range's first segment, or its last
+      pieces[which] = pr.s * H + pr.kvh;
+      const size_t slot = size_t(blockIdx.x) * kKv8Pieces + warp * 2 + which;
+      float *po = p.pieces + slot * n_rep * HD + 2 * g;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (2 * t < n_rep)
+          *reinterpret_cast<float2 *>(po + (2 * t) * HD + c * 16) = make_float2(o[c][0] * i0, o[c][2] * i0);
+        if (2 * t + 1 < n_rep)
+          *reinterpret_cast<float2 *>(po + (2 * t + 1) * HD + c * 16) = make_float2(o[c][1] * i1, o[c][3] * i1);
+      }
+      if (g == 0) {
+        float *pl = p.piece_lse + slot * n_rep;
+        if (2 * t < n_rep) pl[2 * t] = m0 + __log2f(l0);
+        if (2 * t + 1 < n_rep) pl[2 * t + 1] = m1 + __log2f(l1);
       }
     }
-    __syncwarp();
-    if (lane == 0 && i + NSTAGE < n_my) issue(i + NSTAGE);
+    pr = next;
   }
-  if (timed_out_at >= 0) {
-    // Drain this warp's loads still in flight (each wait bounded again) before leaving.
-    if (lane == 0) report(FA_DEVERR_TIMEOUT);
-    for (int j = timed_out_at + 1; j < n_my && j < timed_out_at + NSTAGE; ++j)
-      mbar_wait(bar0 + (j % NSTAGE) * 8, (j / NSTAGE) & 1);
+  if (lane == 0) {
+    s_misc[2 * warp] = pieces[0];
+    s_misc[2 * warp + 1] = pieces[1];
   }
-#pragma unroll
-  for (int x = 4; x < 32; x <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-  }
-  __syncthreads();  // every warp is done with its ring: reuse it as reduction scratch
+  if (tid == 0) s_misc[16] = -1;  // the item last looked at
+  __syncthreads();  // the warps' pieces are written, and every ring is drained
 
-  // ---- combine the 4 warps ------------------------------------------------------------------
-  float *red_o = reinterpret_cast<float *>(smem);                           // [W][8][HD+4]
-  float *red_m = red_o + kDecodeWarps * 8 * S::kRedStride;                  // [W][8]
-  float *red_l = red_m + kDecodeWarps * 8;                                  // [W][8]
-  float *s_lse = red_l + kDecodeWarps * 8;                                  // [8][max_splits]
-  {
-    float *ro = red_o + warp * 8 * S::kRedStride;
+  // ---- join the pieces ------------------------------------------------------------------------
+  // The pieces of an item are those of the workers (warps) that its pairs fall to, the first
+  // segment of a worker's range in its slot 0, a later one in slot 1. An item inside this CTA is
+  // joined here; one that others have a part of by the last CTA to take its ticket. Where more than
+  // kKv8Direct CTAs share an item, each joins its own pieces first.
+  float *s_lse = reinterpret_cast<float *>(smem);  // [8][pieces] over the drained rings
+  const int cpp = kDecodeWarps * ppw;              // pairs per CTA
+  // Piece k of n at row(k) of the pieces -> dst (f32, with its lse), or the output.
+  auto join = [&](int item, int n, auto row, float *dst, float *dst_lse) {
+    for (int x = tid; x < n_rep * n; x += kDecodeThreads)
+      s_lse[x] = __ldcg(&p.piece_lse[row(x / n_rep) * n_rep + x % n_rep]);
+    __syncthreads();
+    for (int x = tid; x < n_rep * (HD / 4); x += kDecodeThreads) {
+      const int h = x / (HD / 4), d = x % (HD / 4) * 4;
+      float M = neg_inf();
+      for (int k = 0; k < n; ++k) M = fmaxf(M, s_lse[k * n_rep + h]);
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      float W = 0.f;
+      for (int k0 = 0; k0 < n; k0 += 8) {  // eight loads in flight
+        float4 v[8];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      *reinterpret_cast<float2 *>(ro + (2 * t) * S::kRedStride + c * 16 + 2 * g) =
-          make_float2(o[c][0], o[c][2]);
-      *reinterpret_cast<float2 *>(ro + (2 * t + 1) * S::kRedStride + c * 16 + 2 * g) =
-          make_float2(o[c][1], o[c][3]);
+        for (int u = 0; u < 8; ++u)
+          if (k0 + u < n)
+            v[u] = __ldcg(reinterpret_cast<const float4 *>(p.pieces + (row(k0 + u) * n_rep + h) * HD + d));
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k0 + u < n) {
+            const float e = ex2(s_lse[(k0 + u) * n_rep + h] - M);
+            O.x += e * v[u].x;
+            O.y += e * v[u].y;
+            O.z += e * v[u].z;
+            O.w += e * v[u].w;
+            W += e;
+          }
+      }
+      const float i = 1.f / W;
+      if (dst) {
+        *reinterpret_cast<float4 *>(dst + h * HD + d) = make_float4(O.x * i, O.y * i, O.z * i, O.w * i);
+        if (d == 0) dst_lse[h] = M + __log2f(W);
+      } else {
+        T *out = static_cast<T *>(p.out) + (size_t(item / H) * p.num_heads + (item % H) * n_rep + h) * HD + d;
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
+      }
     }
-    if (g == 0) {
-      red_m[warp * 8 + 2 * t] = m0;
-      red_m[warp * 8 + 2 * t + 1] = m1;
-      red_l[warp * 8 + 2 * t] = l0;
-      red_l[warp * 8 + 2 * t + 1] = l1;
+    __syncthreads();  // s_lse is free again
+  };
+  struct Span {
+    int a0, a1;  // the item's pairs
+  };
+  auto span = [&](int item) {
+    const int s = item / H, np = offs[s + 1] - offs[s], a0 = offs[s] * H + (item % H) * np;
+    return Span{a0, a0 + np};
+  };
+  // Workers first .. first + n - 1 of item; the row of a worker's piece.
+  auto pieces_of = [&](const Span &sp, int from, int to, int &first) {
+    first = max(sp.a0, from) / ppw;
+    return (min(sp.a1, to) - 1) / ppw - first + 1;
+  };
+  auto row_of = [&](const Span &sp, int worker) {
+    return size_t(worker / kDecodeWarps) * kKv8Pieces + worker % kDecodeWarps * 2 +
+           (worker * ppw < sp.a0 ? 1 : 0);
+  };
+  auto own_row = [&](const Span &sp, int c) {
+    return size_t(c) * kKv8Pieces + 2 * kDecodeWarps + (sp.a0 < c * cpp ? 0 : 1);
+  };
+  // The (at most two) items that other CTAs share: the first with a piece here, and the last.
+  int shared[2] = {-1, -1};
+  for (int k = 0; k < 2 * kDecodeWarps; ++k) {
+    const int item = s_misc[k];
+    if (item < 0 || item == s_misc[16]) continue;
+    // a new item (its pieces follow one another)
+    __syncthreads();
+    if (tid == 0) s_misc[16] = item;
+    __syncthreads();
+    const Span sp = span(item);
+    int first;
+    const int n = pieces_of(sp, c0, c1, first);
+    if (sp.a0 >= c0 && sp.a1 <= c1) {
+      join(item, n, [&](int q) { return row_of(sp, first + q); }, nullptr, nullptr);
+      continue;
     }
+    if ((sp.a1 - 1) / cpp - sp.a0 / cpp >= kKv8Direct) {
+      const size_t own = own_row(sp, blockIdx.x);
+      join(item, n, [&](int q) { return row_of(sp, first + q); }, p.pieces + own * n_rep * HD,
+           p.piece_lse + own * n_rep);
+    }
+    shared[sp.a0 < c0 ? 0 : 1] = item;
+  }
+  if (shared[0] < 0 && shared[1] < 0) return;
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    const int item = shared[tid];
+    int last = 0;
+    if (item >= 0) {
+      const Span sp = span(item);
+      last = atomicAdd(&p.tickets[item], 1) == (sp.a1 - 1) / cpp - sp.a0 / cpp;
+    }
+    s_misc[16 + tid] = last;
   }
   __syncthreads();
-
-  const int hq0 = kvh * n_rep;
-  const bool single = n_splits == 1;
-  for (int idx = tid; idx < n_rep * HD; idx += kDecodeThreads) {
-    const int h = idx / HD, x = idx % HD;
-    float M = neg_inf();
-#pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, red_m[w * 8 + h]);
-    float O = 0.f, Lsum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) {
-      const float e = ex2(red_m[w * 8 + h] - M);  // warps without pages: m = -inf -> 0
-      O += e * red_o[(w * 8 + h) * S::kRedStride + x];
-      Lsum += e * red_l[w * 8 + h];
-    }
-    const size_t ob = size_t(b) * p.num_heads + hq0 + h;
-    if (single) {
-      store_out<T>(p, b, hq0 + h, HD, x, O / Lsum);
+  if (!s_misc[16] && !s_misc[17]) return;
+  __threadfence();
+#pragma unroll 1
+  for (int x = 0; x < 2; ++x) {
+    if (!s_misc[16 + x]) continue;
+    const int item = shared[x];
+    const Span sp = span(item);
+    const int ctas = (sp.a1 - 1) / cpp - sp.a0 / cpp + 1;
+    int first;
+    if (ctas > kKv8Direct) {
+      join(item, ctas, [&](int q) { return own_row(sp, sp.a0 / cpp + q); }, nullptr, nullptr);
     } else {
-      const size_t pi = ob * p.max_splits + split;
-      p.part_o[pi * HD + x] = O / Lsum;
-      if (x == 0) p.part_lse[pi] = M + __log2f(Lsum);
+      const int n = pieces_of(sp, 0, total, first);
+      join(item, n, [&](int q) { return row_of(sp, first + q); }, nullptr, nullptr);
     }
+    if (tid == 0) p.tickets[item] = 0;  // ready for the next launch
   }
-  if (single) return;
-
-  // ---- last split of this (sequence, kv_head) merges the partials ------------------------
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    const int prev = atomicAdd(&p.counters[b * p.num_kv_heads + kvh], 1);
-    s_flag[0] = (prev == n_splits - 1);
-  }
-  __syncthreads();
-  if (!s_flag[0]) return;
-  __threadfence();
-  for (int idx = tid; idx < n_rep * n_splits; idx += kDecodeThreads) {
-    const int h = idx / n_splits, sp = idx % n_splits;
-    s_lse[h * kDecodeMaxSplits + sp] =
-        __ldcg(&p.part_lse[(size_t(b) * p.num_heads + hq0 + h) * p.max_splits + sp]);
-  }
-  __syncthreads();
-  for (int idx = tid; idx < n_rep * HD; idx += kDecodeThreads) {
-    const int h = idx / HD, x = idx % HD;
-    const float *lse = s_lse + h * kDecodeMaxSplits;
-    float M = neg_inf();
-    for (int sp = 0; sp < n_splits; ++sp) M = fmaxf(M, lse[sp]);
-    const size_t ob = size_t(b) * p.num_heads + hq0 + h;
-    const float *po = p.part_o + ob * p.max_splits * HD + x;
-    float O = 0.f, W = 0.f;
-    for (int sp = 0; sp < n_splits; ++sp) {
-      const float w = ex2(lse[sp] - M);
-      O += w * __ldcg(po + size_t(sp) * HD);
-      W += w;
-    }
-    store_out<T>(p, b, hq0 + h, HD, x, O / W);
-  }
-  if (tid == 0) p.counters[b * p.num_kv_heads + kvh] = 0;  // ready for the next launch
 }
 
 }  // namespace fa
