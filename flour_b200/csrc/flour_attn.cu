@@ -388,11 +388,11 @@ int sm_count() {
   return cached[dev];
 }
 
-template <typename T, bool kRef>
+template <typename T, bool kRef, bool kSplit = false>
 fa_status launch_prefill_t(const fa::PrefillParams &p, const CUtensorMap &tq, const CUtensorMap &tk,
                            const CUtensorMap &tv, int grid_x, cudaStream_t stream) {
   using S = fa::PrefillSmem;
-  auto kern = fa::paged_prefill_kernel<T, kRef>;
+  auto kern = fa::paged_prefill_kernel<T, kRef, kSplit>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAllocMax);
   if (e != cudaSuccess) return fail(FA_ECUDA, "prefill: set smem attribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
@@ -410,10 +410,18 @@ fa_status launch_prefill_t(const fa::PrefillParams &p, const CUtensorMap &tq, co
   return check_launch("paged_prefill");
 }
 
+// The split form of a prefill: parts of part_tiles KV tiles, their rows in `part` (f32 outputs and,
+// behind parts * total_q * num_heads * 128 of them, the log2-sum-exps).
+struct PrefillSplit {
+  int parts, part_tiles;
+  float *part;
+};
+
 fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const int32_t *cu,
                          const int32_t *ctx, const int32_t *tables, int max_blocks, int num_seqs,
                          int num_heads, int n_rep, int total_q, float scale, int score_flow,
-                         void *ws, size_t ws_bytes, cudaStream_t stream, int q_rows = 0) {
+                         void *ws, size_t ws_bytes, cudaStream_t stream, int q_rows = 0,
+                         const PrefillSplit *split = nullptr) {
   if (!ws) return fail(FA_EINVAL, "prefill: workspace is NULL but %zu bytes are needed", kPrefillWorkspace);
   if (ws_bytes < kPrefillWorkspace)
     return fail(FA_ERANGE, "prefill: workspace of %zu bytes, %zu needed", ws_bytes, kPrefillWorkspace);
@@ -448,7 +456,16 @@ fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const i
     p.cu_seqlens_q = cu + s0;
     p.context_lens = ctx + s0;
     p.block_tables = tables + size_t(s0) * max_blocks;
-    const int64_t items = ((int64_t(total_q) + chunk - 1) / chunk + p.num_seqs) * L->num_kv_heads;
+    int64_t items = ((int64_t(total_q) + chunk - 1) / chunk + p.num_seqs) * L->num_kv_heads;
+    if (split) {  // one launch: callers split no batch of more than kPfMaxSeqs sequences
+      p.part_tiles = split->part_tiles;
+      p.part_o = split->part;
+      p.part_lse = split->part + size_t(split->parts) * total_q * num_heads * 128;
+      items *= split->parts;
+      const int g = int(std::min<int64_t>(sm_count(), items));
+      return L->dtype == FA_BF16 ? launch_prefill_t<__nv_bfloat16, false, true>(p, tmq, tk, tv, g, stream)
+                                 : launch_prefill_t<__half, false, true>(p, tmq, tk, tv, g, stream);
+    }
     const int grid = int(std::max<int64_t>(1, std::min<int64_t>(sm_count(), items)));
     fa_status st =
         L->dtype == FA_BF16
@@ -1024,14 +1041,40 @@ bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float s
          aligned(L->k_cache, 8) && aligned(L->v_cache, 8) && aligned(q, 16) && aligned(out, 32);
 }
 
+// How many parts to cut the contexts of a batch into: as long as the chunks (upper bound: the host
+// knows total_q, not the lengths) do not fill the SMs a few times. In KV tiles of one item (about
+// 2.1 us): a wave of items lasts its longest part plus 1.2 for the item's start and end, and the
+// join moves every part's rows twice (one tile per 14 MB). Measured on one sequence of 509 tokens
+// over 30001 (28 query heads, 4 KV heads, 60 items): 512 us unsplit; see prefill_split's callers.
+PrefillSplit plan_prefill_split(int num_seqs, int num_heads, int num_kv_heads, int total_q, int max_context_len) {
+  const int chunk = 2 * (128 / (num_heads / num_kv_heads)), sms = sm_count();
+  const int64_t items =
+      std::min<int64_t>((int64_t(total_q) + chunk - 1) / chunk + num_seqs - 1, total_q) * num_kv_heads;
+  const int tiles = (max_context_len + fa::kPfBN - 1) / fa::kPfBN;
+  PrefillSplit best{1, std::max(1, tiles), nullptr};
+  double least = 1e30;
+  for (int parts = 1; parts <= std::min(32, tiles); ++parts) {
+    const int pt = (tiles + parts - 1) / parts;
+    const int64_t waves = (items * parts + sms - 1) / sms;
+    const double join = parts == 1 ? 0.0 : 1.5 + double(parts) * total_q * num_heads * 129 * 8 / 14e6;
+    const double cost = double(waves) * (pt + 1.2) + join;
+    if (cost < least) {
+      least = cost;
+      best.parts = (tiles + pt - 1) / pt;
+      best.part_tiles = pt;
+    }
+  }
+  return best;
+}
+
 struct Prefill8Workspace {
-  size_t q_off, ctx_off, tables_off, k_off, v_off, bytes;
+  size_t q_off, ctx_off, tables_off, k_off, v_off, part_off, bytes;
 };
 
 // Work counters of the prefill kernel, a padded copy of a query batch shorter than one box, the
-// copy's context lengths and block tables, the copied pages.
+// copy's context lengths and block tables, the copied pages, the parts of a split.
 Prefill8Workspace prefill8_workspace_layout(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
-                                            int max_context_len, int32_t total_blocks) {
+                                            int total_q, int max_context_len, int32_t total_blocks) {
   auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
   Prefill8Workspace w{};
   const int width = std::max(1, (max_context_len + fa::kPage - 1) / fa::kPage);
@@ -1041,7 +1084,11 @@ Prefill8Workspace prefill8_workspace_layout(int num_seqs, int num_heads, int num
   w.k_off = w.tables_off + r256(size_t(num_seqs) * width * 4);
   const size_t slab = r256(size_t(std::max(1, total_blocks)) * num_kv_heads * fa::kPage * head_dim * 2);
   w.v_off = w.k_off + slab;
-  w.bytes = w.v_off + slab;
+  w.part_off = w.v_off + slab;
+  const int parts = num_heads / num_kv_heads > 128
+                        ? 1
+                        : plan_prefill_split(num_seqs, num_heads, num_kv_heads, total_q, max_context_len).parts;
+  w.bytes = w.part_off + (parts > 1 ? size_t(parts) * total_q * num_heads * 129 * 4 : 0);
   return w;
 }
 
@@ -1051,7 +1098,7 @@ fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32
                           float scale, void *ws, size_t ws_bytes, cudaStream_t stream) {
   const char *who = "paged_prefill_kv8";
   const Prefill8Workspace w = prefill8_workspace_layout(num_seqs, num_heads, L->num_kv_heads, L->head_dim,
-                                                        max_context_len, total_blocks);
+                                                        total_q, max_context_len, total_blocks);
   if (!ws) return fail(FA_EINVAL, "%s: workspace is NULL but %zu bytes are needed", who, w.bytes);
   if (ws_bytes < w.bytes)
     return fail(FA_ERANGE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, w.bytes);
@@ -1096,9 +1143,29 @@ fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32
   if (st != FA_OK) return st;
   const fa_kv_layer copy{wsb + w.k_off, wsb + w.v_off, total_blocks, L->num_kv_heads, L->block_size,
                          L->head_dim, dtype};
-  return launch_prefill(&copy, pad ? e.q_out : q, out, cu, e.out_ctx, e.out_tables, e.out_width, num_seqs,
-                        num_heads, n_rep, total_q, scale, FA_SCORES_F32, ws, kPrefillWorkspace, stream,
-                        pad ? box : 0);
+  PrefillSplit split = plan_prefill_split(num_seqs, num_heads, L->num_kv_heads, total_q, max_context_len);
+  split.part = reinterpret_cast<float *>(wsb + w.part_off);
+  st = launch_prefill(&copy, pad ? e.q_out : q, out, cu, e.out_ctx, e.out_tables, e.out_width, num_seqs,
+                      num_heads, n_rep, total_q, scale, FA_SCORES_F32, ws, kPrefillWorkspace, stream,
+                      pad ? box : 0, split.parts > 1 ? &split : nullptr);
+  if (st != FA_OK || split.parts == 1) return st;
+  fa::PrefillParams j{};
+  j.out = out;
+  j.cu_seqlens_q = cu;
+  j.context_lens = e.out_ctx;
+  j.max_blocks_per_seq = e.out_width;
+  j.num_seqs = num_seqs;
+  j.num_heads = num_heads;
+  j.total_q = total_q;
+  j.tq = box;
+  j.part_tiles = split.part_tiles;
+  j.part_o = split.part;
+  j.part_lse = split.part + size_t(split.parts) * total_q * num_heads * 128;
+  const int64_t warps = int64_t(total_q) * num_heads;
+  const dim3 jgrid(unsigned((warps + 7) / 8));
+  return dtype == FA_BF16
+             ? launch_pdl(who, fa::prefill_join_kernel<__nv_bfloat16>, jgrid, 256, 0, stream, 1, j)
+             : launch_pdl(who, fa::prefill_join_kernel<__half>, jgrid, 256, 0, stream, 1, j);
 }
 
 }  // namespace
@@ -1683,12 +1750,12 @@ fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void
 }
 
 size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                           int32_t head_dim, int32_t max_context_len, int32_t max_seqlen_q,
-                                           int32_t total_blocks) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context_len <= 0 ||
-      total_blocks < 0)
+                                           int32_t head_dim, int32_t total_q, int32_t max_context_len,
+                                           int32_t max_seqlen_q, int32_t total_blocks) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || total_q <= 0 ||
+      max_context_len <= 0 || total_blocks < 0 || num_heads % num_kv_heads != 0)
     return 0;
-  const size_t copy = prefill8_workspace_layout(num_seqs, num_heads, num_kv_heads, head_dim,
+  const size_t copy = prefill8_workspace_layout(num_seqs, num_heads, num_kv_heads, head_dim, total_q,
                                                 max_context_len, total_blocks)
                           .bytes;
   if (max_seqlen_q != 1) return copy;

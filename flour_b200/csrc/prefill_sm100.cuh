@@ -35,6 +35,10 @@
 // only when the max grows by more than 8 (so un-rescaled P stays below 2^8); the final output is
 // O / rowsum, cast to the query dtype (cpu.rs:111).
 //
+// Split form (kSplit, for batches with fewer chunks than SMs over long contexts): an item is also one
+// of the parts of `part_tiles` KV tiles that its chunk's context is cut into. Each part leaves its
+// rows' O / l (f32) and log2-sum-exp, and prefill_join_kernel, the next launch, joins them.
+//
 // Every mbarrier wait is bounded; a timeout sets FA_DEVERR_TIMEOUT, the roles stop, issued MMAs
 // are drained and TMEM is released before the CTA exits.
 #pragma once
@@ -59,6 +63,9 @@ struct PrefillParams {
   int32_t tq;                    // query tokens per Q tile (128 / n_rep)
   float scale_log2;              // scale * log2(e), > 0
   float scale;                   // scale as passed (the reference flow rounds it to the dtype)
+  int32_t part_tiles;            // split form: KV tiles per part
+  float *part_o;                 // split form: [parts][total_q][num_heads][128]
+  float *part_lse;               // split form: [parts][total_q][num_heads]
 };
 
 constexpr int kPfSoftmaxWarps = 16;         // 2 Q tiles x 2 column halves x 4 row quadrants
@@ -75,7 +82,8 @@ constexpr int kPfMaxSeqs = 2048;            // sequences per launch (chunk table
 struct PfItem {
   int32_t kind;  // 0 work, 1 invalid sequence data (rows are zeroed), 2 no more work
   int32_t seq, kvh, t0, q0, S_len, Pfx, n_tiles, n_pages;
-  int32_t pad[7];
+  int32_t tile0, part;  // split form: the part's first KV tile, its number (0 otherwise)
+  int32_t pad[5];
 };
 
 struct PrefillSmem {
@@ -117,8 +125,13 @@ __device__ __forceinline__ bool pair_all(int id, bool v) {
   return r != 0;
 }
 
+// Parts that a context of L tokens is cut into (at least one).
+__device__ __forceinline__ int prefill_parts(int L, int part_tiles) {
+  return max(1, ((max(L, 0) + kPfBN - 1) / kPfBN + part_tiles - 1) / part_tiles);
+}
+
 // kRef: the reference's dtype rounding of the scores (ref_score, FA_SCORES_REFERENCE).
-template <typename T, bool kRef>
+template <typename T, bool kRef, bool kSplit = false>
 __global__ void __launch_bounds__(kPfThreads, 1)
     paged_prefill_kernel(const __grid_constant__ PrefillParams p,
                          const __grid_constant__ CUtensorMap tm_q,
@@ -164,6 +177,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   for (int s = tid; s < p.num_seqs; s += kPfThreads) {
     const int len = p.cu_seqlens_q[s + 1] - p.cu_seqlens_q[s];
     offs[s + 1] = len > 0 ? (len + chunk - 1) / chunk : 0;
+    if constexpr (kSplit) offs[s + 1] *= prefill_parts(p.context_lens[s], p.part_tiles);
   }
   __syncthreads();
   if (warp == 0) {
@@ -198,34 +212,49 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       // Next work item: global ticket + the sequence's metadata. Called one item ahead, where the
       // producer would otherwise wait for a free ring stage, so its latency stays hidden.
       auto fetch = [&](PfItem &it) {
-        it = PfItem{};
-        const int w = *s_abort ? n_items : atomicAdd(p.counters, 1);
-        if (w >= n_items) {
-          it.kind = 2;
+        for (;;) {
+          it = PfItem{};
+          const int w = *s_abort ? n_items : atomicAdd(p.counters, 1);
+          if (w >= n_items) {
+            it.kind = 2;
+            return;
+          }
+          const int c = w / p.num_kv_heads;
+          it.kvh = w % p.num_kv_heads;
+          int lo = 0, hi = p.num_seqs;  // last s with offs[s] <= c
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (offs[mid] <= c) lo = mid; else hi = mid;
+          }
+          it.seq = lo;
+          it.q0 = p.cu_seqlens_q[lo];
+          it.S_len = p.cu_seqlens_q[lo + 1] - it.q0;
+          const int L = p.context_lens[lo];
+          if constexpr (kSplit) {
+            const int parts = prefill_parts(L, p.part_tiles);
+            const int from_end = (c - offs[lo]) / parts;
+            it.part = (c - offs[lo]) % parts;
+            it.t0 = ((it.S_len + chunk - 1) / chunk - 1 - from_end) * chunk;
+          } else {
+            it.t0 = (offs[lo + 1] - 1 - c) * chunk;  // last chunk (most KV) of a sequence first
+          }
+          it.Pfx = L - it.S_len;
+          if (L < it.S_len || int64_t(L) > int64_t(p.max_blocks_per_seq) * kPage || it.q0 < 0 ||
+              it.q0 + it.S_len > p.total_q) {
+            it.kind = 1;
+            report(it.q0 < 0 || it.q0 + it.S_len > p.total_q ? FA_DEVERR_SEQLEN : FA_DEVERR_CONTEXT);
+          } else {
+            it.kind = 0;
+            const int kv_end = it.Pfx + min(it.t0 + chunk, it.S_len);
+            it.n_tiles = (kv_end + kPfBN - 1) / kPfBN;
+            it.n_pages = (L + kPage - 1) / kPage;
+            if constexpr (kSplit) {
+              it.tile0 = it.part * p.part_tiles;
+              it.n_tiles = min(it.n_tiles - it.tile0, p.part_tiles);
+              if (it.n_tiles <= 0) continue;  // past this chunk's last visible key
+            }
+          }
           return;
-        }
-        const int c = w / p.num_kv_heads;
-        it.kvh = w % p.num_kv_heads;
-        int lo = 0, hi = p.num_seqs;  // last s with offs[s] <= c
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (offs[mid] <= c) lo = mid; else hi = mid;
-        }
-        it.seq = lo;
-        it.t0 = (offs[lo + 1] - 1 - c) * chunk;  // last chunk (most KV) of a sequence first
-        it.q0 = p.cu_seqlens_q[lo];
-        it.S_len = p.cu_seqlens_q[lo + 1] - it.q0;
-        const int L = p.context_lens[lo];
-        it.Pfx = L - it.S_len;
-        if (L < it.S_len || int64_t(L) > int64_t(p.max_blocks_per_seq) * kPage || it.q0 < 0 ||
-            it.q0 + it.S_len > p.total_q) {
-          it.kind = 1;
-          report(it.q0 < 0 || it.q0 + it.S_len > p.total_q ? FA_DEVERR_SEQLEN : FA_DEVERR_CONTEXT);
-        } else {
-          it.kind = 0;
-          const int kv_end = it.Pfx + min(it.t0 + chunk, it.S_len);
-          it.n_tiles = (kv_end + kPfBN - 1) / kPfBN;
-          it.n_pages = (L + kPage - 1) / kPage;
         }
       };
       PfItem next;
@@ -244,7 +273,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int32_t *table = p.block_tables + size_t(it.seq) * p.max_blocks_per_seq;
         int ids[kPfPages];  // block ids of the tile being issued (loaded one tile ahead)
 #pragma unroll
-        for (int j = 0; j < kPfPages; ++j) ids[j] = table[min(j, it.n_pages - 1)];
+        for (int j = 0; j < kPfPages; ++j)
+          ids[j] = table[min((kSplit ? it.tile0 * kPfPages : 0) + j, it.n_pages - 1)];
         // Q tiles of this item (each waits for the previous item's last S MMA reading it).
         const int qbytes = 2 * 64 * p.n_rep * p.tq * 2;
         bool ok = true;
@@ -275,7 +305,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             }
             rows[j] = (id * p.num_kv_heads + it.kvh) * kPage;
             // next tile's ids: in flight while this tile waits for its ring stage
-            nids[j] = table[min((i + 1) * kPfPages + j, it.n_pages - 1)];
+            nids[j] = table[min(((kSplit ? it.tile0 : 0) + i + 1) * kPfPages + j, it.n_pages - 1)];
           }
           if (g >= kPfStages && !mbar_wait(bar(S::KEMPTY + st), ph)) { ok = false; break; }
           mbar_arrive_expect_tx(bar(S::KFULL + st), S::kTile);
@@ -473,7 +503,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         tc::ld32(s_addr + 32, sr[1]);
         tc::wait_ld();
         // Row max on the raw scores (scale > 0); keys past the causal limit become -inf.
-        const int j0 = i * kPfBN + hh * 64;
+        const int j0 = ((kSplit ? it.tile0 : 0) + i) * kPfBN + hh * 64;
         float mxp[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) mxp[q] = neg_inf();
@@ -563,7 +593,18 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         uint32_t o[32];
         tc::ld32(o_addr + c * 32, o);
         tc::wait_ld();
-        if (row_valid) {
+        if constexpr (kSplit) {
+          if (row_valid) {
+            const size_t row = (size_t(it.part) * p.total_q + it.q0 + tok) * p.num_heads +
+                               it.kvh * p.n_rep + r % p.n_rep;
+            float *po = p.part_o + row * 128 + hh * 64 + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) st_global_v8(po + e, o + e);
+            if (hh == 0 && c == 0) p.part_lse[row] = lt > 0.f ? m_run + __log2f(lt) : neg_inf();
+          }
+        } else if (row_valid) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -599,6 +640,49 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       atomicExch(&p.counters[1], 0);
     }
   }
+}
+
+// Joins the parts of the split form: one warp per (query token, head), four values of head_dim a
+// lane. The parts that exist are those that the prefill's items covered: up to the last tile that
+// the row's chunk sees. Rows of refused sequences were zeroed there and stay.
+template <typename T>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const PrefillParams p) {
+  if (threadIdx.x == 0) pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t rh = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (rh >= int64_t(p.total_q) * p.num_heads) return;
+  const int row = int(rh / p.num_heads);
+  if (row >= p.cu_seqlens_q[p.num_seqs]) return;
+  int lo = 0, hi = p.num_seqs;  // last s with cu[s] <= row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid;
+  }
+  const int q0 = p.cu_seqlens_q[lo], S_len = p.cu_seqlens_q[lo + 1] - q0, L = p.context_lens[lo];
+  if (q0 < 0 || row < q0 || row >= q0 + S_len || q0 + S_len > p.total_q || L < S_len ||
+      int64_t(L) > int64_t(p.max_blocks_per_seq) * kPage)
+    return;
+  const int chunk = 2 * p.tq, kv_end = L - S_len + min(((row - q0) / chunk + 1) * chunk, S_len);
+  const int parts = ((kv_end + kPfBN - 1) / kPfBN + p.part_tiles - 1) / p.part_tiles;
+  const size_t stride = size_t(p.total_q) * p.num_heads;
+  float M = neg_inf();
+  for (int k = 0; k < parts; ++k) M = fmaxf(M, p.part_lse[k * stride + rh]);
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  float W = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) {
+    const float e = ex2(p.part_lse[k * stride + rh] - M);  // a part that the row does not see: 0
+    const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (k * stride + rh) * 128 + lane * 4);
+    O.x += e * v.x;
+    O.y += e * v.y;
+    O.z += e * v.z;
+    O.w += e * v.w;
+    W += e;
+  }
+  const float i = 1.f / W;  // part 0 holds position 0, which every row sees
+  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + rh * 128 + lane * 4) =
+      make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
 }
 
 }  // namespace fa

@@ -520,7 +520,7 @@ def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, c
     bt, cl = _tables(block_tables, context_lens, S)
     cu = _cu(cu_seqlens_q, S)
     dev = _device(k_cache.device, query, out, bt, cl, cu)
-    need = int(lib().fa_paged_prefill_kv8_workspace_size(S, hq, k_cache.shape[1], d, max_context_len,
+    need = int(lib().fa_paged_prefill_kv8_workspace_size(S, hq, k_cache.shape[1], d, tq, max_context_len,
                                                          max_seqlen_q, total_blocks))
     wp, wn = _ws8(workspace, need, dev)
     _call_on(dev, stream, "paged_prefill_kv8", lib().fa_paged_prefill_kv8, ctypes.byref(layer),

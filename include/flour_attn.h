@@ -360,15 +360,17 @@ FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *quer
  * and total_blocks, a host-side upper bound of the sum over the sequences of
  * ceil(context_len / block_size): the tensor-core path (FA_BF16 / FA_F16, block_size 16,
  * head_dim 128, at most 2048 sequences, scale > 0, 16-byte aligned query, 32-byte aligned out)
- * turns those blocks into the query type in the workspace first, in one launch. Sequences that no
+ * turns those blocks into the query type in the workspace first, in one launch; where the batch
+ * has too few query rows for the SMs, contexts are cut into parts whose results (f32, in the
+ * workspace) one more launch joins. Sequences that no
  * longer fit total_blocks give zeros and FA_DEVERR_CONTEXT. Other shapes, and total_blocks 0, run
  * the generic kernel, which needs no workspace. One new token per sequence (max_seqlen_q 1,
  * total_q == num_seqs) is fa_paged_decode_kv8. Output rows behind cu_seqlens_q[num_seqs] are not
  * written by the tensor-core path. */
 FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads,
                                                   int32_t num_kv_heads, int32_t head_dim,
-                                                  int32_t max_context_len, int32_t max_seqlen_q,
-                                                  int32_t total_blocks);
+                                                  int32_t total_q, int32_t max_context_len,
+                                                  int32_t max_seqlen_q, int32_t total_blocks);
 FA_API fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, void *out,
                                       int32_t dtype, const int32_t *cu_seqlens_q,
                                       const int32_t *context_lens, const int32_t *block_tables,

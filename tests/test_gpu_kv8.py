@@ -306,6 +306,36 @@ def test_prefill(device, fmt, dtype, Hq, Hkv, d, ctx, new):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq, Hkv, ctx, new", [
+    (8, 2, [3000], [40]),                    # one chunk over many parts
+    (7, 1, [1500], [1400]),                  # chunks that end in early parts
+    (8, 1, [2500, 129, 700, 1], [3, 129, 70, 1]),  # short sequences beside a long one
+    (16, 1, [5000], [9]),                    # n_rep 16: fewer rows than one query tile
+])
+def test_prefill_split_over_the_context(device, dtype, Hq, Hkv, ctx, new):
+    bt, nb = make_tables(ctx, 16, 44)
+    g = gen_of(device, 44)
+    pool = random_pool(nb, Hkv, 16, 128, torch.float8_e4m3fn, g, device)
+    poison_tails(pool, bt, ctx)
+    q = torch.randn((sum(new) + 5, Hq, 128), device=device, generator=g).to(dtype)
+    out = torch.full_like(q, 7.0)
+    ws = ops.Workspace()
+    for _ in range(2):
+        run_prefill(pool, q, bt, ctx, new, Hkv, device, ws=ws, out=out)
+        want, tol = attention_ref(q[:sum(new)].double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new,
+                                  Hq // Hkv, inv_sqrt(128), 2.0 ** -8 if dtype == torch.bfloat16 else U16)
+        assert_close(out[:sum(new)], want, tol)
+        assert (out[sum(new):] == 7.0).all()
+    assert ops.device_status() == 0
+    # A refused sequence (its blocks do not fit) is zeroed, the others stand.
+    if len(ctx) > 1:
+        run_prefill(pool, q, bt, ctx, new, Hkv, device, ws=ws, out=out, slack=-1)
+        assert ops.device_status() == _lib.FA_DEVERR_CONTEXT
+        assert not out[sum(new) - 1].any()
+        assert_close(out[:sum(new) - 1], want[:-1], tol[:-1])
+
+
 def test_prefill_equals_the_16_bit_prefill_of_the_same_values(device):
     # Power-of-two scales make the bf16 copy exact, so both prefills see one cache.
     ctx, new = [400, 129, 1000], [400, 60, 513]

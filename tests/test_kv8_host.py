@@ -77,12 +77,12 @@ def test_attention_refusals():
     assert prefill(layer8(), mq=65) == _lib.FA_ERANGE
     assert prefill(layer8(), T=0) == _lib.FA_OK
     fast = layer8(d=128)
-    need = lib().fa_paged_prefill_kv8_workspace_size(1, 4, 2, 128, 64, 8, 4)
+    need = lib().fa_paged_prefill_kv8_workspace_size(1, 4, 2, 128, 8, 64, 8, 4)
     assert need >= 2 * 4 * 2 * 16 * 128 * 2
     assert prefill(fast, ws=None) == _lib.FA_EINVAL
     assert prefill(fast, ws=P(0x100000), n=need - 1) == _lib.FA_ERANGE
     # One token each may take the decode: its workspace is covered too.
-    assert lib().fa_paged_prefill_kv8_workspace_size(64, 32, 8, 128, 4096, 1, 0) >= \
+    assert lib().fa_paged_prefill_kv8_workspace_size(64, 32, 8, 128, 64, 4096, 1, 0) >= \
         lib().fa_paged_decode_kv8_workspace_size(64, 32, 8, 128, 4096)
 
 
