@@ -380,28 +380,31 @@ def o_proj_residual(attn, weight, residual=None, out=None, stream=None) -> torch
 _KV8 = {torch.float8_e4m3fn: _lib.FA_KV8_E4M3, torch.int8: _lib.FA_KV8_I8}
 
 
-def _device(device: torch.device, *tensors: torch.Tensor | None) -> torch.device:
-    """The one CUDA device that all tensors live on; the call is made with it current."""
-    if device.type != "cuda":
-        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"tensors must be on a CUDA device, not {device}")
+def _device(*tensors: torch.Tensor | None) -> int:
+    """Index of the one CUDA device that all tensors live on; the call is made with it current."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise _lib.FlourAttnError(_lib.FA_EINVAL, f"tensors on {device} and {t.device} in one call")
-    return device
+        if t is not None and t.get_device() != dev:
+            raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                      f"tensors on {tensors[0].device} and {t.device} in one call")
+    if dev < 0 or not tensors[0].is_cuda:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                  f"tensors must be on a CUDA device, not {tensors[0].device}")
+    return dev
 
 
-def _call_on(device: torch.device, stream, what: str, fn, *args) -> None:
+def _call_on(dev: int, stream, what: str, fn, *args) -> None:
     """fn(*args, stream) on `stream`, or on the device's current stream, with it current."""
     if stream is None:
-        raw = torch._C._cuda_getCurrentRawStream(device.index)  # current_stream().cuda_stream, 2 us less
-    elif stream.device != device:
-        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"{what}: stream of {stream.device}, tensors on {device}")
+        raw = torch._C._cuda_getCurrentRawStream(dev)  # current_stream().cuda_stream, 2 us less
+    elif stream.device.index != dev:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"{what}: stream of {stream.device}, tensors on cuda:{dev}")
     else:
         raw = stream.cuda_stream
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == dev:
         st = fn(*args, raw)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(dev):
             st = fn(*args, raw)
     if st != _lib.FA_OK:
         check(st, what)
@@ -411,20 +414,22 @@ def kv8_layer_desc(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.
                    v_scale: torch.Tensor) -> _lib.FaKv8Layer:
     """``fa_kv8_layer`` of 8-bit slabs [num_blocks, kv_heads, bs, head_dim] (torch.float8_e4m3fn
     or torch.int8) and their f32 scales [num_blocks, kv_heads]."""
-    if k_cache.dtype not in _KV8:
+    fmt = _KV8.get(k_cache.dtype)
+    if fmt is None:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"unsupported 8-bit cache dtype {k_cache.dtype}")
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    shape = k_cache.shape
+    if v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, "k_cache and v_cache differ in shape or dtype")
-    if k_cache.dim() != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if len(shape) != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise _lib.FlourAttnError(_lib.FA_EINVAL,
                                   "cache slabs must be contiguous [num_blocks, kv_heads, bs, d]")
-    nb, kvh, bs, d = k_cache.shape
-    for t in (k_scale, v_scale):
-        if t.dtype != torch.float32 or t.shape != (nb, kvh) or not t.is_contiguous():
-            raise _lib.FlourAttnError(_lib.FA_EINVAL, f"scales must be contiguous f32 [{nb}, {kvh}]")
-    _device(k_cache.device, v_cache, k_scale, v_scale)
+    nb, kvh, bs, d = shape
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or \
+            k_scale.shape != (nb, kvh) or v_scale.shape != (nb, kvh) or \
+            not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"scales must be contiguous f32 [{nb}, {kvh}]")
     return _lib.FaKv8Layer(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                           v_scale.data_ptr(), nb, kvh, bs, d, _KV8[k_cache.dtype])
+                           v_scale.data_ptr(), nb, kvh, bs, d, fmt)
 
 
 def _tables(block_tables, context_lens, num_seqs: int):
@@ -442,13 +447,14 @@ def _cu(cu_seqlens_q, num_seqs: int):
     return cu
 
 
-def _query8(query, k_cache, out):
-    if query.dim() != 3 or query.shape[2] != k_cache.shape[3]:
-        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"query must be [tokens, heads, {k_cache.shape[3]}]")
+def _query8(query, d: int, out):
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != d:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"query must be [tokens, heads, {d}]")
     query = query.contiguous()
     if out is None:
         return query, torch.empty_like(query)
-    if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+    if out.shape != shape or out.dtype != query.dtype or not out.is_contiguous():
         raise _lib.FlourAttnError(_lib.FA_EINVAL, "out must be contiguous, of the query's shape and dtype")
     return query, out
 
@@ -461,33 +467,40 @@ def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_table
     when cu_seqlens_q is None) included. A block's scale is a power of two that grows as it
     fills. A block that receives tokens belongs to one sequence of the call."""
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
-    if key.shape != value.shape or key.dtype != value.dtype or \
-            key.dim() != 3 or key.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
+    shape = key.shape
+    if value.shape != shape or value.dtype is not key.dtype or len(shape) != 3 or \
+            shape[1] != layer.num_kv_heads or shape[2] != layer.head_dim:
         raise _lib.FlourAttnError(
-            _lib.FA_EINVAL, f"key/value must be [T, {k_cache.shape[1]}, {k_cache.shape[3]}] of one dtype")
-    if key.stride(-1) != 1 or value.stride(-1) != 1:
+            _lib.FA_EINVAL, f"key/value must be [T, {layer.num_kv_heads}, {layer.head_dim}] of one dtype")
+    k_token, k_head, k_unit = key.stride()
+    v_token, v_head, v_unit = value.stride()
+    if layer.head_dim > 1 and (k_unit != 1 or v_unit != 1):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, "key/value need unit stride on head_dim")
-    T = key.shape[0]
-    S = T if cu_seqlens_q is None else context_lens.numel()
+    T = shape[0]
+    cu = None
+    if cu_seqlens_q is None:
+        S = T
+    else:
+        S = context_lens.numel()
+        cu = _cu(cu_seqlens_q, S)
     bt, cl = _tables(block_tables, context_lens, S)
-    cu = None if cu_seqlens_q is None else _cu(cu_seqlens_q, S)
-    dev = _device(k_cache.device, key, value, bt, cl, cu)
+    dev = _device(k_cache, v_cache, k_scale, v_scale, key, value, bt, cl, cu)
     _call_on(dev, stream, "paged_append_kv8", lib().fa_paged_append_kv8, ctypes.byref(layer),
-             key.data_ptr(), value.data_ptr(), fa_dtype(key.dtype), key.stride(0), key.stride(1),
-             value.stride(0), value.stride(1), None if cu is None else cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1], S, T)
+             key.data_ptr(), value.data_ptr(), fa_dtype(key.dtype), k_token, k_head, v_token, v_head,
+             None if cu is None else cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1], S, T)
 
 
-def _ws8(workspace: Workspace | None, need: int, device: torch.device):
+def _ws8(workspace: Workspace | None, need: int, dev: int):
     if workspace is None or not need:
         return _ws_args(workspace, need)
-    if torch.cuda.current_device() == device.index:
-        args = _ws_args(workspace, need)
+    if torch._C._cuda_getDevice() == dev:
+        buf = workspace.get(need)
     else:
-        with torch.cuda.device(device):
-            args = _ws_args(workspace, need)
-    if workspace.buf.device != device:
-        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"workspace on {workspace.buf.device}, tensors on {device}")
-    return args
+        with torch.cuda.device(dev):
+            buf = workspace.get(need)
+    if buf.get_device() != dev:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"workspace on {buf.device}, tensors on cuda:{dev}")
+    return buf.data_ptr(), buf.numel()
 
 
 def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
@@ -495,15 +508,16 @@ def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, co
                      workspace: Workspace | None = None, out=None, stream=None):
     """paged_decode over an 8-bit pool: query [B, Hq, d] (bf16, f16 or f32) -> out [B, Hq, d]."""
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
-    query, out = _query8(query, k_cache, out)
+    query, out = _query8(query, layer.head_dim, out)
     B, hq, d = query.shape
     bt, cl = _tables(block_tables, context_lens, B)
-    dev = _device(k_cache.device, query, out, bt, cl)
-    need = int(lib().fa_paged_decode_kv8_workspace_size(B, hq, k_cache.shape[1], d, max_context_len))
-    wp, wn = _ws8(workspace, need, dev)
-    _call_on(dev, stream, "paged_decode_kv8", lib().fa_paged_decode_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cl.data_ptr(), bt.data_ptr(), bt.shape[1], B, hq,
-             n_rep, max_context_len, scale, wp, wn)
+    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl)
+    L = lib()
+    wp, wn = _ws8(workspace, L.fa_paged_decode_kv8_workspace_size(B, hq, layer.num_kv_heads, d,
+                                                                  max_context_len), dev)
+    _call_on(dev, stream, "paged_decode_kv8", L.fa_paged_decode_kv8, ctypes.byref(layer),
+             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cl.data_ptr(), bt.data_ptr(),
+             bt.shape[1], B, hq, n_rep, max_context_len, scale, wp, wn)
     return out
 
 
@@ -514,18 +528,19 @@ def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, c
     """paged_prefill over an 8-bit pool whose suffix tokens are already appended. `total_blocks`:
     at least the sum of ceil(context_len / block_size) over the batch."""
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
-    query, out = _query8(query, k_cache, out)
+    query, out = _query8(query, layer.head_dim, out)
     tq, hq, d = query.shape
     S = context_lens.numel()
     bt, cl = _tables(block_tables, context_lens, S)
     cu = _cu(cu_seqlens_q, S)
-    dev = _device(k_cache.device, query, out, bt, cl, cu)
-    need = int(lib().fa_paged_prefill_kv8_workspace_size(S, hq, k_cache.shape[1], d, tq, max_context_len,
-                                                         max_seqlen_q, total_blocks))
-    wp, wn = _ws8(workspace, need, dev)
-    _call_on(dev, stream, "paged_prefill_kv8", lib().fa_paged_prefill_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1],
-             S, hq, n_rep, tq, max_seqlen_q, max_context_len, total_blocks, scale, wp, wn)
+    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl, cu)
+    L = lib()
+    wp, wn = _ws8(workspace, L.fa_paged_prefill_kv8_workspace_size(
+        S, hq, layer.num_kv_heads, d, tq, max_context_len, max_seqlen_q, total_blocks), dev)
+    _call_on(dev, stream, "paged_prefill_kv8", L.fa_paged_prefill_kv8, ctypes.byref(layer),
+             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cu.data_ptr(), cl.data_ptr(),
+             bt.data_ptr(), bt.shape[1], S, hq, n_rep, tq, max_seqlen_q, max_context_len,
+             total_blocks, scale, wp, wn)
     return out
 
 
@@ -544,11 +559,12 @@ def token_logprobs(logits, token_ids=None, top_k: int = 0, stream=None):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"token_ids must be [{R}]")
     if not 0 <= top_k <= _lib.FA_MAX_TOP_LOGPROBS:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"top_k {top_k} outside [0, {_lib.FA_MAX_TOP_LOGPROBS}]")
-    dev = _device(logits.device, ids)
-    logprobs = None if ids is None else torch.empty(R, dtype=torch.float32, device=dev)
-    entropy = torch.empty(R, dtype=torch.float32, device=dev)
-    top_ids = torch.empty((R, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((R, top_k), dtype=torch.float32, device=dev)
+    dev = _device(logits, ids)
+    device, f32 = logits.device, torch.float32
+    logprobs = None if ids is None else torch.empty(R, dtype=f32, device=device)
+    entropy = torch.empty(R, dtype=f32, device=device)
+    top_ids = torch.empty((R, top_k), dtype=torch.int32, device=device)
+    top = torch.empty((R, top_k), dtype=f32, device=device)
     _call_on(dev, stream, "token_logprobs", lib().fa_token_logprobs, logits.data_ptr(), fa_dtype(logits.dtype),
              logits.stride(0), R, V, None if ids is None else ids.data_ptr(),
              None if ids is None else logprobs.data_ptr(), entropy.data_ptr(), top_k,
