@@ -469,7 +469,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     s_misc[2 * warp] = pieces[0];
     s_misc[2 * warp + 1] = pieces[1];
   }
-  if (tid == 0) s_misc[16] = -1;  // the item last looked at
   __syncthreads();  // the warps' pieces are written, and every ring is drained
 
   // ---- join the pieces ------------------------------------------------------------------------
@@ -477,35 +476,43 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   // segment of a worker's range in its slot 0, a later one in slot 1. An item inside this CTA is
   // joined here; one that others have a part of by the last CTA to take its ticket. Where more than
   // kKv8Direct CTAs share an item, each joins its own pieces first.
-  float *s_lse = reinterpret_cast<float *>(smem);  // [8][pieces] over the drained rings
-  const int cpp = kDecodeWarps * ppw;              // pairs per CTA
-  // Piece k of n at row(k) of the pieces -> dst (f32, with its lse), or the output.
+  const int cpp = kDecodeWarps * ppw;  // pairs per CTA
+  // Piece k of n at row(k) of the pieces -> dst (f32, with its lse), or the output. Four values of
+  // head_dim a thread; eight pieces and their sums in flight, folded into a running maximum.
   auto join = [&](int item, int n, auto row, float *dst, float *dst_lse) {
-    for (int x = tid; x < n_rep * n; x += kDecodeThreads)
-      s_lse[x] = __ldcg(&p.piece_lse[row(x / n_rep) * n_rep + x % n_rep]);
-    __syncthreads();
     for (int x = tid; x < n_rep * (HD / 4); x += kDecodeThreads) {
       const int h = x / (HD / 4), d = x % (HD / 4) * 4;
-      float M = neg_inf();
-      for (int k = 0; k < n; ++k) M = fmaxf(M, s_lse[k * n_rep + h]);
+      float M = neg_inf(), W = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-      float W = 0.f;
-      for (int k0 = 0; k0 < n; k0 += 8) {  // eight loads in flight
+      for (int k0 = 0; k0 < n; k0 += 8) {
         float4 v[8];
+        float e[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (k0 + u < n)
-            v[u] = __ldcg(reinterpret_cast<const float4 *>(p.pieces + (row(k0 + u) * n_rep + h) * HD + d));
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 8; ++u) {
+          e[u] = neg_inf();
+          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (k0 + u < n) {
-            const float e = ex2(s_lse[(k0 + u) * n_rep + h] - M);
-            O.x += e * v[u].x;
-            O.y += e * v[u].y;
-            O.z += e * v[u].z;
-            O.w += e * v[u].w;
-            W += e;
+            const size_t r = row(k0 + u) * n_rep + h;
+            e[u] = __ldcg(p.piece_lse + r);
+            v[u] = __ldcg(reinterpret_cast<const float4 *>(p.pieces + r * HD + d));
           }
+        }
+        float m = M;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m = fmaxf(m, e[u]);
+        const float c = ex2(M - m);
+        O = make_float4(O.x * c, O.y * c, O.z * c, O.w * c);
+        W *= c;
+        M = m;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float w = ex2(e[u] - m);
+          O.x += w * v[u].x;
+          O.y += w * v[u].y;
+          O.z += w * v[u].z;
+          O.w += w * v[u].w;
+          W += w;
+        }
       }
       const float i = 1.f / W;
       if (dst) {
@@ -516,7 +523,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
         *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
       }
     }
-    __syncthreads();  // s_lse is free again
   };
   struct Span {
     int a0, a1;  // the item's pairs
@@ -539,13 +545,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   };
   // The (at most two) items that other CTAs share: the first with a piece here, and the last.
   int shared[2] = {-1, -1};
-  for (int k = 0; k < 2 * kDecodeWarps; ++k) {
+  for (int k = 0, seen = -1; k < 2 * kDecodeWarps; ++k) {
     const int item = s_misc[k];
-    if (item < 0 || item == s_misc[16]) continue;
-    // a new item (its pieces follow one another)
-    __syncthreads();
-    if (tid == 0) s_misc[16] = item;
-    __syncthreads();
+    if (item < 0 || item == seen) continue;  // an item's pieces follow one another
+    seen = item;
     const Span sp = span(item);
     int first;
     const int n = pieces_of(sp, c0, c1, first);
@@ -561,20 +564,21 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     shared[sp.a0 < c0 ? 0 : 1] = item;
   }
   if (shared[0] < 0 && shared[1] < 0) return;
-  __threadfence();
+  // The barrier orders the CTA's pieces before the release of its tickets.
   __syncthreads();
   if (tid < 2) {
     const int item = shared[tid];
     int last = 0;
     if (item >= 0) {
       const Span sp = span(item);
+      __threadfence();
       last = atomicAdd(&p.tickets[item], 1) == (sp.a1 - 1) / cpp - sp.a0 / cpp;
+      __threadfence();
     }
     s_misc[16 + tid] = last;
   }
   __syncthreads();
   if (!s_misc[16] && !s_misc[17]) return;
-  __threadfence();
 #pragma unroll 1
   for (int x = 0; x < 2; ++x) {
     if (!s_misc[16 + x]) continue;
