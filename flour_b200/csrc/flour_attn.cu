@@ -902,7 +902,8 @@ Decode8Plan plan_decode8(int num_seqs, int num_kv_heads, int max_context_len) {
   d.seqs = int(std::min<int64_t>(std::min(num_seqs, fa::kKv8MaxSeqs),
                                  std::max<int64_t>(1, (int64_t(1) << 30) / std::max<int64_t>(1, pairs))));
   const int64_t cta = fa::kDecodeWarps * fa::kKv8MinPairs;
-  d.grid = int(std::max<int64_t>(1, std::min<int64_t>(3 * sm_count(), (d.seqs * pairs + cta - 1) / cta)));
+  const int64_t most = std::max<int64_t>((d.seqs * pairs + cta - 1) / cta, int64_t(d.seqs) * num_kv_heads);
+  d.grid = int(std::max<int64_t>(1, std::min<int64_t>(3 * sm_count(), most)));
   return d;
 }
 
