@@ -147,23 +147,42 @@ __device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
     return unpack2<T>(i == 0 ? v.x : i == 2 ? v.y : i == 4 ? v.z : v.w);
 }
 
-// z and w of the logits in `raw` against m >= all of them (m may be -inf: then nothing but NaN
-// counts). Four operations a logit: with L = log2(e), M = m L rounded and r = m L - M (one fma, so
-// exact), s = x L - M is one fma, e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r leaves the sums.
-template <typename T, int NV>
+// z and w of one vector of logits with care: masked logits (whose 0 * -inf must not count), a NaN,
+// logits whose product with log2(e) overflows, or none but -inf (m = -inf: only NaN counts).
+template <typename T>
+__device__ __forceinline__ float2 lp_sums_slow(uint4 v, float m) {
+  const uint4 raw[1] = {v};
+  float z = 0.f, w = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16 / int(sizeof(T)); j += 2) {
+    const float2 x = lp_pair<T>(raw, j);
+    if (m == neg_inf()) {
+      if (x.x != x.x || x.y != x.y) z = x.x + x.y;
+    } else {
+      const float d0 = x.x - m, d1 = x.y - m;
+      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
+      z += e0 + e1;
+      w = fmaf(e0, fmaxf(d0, -1e30f), w);
+      w = fmaf(e1, fmaxf(d1, -1e30f), w);
+    }
+  }
+  return make_float2(z, w);
+}
+
+template <typename T> __device__ __noinline__ float2 lp_sums_slow_call(uint4 v, float m) {
+  return lp_sums_slow<T>(v, m);
+}
+
+// z and w of the logits in `raw` against m >= all of them. Four operations a logit: with
+// L = log2(e), M = m L rounded and r = m L - M (one fma, so exact), s = x L - M is one fma,
+// e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r leaves the sums. Where that fails (see above; all
+// such cases make the sum NaN) the vectors are summed once more with care: by a call in the streaming
+// loop, whose code has to stay in the instruction cache (-2.5 %), in place in the part kernel, where
+// every row's last threads come here (-0.5 us).
+template <typename T, bool kCall, int NV>
 __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &z, float &w) {
   constexpr int N = NV * 16 / sizeof(T);
-  if (m == neg_inf()) {
-#pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const float2 x = lp_pair<T>(raw, j);
-      if (x.x != x.x) z = x.x;
-      if (x.y != x.y) z = x.y;
-    }
-    return;
-  }
-  const float M = m * kLog2e;
-  const float r = fmaf(m, kLog2e, -M);
+  const float M = m * kLog2e, r = fmaf(m, kLog2e, -M);
   float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
@@ -177,17 +196,13 @@ __device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &
   }
   const float back = ex2(-r);
   float zs = (z0 + z1) * back, ws = fmaf(-r, z0 + z1, w0 + w1) * (back * 0.693147180559945f);
-  // A masked logit's 0 * -inf, a NaN, or logits too large for M: once more, with care.
   if (ws != ws) {
     zs = ws = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const float2 x = lp_pair<T>(raw, j);
-      const float d0 = x.x - m, d1 = x.y - m;
-      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
-      zs += e0 + e1;
-      ws = fmaf(e0, fmaxf(d0, -1e30f), ws);
-      ws = fmaf(e1, fmaxf(d1, -1e30f), ws);
+    for (int i = 0; i < NV; ++i) {
+      const float2 a = kCall ? lp_sums_slow_call<T>(raw[i], m) : lp_sums_slow<T>(raw[i], m);
+      zs += a.x;
+      ws += a.y;
     }
   }
   z += zs;
@@ -528,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
   float z = 0.f, w = 0.f;
-  lp_sums<T>(raw, m, z, w);
+  lp_sums<T, false>(raw, m, z, w);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -638,7 +653,7 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
       }
       if (tm >= bound) lp_pool_add(s_pool, raw, vm, bound, r, vt + tid, THREADS);
     }
-    lp_sums<T>(raw, st.m, st.z, st.w);
+    lp_sums<T, true>(raw, st.m, st.z, st.w);
   }
   st = lp_warp_join(st);
   if (lane == 0) s_state[warp] = st;
