@@ -143,10 +143,10 @@ SIGNATURES = {
     "fa_last_token_logits": (_I32, [_P, _P, _I32, _I32, _P, _F, _P, _I32, _I32, _I32, _P, _P, _P]),
     "fa_paged_append_kv8": (_I32, [_L8, _P, _P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32,
                                    _I32, _P]),
-    "fa_paged_decode_kv8_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "fa_paged_decode_kv8_workspace_size": (_SZ, [_I32] * 7),
     "fa_paged_decode_kv8": (_I32, [_L8, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, _P,
                                    _SZ, _P]),
-    "fa_paged_prefill_kv8_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "fa_paged_prefill_kv8_workspace_size": (_SZ, [_I32] * 10),
     "fa_paged_prefill_kv8": (_I32, [_L8, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32,
                                     _I32, _I32, _F, _P, _SZ, _P]),
     "fa_token_logprobs": (_I32, [_P, _I32, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P]),

@@ -871,9 +871,13 @@ fa_status launch_pdl(const char *who, void (*kern)(KArgs...), dim3 grid, int thr
   return check_launch(who);
 }
 
+bool decode8_fast_shape(int32_t dtype, int n_rep, int block_size, int head_dim) {
+  return (dtype == FA_BF16 || dtype == FA_F16) && block_size == fa::kPage &&
+         (head_dim == 64 || head_dim == 128) && n_rep >= 1 && n_rep <= 8;
+}
+
 bool decode8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, const void *q, const void *out) {
-  return (dtype == FA_BF16 || dtype == FA_F16) && L->block_size == fa::kPage &&
-         (L->head_dim == 64 || L->head_dim == 128) && n_rep >= 1 && n_rep <= 8 &&
+  return decode8_fast_shape(dtype, n_rep, L->block_size, L->head_dim) &&
          int64_t(L->num_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
          aligned(L->k_cache, 16) && aligned(L->v_cache, 16) && aligned(q, 8) && aligned(out, 8);
 }
@@ -1034,10 +1038,15 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
 }
 
 // Whether the tcgen05 prefill serves a call, over a copy of the cache in the query type.
+bool prefill8_fast_shape(int32_t dtype, int n_rep, int block_size, int head_dim, int num_seqs,
+                         int32_t total_blocks) {
+  return (dtype == FA_BF16 || dtype == FA_F16) && block_size == fa::kPage && head_dim == 128 &&
+         n_rep >= 1 && n_rep <= 128 && num_seqs <= fa::kExpandMaxSeqs && total_blocks > 0;
+}
+
 bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float scale, const void *q,
                         const void *out, int num_seqs, int32_t total_blocks) {
-  return (dtype == FA_BF16 || dtype == FA_F16) && L->block_size == fa::kPage && L->head_dim == 128 &&
-         n_rep >= 1 && n_rep <= 128 && scale > 0.f && num_seqs <= fa::kExpandMaxSeqs &&
+  return prefill8_fast_shape(dtype, n_rep, L->block_size, L->head_dim, num_seqs, total_blocks) && scale > 0.f &&
          int64_t(total_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
          aligned(L->k_cache, 8) && aligned(L->v_cache, 8) && aligned(q, 16) && aligned(out, 32);
 }
@@ -1045,8 +1054,8 @@ bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float s
 // How many parts to cut the contexts of a batch into: as long as the chunks (upper bound: the host
 // knows total_q, not the lengths) do not fill the SMs a few times. In KV tiles of one item (about
 // 2.1 us): a wave of items lasts its longest part plus 1.2 for the item's start and end, and the
-// join moves every part's rows twice (one tile per 14 MB). Measured on one sequence of 509 tokens
-// over 30001 (28 query heads, 4 KV heads, 60 items): 512 us unsplit; see prefill_split's callers.
+// join moves every part's rows twice (one tile per 14 MB). One sequence of 509 tokens over 30001 (28
+// query heads, 4 KV heads: 60 items) takes 512 us unsplit and 274 in the 7 parts chosen here.
 PrefillSplit plan_prefill_split(int num_seqs, int num_heads, int num_kv_heads, int total_q, int max_context_len) {
   const int chunk = 2 * (128 / (num_heads / num_kv_heads)), sms = sm_count();
   const int64_t items =
@@ -1086,9 +1095,7 @@ Prefill8Workspace prefill8_workspace_layout(int num_seqs, int num_heads, int num
   const size_t slab = r256(size_t(std::max(1, total_blocks)) * num_kv_heads * fa::kPage * head_dim * 2);
   w.v_off = w.k_off + slab;
   w.part_off = w.v_off + slab;
-  const int parts = num_heads / num_kv_heads > 128
-                        ? 1
-                        : plan_prefill_split(num_seqs, num_heads, num_kv_heads, total_q, max_context_len).parts;
+  const int parts = plan_prefill_split(num_seqs, num_heads, num_kv_heads, total_q, max_context_len).parts;
   w.bytes = w.part_off + (parts > 1 ? size_t(parts) * total_q * num_heads * 129 * 4 : 0);
   return w;
 }
@@ -1717,10 +1724,11 @@ fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const 
   });
 }
 
-size_t fa_paged_decode_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                          int32_t head_dim, int32_t max_context_len) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context_len <= 0 ||
-      num_heads % num_kv_heads != 0)
+size_t fa_paged_decode_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                                          int32_t max_context_len) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len <= 0 ||
+      num_heads % num_kv_heads != 0 || !decode8_fast_shape(dtype, num_heads / num_kv_heads, block_size, head_dim))
     return 0;
   return decode8_workspace_layout(num_heads, num_kv_heads, head_dim,
                                   plan_decode8(num_seqs, num_kv_heads, max_context_len))
@@ -1750,18 +1758,21 @@ fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void
                          num_seqs, num_heads, n_rep, num_seqs, scale, st, who);
 }
 
-size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                           int32_t head_dim, int32_t total_q, int32_t max_context_len,
-                                           int32_t max_seqlen_q, int32_t total_blocks) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || total_q <= 0 ||
-      max_context_len <= 0 || total_blocks < 0 || num_heads % num_kv_heads != 0)
+size_t fa_paged_prefill_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
+                                           int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                                           int32_t total_q, int32_t max_context_len, int32_t max_seqlen_q,
+                                           int32_t total_blocks) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || total_q <= 0 || max_context_len <= 0 ||
+      num_heads % num_kv_heads != 0)
     return 0;
-  const size_t copy = prefill8_workspace_layout(num_seqs, num_heads, num_kv_heads, head_dim, total_q,
-                                                max_context_len, total_blocks)
-                          .bytes;
-  if (max_seqlen_q != 1) return copy;
-  return std::max(copy, fa_paged_decode_kv8_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim,
-                                                           max_context_len));
+  if (max_seqlen_q == 1 && total_q == num_seqs)  // the decode
+    return fa_paged_decode_kv8_workspace_size(dtype, num_seqs, num_heads, num_kv_heads, block_size, head_dim,
+                                              max_context_len);
+  if (!prefill8_fast_shape(dtype, num_heads / num_kv_heads, block_size, head_dim, num_seqs, total_blocks))
+    return 0;
+  return prefill8_workspace_layout(num_seqs, num_heads, num_kv_heads, head_dim, total_q, max_context_len,
+                                   total_blocks)
+      .bytes;
 }
 
 fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, void *out, int32_t dtype,
@@ -1788,8 +1799,7 @@ fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, voi
                                num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
                                workspace_bytes, stream);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (total_blocks > 0 &&
-      prefill8_fast_path(layer, n_rep, dtype, scale, query, out, num_seqs, total_blocks))
+  if (prefill8_fast_path(layer, n_rep, dtype, scale, query, out, num_seqs, total_blocks))
     return launch_prefill8(layer, query, out, dtype, cu_seqlens_q, context_lens, block_tables,
                            max_blocks_per_seq, num_seqs, num_heads, n_rep, total_q, max_context_len,
                            total_blocks, scale, workspace, workspace_bytes, st);

@@ -513,10 +513,11 @@ def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, co
     bt, cl = _tables(block_tables, context_lens, B)
     dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl)
     L = lib()
-    wp, wn = _ws8(workspace, L.fa_paged_decode_kv8_workspace_size(B, hq, layer.num_kv_heads, d,
-                                                                  max_context_len), dev)
+    dt = fa_dtype(query.dtype)
+    wp, wn = _ws8(workspace, L.fa_paged_decode_kv8_workspace_size(
+        dt, B, hq, layer.num_kv_heads, layer.block_size, d, max_context_len), dev)
     _call_on(dev, stream, "paged_decode_kv8", L.fa_paged_decode_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cl.data_ptr(), bt.data_ptr(),
+             query.data_ptr(), out.data_ptr(), dt, cl.data_ptr(), bt.data_ptr(),
              bt.shape[1], B, hq, n_rep, max_context_len, scale, wp, wn)
     return out
 
@@ -535,10 +536,12 @@ def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, c
     cu = _cu(cu_seqlens_q, S)
     dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl, cu)
     L = lib()
+    dt = fa_dtype(query.dtype)
     wp, wn = _ws8(workspace, L.fa_paged_prefill_kv8_workspace_size(
-        S, hq, layer.num_kv_heads, d, tq, max_context_len, max_seqlen_q, total_blocks), dev)
+        dt, S, hq, layer.num_kv_heads, layer.block_size, d, tq, max_context_len, max_seqlen_q,
+        total_blocks), dev)
     _call_on(dev, stream, "paged_prefill_kv8", L.fa_paged_prefill_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), fa_dtype(query.dtype), cu.data_ptr(), cl.data_ptr(),
+             query.data_ptr(), out.data_ptr(), dt, cu.data_ptr(), cl.data_ptr(),
              bt.data_ptr(), bt.shape[1], S, hq, n_rep, tq, max_seqlen_q, max_context_len,
              total_blocks, scale, wp, wn)
     return out

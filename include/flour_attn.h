@@ -327,8 +327,8 @@ typedef struct fa_kv8_layer {
  * loses at most one int8 step in all, and nothing in e4m3 above its subnormals.
  * Infinities saturate; NaN is stored as e4m3's NaN or int8's 0; either sets FA_DEVERR_VALUE and
  * leaves the scale to the finite values.
- * A block that receives tokens must belong to one sequence of the call (a shared prefix block is
- * copied before it is written). Rows of key/value behind cu_seqlens_q[num_seqs] are not read. A
+ * A block that receives tokens must appear once, in one sequence's table (a shared prefix block is
+ * copied before it is written): where it does not, its bytes are those of any of the writers. Rows of key/value behind cu_seqlens_q[num_seqs] are not read. A
  * sequence with bad lengths (FA_DEVERR_CONTEXT / FA_DEVERR_SEQLEN) or block ids
  * (FA_DEVERR_BLOCK_ID) is not written there. No workspace. */
 FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const void *value,
@@ -344,11 +344,12 @@ FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key,
  * bytes among them). A sequence with an invalid length gives zeros and FA_DEVERR_CONTEXT.
  * The fast kernel takes FA_BF16 / FA_F16 queries, block_size 16, head_dim 64 or 128, n_rep <= 8,
  * 16-byte aligned slabs and an 8-byte aligned query; everything else runs the generic kernel.
- * Workspace: fa_paged_decode_kv8_workspace_size bytes, under the rules of
- * fa_paged_attention_workspace_size (it may be the same buffer). */
-FA_API size_t fa_paged_decode_kv8_workspace_size(int32_t num_seqs, int32_t num_heads,
-                                                 int32_t num_kv_heads, int32_t head_dim,
-                                                 int32_t max_context_len);
+ * Workspace: fa_paged_decode_kv8_workspace_size bytes (0: none), under the rules of
+ * fa_paged_attention_workspace_size (it may be the same buffer). The generic kernel needs none;
+ * buffers that are not aligned for the fast kernel run it whatever the workspace. */
+FA_API size_t fa_paged_decode_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
+                                                 int32_t num_kv_heads, int32_t block_size,
+                                                 int32_t head_dim, int32_t max_context_len);
 FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void *out,
                                      int32_t dtype, const int32_t *context_lens,
                                      const int32_t *block_tables, int32_t max_blocks_per_seq,
@@ -367,10 +368,11 @@ FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *quer
  * the generic kernel, which needs no workspace. One new token per sequence (max_seqlen_q 1,
  * total_q == num_seqs) is fa_paged_decode_kv8. Output rows behind cu_seqlens_q[num_seqs] are not
  * written by the tensor-core path. */
-FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t num_seqs, int32_t num_heads,
-                                                  int32_t num_kv_heads, int32_t head_dim,
-                                                  int32_t total_q, int32_t max_context_len,
-                                                  int32_t max_seqlen_q, int32_t total_blocks);
+FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
+                                                  int32_t num_kv_heads, int32_t block_size,
+                                                  int32_t head_dim, int32_t total_q,
+                                                  int32_t max_context_len, int32_t max_seqlen_q,
+                                                  int32_t total_blocks);
 FA_API fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, void *out,
                                       int32_t dtype, const int32_t *cu_seqlens_q,
                                       const int32_t *context_lens, const int32_t *block_tables,

@@ -469,6 +469,104 @@ def test_side_stream_and_append_then_decode_chain(device):
         assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("S, ctx_hi", [(500, 40), (1100, 20)])
+def test_many_sequences(device, S, ctx_hi):
+    # More sequences than one decode launch takes, more than the append searches in shared memory.
+    rng = np.random.default_rng(45)
+    ctx = rng.integers(1, ctx_hi + 1, S)
+    new = np.minimum(rng.integers(0, 4, S), ctx)
+    ctx[::7], new[::7] = 2, 2
+    bt, nb = make_tables(ctx, 16, 45)
+    g = gen_of(device, 45)
+    pool = random_pool(nb, 2, 16, 64, torch.int8, g, device)
+    T = int(new.sum())
+    key, value = (torch.randn((T, 2, 64), device=device, generator=g).to(torch.float16) for _ in "kv")
+    before = clone(pool)
+    run_append(pool, key, value, bt, ctx, new, device)
+    check_append(pool, before, key, value, bt, ctx, new)
+    q = torch.randn((S, 8, 64), device=device, generator=g).to(torch.bfloat16)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [1] * S, 4,
+                              inv_sqrt(64), U16)
+    assert_close(run_decode(pool, q, i32(bt, device), i32(ctx, device), ctx, 2), want, tol)
+    assert ops.device_status() == 0
+
+
+def test_prefill_of_many_sequences(device):
+    # 2049 sequences are more than the copy to 16 bits takes in one call: the generic kernel.
+    for S in (300, 2049):
+        rng = np.random.default_rng(46)
+        ctx = rng.integers(1, 20, S)
+        new = np.minimum(rng.integers(0, 3, S), ctx)
+        bt, nb = make_tables(ctx, 16, 46)
+        g = gen_of(device, 46)
+        pool = random_pool(nb, 1, 16, 128, torch.float8_e4m3fn, g, device)
+        q = torch.randn((int(new.sum()), 4, 128), device=device, generator=g).to(torch.float16)
+        want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, 4,
+                                  inv_sqrt(128), U16)
+        assert_close(run_prefill(pool, q, bt, ctx, new, 1, device), want, tol)
+        assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("ctx", [[20000, 5, 17, 90, 1], [31, 4000, 30, 33, 3000], [512] * 9, [513] * 60])
+def test_decode_skewed_batches_repeat(device, ctx):
+    # One sequence holds nearly all pages, or items end inside and at the ends of the warps' ranges.
+    for fmt in FMTS:
+        pool, q, bt, cl, want, tol = decode_case(device, fmt, torch.float16, 8, 2, 128, ctx, 47)
+        ws = ops.Workspace()
+        out = run_decode(pool, q, bt, cl, ctx, 2, ws)
+        assert_close(out, want, tol)
+        for _ in range(3):  # the same bits whichever CTA joins, and tickets back at zero
+            assert torch.equal(run_decode(pool, q, bt, cl, ctx, 2, ws), out)
+        # A larger bound than the longest context: the same ranges.
+        again = ops.paged_decode_kv8(q, *pool, bt, cl, 4, inv_sqrt(128), bt.shape[1] * 16, ws)
+        assert_close(again, want, tol)
+    assert ops.device_status() == 0
+
+
+def test_zero_and_invalid_sequences_in_a_batch(device):
+    ctx = [100, 0, 700, 64]
+    pool, q, bt, cl, want, tol = decode_case(device, torch.float8_e4m3fn, torch.bfloat16, 8, 2, 128,
+                                             [100, 16, 700, 64], 48)
+    cl = i32([100, 0, 701 + 16, 64], device)  # none, fine but for the third: past the table
+    ops.device_status()
+    out = run_decode(pool, q, bt[:, :44].contiguous(), cl, [704], 2)
+    assert ops.device_status() == _lib.FA_DEVERR_CONTEXT
+    assert not out[1].any() and not out[2].any()
+    for r in (0, 3):
+        assert_close(out[r:r + 1], want[r:r + 1], tol[r:r + 1])
+    out = run_decode(pool, q, bt, i32([0, -5, 0, 0], device), ctx, 2)
+    assert ops.device_status() == _lib.FA_DEVERR_CONTEXT
+    assert not out.any()
+
+
+def test_offsets_past_32_bits(device):
+    # Slabs of more than 2^32 bytes, the batch's blocks at both ends.
+    H, d, nb = 8, 128, (1 << 32) // (8 * 16 * 128) + 5000
+    kc = torch.zeros((nb, H, 16, d), dtype=torch.int8, device=device)
+    vc = torch.zeros_like(kc)
+    ks, vs = (torch.zeros((nb, H), device=device) for _ in "kv")
+    g = gen_of(device, 49)
+    ctx, ids = [60, 75], [[3, nb - 1, 0, nb - 7, 0], [nb - 2, 1, nb - 3, 5, nb - 4]]
+    bt = np.array(ids, np.int32)
+    key, value = (torch.randn((135, H, d), device=device, generator=g).to(torch.bfloat16) for _ in "kv")
+    ops.paged_append_kv8(kc, vc, ks, vs, key, value, i32(bt, device), i32(ctx, device), i32([0, 60, 135], device))
+    q = torch.randn((135, 32, d), device=device, generator=g).to(torch.bfloat16)
+    small = {int(b): i for i, b in enumerate(sorted({b for r in ids for b in r}))}
+    at = torch.tensor(sorted(small), device=device)
+    pool = tuple(t[at] for t in (kc, vc, ks, vs))
+    bt_small = np.vectorize(lambda b: small[int(b)])(bt).astype(np.int32)
+    raw, sc = np.zeros(pool[0].shape, np.uint8), np.zeros(pool[2].shape, np.float32)
+    append_ref(raw, sc, torch.int8, key.double().cpu().numpy(), bt_small, ctx, ctx)
+    np.testing.assert_array_equal(pool[0].view(torch.uint8).cpu().numpy(), raw)
+    np.testing.assert_array_equal(pool[2].cpu().numpy(), sc)
+    big = (kc, vc, ks, vs)
+    assert torch.equal(run_prefill(big, q, bt, ctx, ctx, H, device), run_prefill(pool, q, bt_small, ctx, ctx, H, device))
+    last = q[[59, 134]].contiguous()
+    assert torch.equal(run_decode(big, last, i32(bt, device), i32(ctx, device), ctx, H),
+                       run_decode(pool, last, i32(bt_small, device), i32(ctx, device), ctx, H))
+    assert ops.device_status() == 0
+
+
 def test_blocks_are_copied_with_their_scales(device):
     # Copy-on-write of an 8-bit block with fa_copy_blocks: slabs as bf16 of half the head_dim,
     # scales as f32 layers of one element.

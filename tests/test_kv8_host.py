@@ -66,7 +66,7 @@ def test_attention_refusals():
     assert decode(layer8(), S=65536) == _lib.FA_EUNSUPPORTED
     assert decode(layer8(), S=0) == _lib.FA_OK
     big = layer8(nb=4096, kvh=8, d=128)
-    need = lib().fa_paged_decode_kv8_workspace_size(64, 32, 8, 128, 4096)
+    need = lib().fa_paged_decode_kv8_workspace_size(_lib.FA_BF16, 64, 32, 8, 16, 128, 4096)
     assert need > 0
     for ws, n, st in ((None, 0, _lib.FA_EINVAL), (P(0x100000), need - 1, _lib.FA_ERANGE),
                       (P(0x100010), need, _lib.FA_EINVAL)):
@@ -77,13 +77,29 @@ def test_attention_refusals():
     assert prefill(layer8(), mq=65) == _lib.FA_ERANGE
     assert prefill(layer8(), T=0) == _lib.FA_OK
     fast = layer8(d=128)
-    need = lib().fa_paged_prefill_kv8_workspace_size(1, 4, 2, 128, 8, 64, 8, 4)
+    need = lib().fa_paged_prefill_kv8_workspace_size(_lib.FA_BF16, 1, 4, 2, 16, 128, 8, 64, 8, 4)
     assert need >= 2 * 4 * 2 * 16 * 128 * 2
     assert prefill(fast, ws=None) == _lib.FA_EINVAL
     assert prefill(fast, ws=P(0x100000), n=need - 1) == _lib.FA_ERANGE
-    # One token each may take the decode: its workspace is covered too.
-    assert lib().fa_paged_prefill_kv8_workspace_size(64, 32, 8, 128, 64, 4096, 1, 0) >= \
-        lib().fa_paged_decode_kv8_workspace_size(64, 32, 8, 128, 4096)
+
+
+def test_workspace_sizes_follow_the_path():
+    dec, pre = lib().fa_paged_decode_kv8_workspace_size, lib().fa_paged_prefill_kv8_workspace_size
+    # One token each is the decode.
+    assert pre(_lib.FA_F16, 64, 32, 8, 16, 128, 64, 4096, 1, 9) == dec(_lib.FA_F16, 64, 32, 8, 16, 128, 4096) > 0
+    # Shapes of the generic kernel need none.
+    assert dec(_lib.FA_F32, 64, 32, 8, 16, 128, 4096) == 0
+    assert dec(_lib.FA_BF16, 64, 32, 8, 8, 128, 4096) == 0
+    assert dec(_lib.FA_BF16, 64, 32, 8, 16, 96, 4096) == 0
+    assert dec(_lib.FA_BF16, 64, 32, 2, 16, 128, 4096) == 0   # n_rep 16
+    assert dec(_lib.FA_BF16, 64, 30, 8, 16, 128, 4096) == 0   # not a multiple
+    for bad in ((_lib.FA_F32, 1, 4, 2, 16, 128, 8, 64, 8, 4), (_lib.FA_BF16, 1, 4, 2, 16, 64, 8, 64, 8, 4),
+                (_lib.FA_BF16, 1, 4, 2, 16, 128, 8, 64, 8, 0), (_lib.FA_BF16, 2049, 4, 2, 16, 128, 9000, 64, 8, 4)):
+        assert pre(*bad) == 0
+    # The copy grows with the blocks, the parts with the query rows of a long context.
+    a, b = (pre(_lib.FA_BF16, 1, 28, 4, 16, 128, 509, 30001, 509, n) for n in (1876, 3752))
+    assert b - a == 2 * 1876 * 4 * 16 * 128 * 2
+    assert a - 2 * 1876 * 4 * 16 * 128 * 2 > 509 * 28 * 129 * 4 * 2
 
 
 def test_logprobs_refusals():
