@@ -871,13 +871,19 @@ fa_status launch_pdl(const char *who, void (*kern)(KArgs...), dim3 grid, int thr
   return check_launch(who);
 }
 
+// Start of an 8-bit workspace: the prefill kernel's work counters, then the decode's tickets, both
+// zero between launches. What calls leave behind lies past it, so calls of any sizes, captured or
+// not, may share a workspace without clearing anything.
+constexpr size_t kKv8Reserved = 256 * 1024;
+constexpr int kKv8MaxTickets = int((kKv8Reserved - kPrefillWorkspace) / 4);
+
 bool decode8_fast_shape(int32_t dtype, int n_rep, int block_size, int head_dim) {
   return (dtype == FA_BF16 || dtype == FA_F16) && block_size == fa::kPage &&
          (head_dim == 64 || head_dim == 128) && n_rep >= 1 && n_rep <= 8;
 }
 
 bool decode8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, const void *q, const void *out) {
-  return decode8_fast_shape(dtype, n_rep, L->block_size, L->head_dim) &&
+  return decode8_fast_shape(dtype, n_rep, L->block_size, L->head_dim) && L->num_kv_heads <= kKv8MaxTickets &&
          int64_t(L->num_blocks) * L->num_kv_heads * L->block_size < (int64_t(1) << 31) &&
          aligned(L->k_cache, 16) && aligned(L->v_cache, 16) && aligned(q, 8) && aligned(out, 8);
 }
@@ -896,15 +902,17 @@ fa_status launch_decode8_t(const fa::Kv8DecodeParams &p, int grid, const CUtenso
 }
 
 // CTAs of one launch: three per SM, fewer where even the longest possible batch has fewer ranges.
-// Sequences of one launch: as many as the kernel's prefix sums hold, and as their pairs fit 30 bits.
+// Sequences of one launch: as many as the kernel's prefix sums and the tickets hold, and as their
+// pairs fit 30 bits.
 struct Decode8Plan {
   int seqs, grid;
 };
 Decode8Plan plan_decode8(int num_seqs, int num_kv_heads, int max_context_len) {
   const int64_t pairs = int64_t(num_kv_heads) * ((max_context_len + 2 * fa::kPage - 1) / (2 * fa::kPage));
   Decode8Plan d;
-  d.seqs = int(std::min<int64_t>(std::min(num_seqs, fa::kKv8MaxSeqs),
-                                 std::max<int64_t>(1, (int64_t(1) << 30) / std::max<int64_t>(1, pairs))));
+  const int64_t fit = std::min<int64_t>((int64_t(1) << 30) / std::max<int64_t>(1, pairs),
+                                        kKv8MaxTickets / num_kv_heads);
+  d.seqs = int(std::min<int64_t>(std::min(num_seqs, fa::kKv8MaxSeqs), std::max<int64_t>(1, fit)));
   const int64_t cta = fa::kDecodeWarps * fa::kKv8MinPairs;
   const int64_t most = std::max<int64_t>((d.seqs * pairs + cta - 1) / cta, int64_t(d.seqs) * num_kv_heads);
   d.grid = int(std::max<int64_t>(1, std::min<int64_t>(3 * sm_count(), most)));
@@ -912,13 +920,13 @@ Decode8Plan plan_decode8(int num_seqs, int num_kv_heads, int max_context_len) {
 }
 
 struct Decode8Workspace {
-  size_t lse_off, o_off, bytes;  // tickets at 0
+  size_t lse_off, o_off, bytes;
 };
 Decode8Workspace decode8_workspace_layout(int num_heads, int num_kv_heads, int head_dim, const Decode8Plan &d) {
   auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
   Decode8Workspace w;
   const size_t rows = size_t(d.grid) * fa::kKv8Pieces * (num_heads / num_kv_heads);
-  w.lse_off = r256(size_t(d.seqs) * num_kv_heads * 4);
+  w.lse_off = kKv8Reserved;
   w.o_off = w.lse_off + r256(rows * 4);
   w.bytes = w.o_off + rows * head_dim * 4;
   return w;
@@ -933,10 +941,9 @@ fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_
   if (ws_bytes < w.bytes)
     return fail(FA_ERANGE, "paged_decode_kv8: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
   if (!aligned(ws, 256)) return fail(FA_EINVAL, "paged_decode_kv8: workspace must be 256-byte aligned");
-  if (fa_status s = zero_stale_tickets(ws, w.lse_off, stream); s != FA_OK) return s;
   fa::Kv8DecodeParams p{};
   char *wsb = static_cast<char *>(ws);
-  p.tickets = reinterpret_cast<int32_t *>(wsb);
+  p.tickets = reinterpret_cast<int32_t *>(wsb + kPrefillWorkspace);
   p.piece_lse = reinterpret_cast<float *>(wsb + w.lse_off);
   p.pieces = reinterpret_cast<float *>(wsb + w.o_off);
   p.k_scale = L->k_scale;
@@ -1088,7 +1095,7 @@ Prefill8Workspace prefill8_workspace_layout(int num_seqs, int num_heads, int num
   auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
   Prefill8Workspace w{};
   const int width = std::max(1, (max_context_len + fa::kPage - 1) / fa::kPage);
-  w.q_off = kPrefillWorkspace;
+  w.q_off = kKv8Reserved;
   w.ctx_off = w.q_off + r256(size_t(128) * num_heads * head_dim * 2);
   w.tables_off = w.ctx_off + r256(size_t(num_seqs) * 4);
   w.k_off = w.tables_off + r256(size_t(num_seqs) * width * 4);
@@ -1111,9 +1118,6 @@ fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32
   if (ws_bytes < w.bytes)
     return fail(FA_ERANGE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, w.bytes);
   if (!aligned(ws, 256)) return fail(FA_EINVAL, "%s: workspace must be 256-byte aligned", who);
-  // The work counters must be zero and this call's copy lies behind them, as a decode's partials
-  // lie behind its tickets.
-  if (fa_status s = zero_stale_tickets(ws, kPrefillWorkspace, stream); s != FA_OK) return s;
   char *wsb = static_cast<char *>(ws);
   const int box = 128 / n_rep;
   const bool pad = total_q < box;

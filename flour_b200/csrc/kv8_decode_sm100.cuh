@@ -11,8 +11,10 @@
 // range through a ring of its own, across the ends of sequences, with no barrier to wait at. So
 // every SM has the same bytes to read whatever the lengths, and the latencies of a start (lengths,
 // block table, first bytes) are paid once a launch and not once a split: half the bytes of a
-// 16-bit cache leave half the time to hide them in. (The 16-bit decode's grid of splits measured
-// 63 us for 64 contexts of U[512, 4096] and 58 us for 59 of U[1, 6438]; see the figures below.)
+// 16-bit cache leave half the time to hide them in. Measured: 64 contexts of U[512, 4096], 8 KV
+// heads of 128, 60.4 us (4.95 TB/s; 63.3 with the 16-bit decode's grid of splits and this inner
+// loop); 59 of U[1, 6438], 4 KV heads, 7 query heads each, int8, 52.0 us (61.1); 16 of U[16384,
+// 32768] 148 us (5.77 TB/s of the 6.56 that a copy reaches).
 // A (sequence, KV head) that ends inside one range is written by its warp; the others leave pieces
 // (O / l, log2-sum-exp) in the workspace, which the CTA joins when its warps are done, and the last
 // CTA of a (sequence, KV head) to finish (a ticket, no waiting) joins the CTAs' pieces. The ranges
@@ -132,12 +134,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
                       int64_t(ctx) <= int64_t(p.max_blocks_per_seq) * kPage;
       n = ok ? (ctx + 2 * kPage - 1) / (2 * kPage) : 0;
       s_ctx[s] = ctx;
-      if (!ok && s % int(gridDim.x) == int(blockIdx.x)) {
-        // Nothing valid to attend to: one CTA zeroes the sequence's heads and reports.
-        report(FA_DEVERR_CONTEXT);
-        T *o = static_cast<T *>(p.out) + size_t(s) * p.num_heads * HD;
-        for (int x = 0; x < p.num_heads * HD; ++x) o[x] = Elem<T>::from_f(0.f);
-      }
     }
     int incl = n;
 #pragma unroll
@@ -164,6 +160,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   }
   if (tid == 0) offs[0] = 0;
   __syncthreads();
+  auto pairs_of = [&](int s) { return offs[s + 1] - offs[s]; };
+  for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+    if (pairs_of(s) > 0) continue;
+    // Nothing valid to attend to: one CTA zeroes the sequence's heads and reports.
+    if (tid == 0) report(FA_DEVERR_CONTEXT);
+    uint2 *o = reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + size_t(s) * p.num_heads * HD);
+    for (int x = tid; x < p.num_heads * (HD / 4); x += kDecodeThreads) o[x] = make_uint2(0u, 0u);
+  }
   // Short contexts of few (sequence, KV head) items: a CTA takes one item each, a warp a quarter of
   // its pairs, and joins it without a ticket (16 contexts of 300, 8 KV heads: 9.5 us, 13.4 in
   // ranges). The items are then laid out at a stride of four quarters of the longest, which is all
@@ -178,7 +182,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   if (c0 >= total) return;
   const int c1 = min(total, c0 + kDecodeWarps * ppw);
   const int w0 = min(total, c0 + warp * ppw);
-  auto pairs_of = [&](int s) { return offs[s + 1] - offs[s]; };
   const int end = by_item ? c0 + pairs_of(int(blockIdx.x) / H) : total;  // of this CTA's pairs
   const int n_my = max(0, min(end, w0 + ppw) - w0);
 

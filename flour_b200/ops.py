@@ -131,11 +131,20 @@ def workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: i
 
 class Workspace:
     """Caller-owned, zero-initialised scratch for the split-K partials (grown on demand).
-    One Workspace per stream: concurrent calls must not share it."""
+    One Workspace per stream: concurrent calls must not share it. The 8-bit entry points (kv8)
+    keep a Workspace of their own, apart from the others'."""
 
     def __init__(self, device=None):
         self.device = torch.device(device if device is not None else "cuda")
         self.buf: torch.Tensor | None = None
+        self.kv8: bool | None = None  # which entry points use it, from the first call that needs it
+
+    def claim(self, kv8: bool) -> None:
+        if self.kv8 is None:
+            self.kv8 = kv8
+        elif self.kv8 is not kv8:
+            raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                      "8-bit and 16/32-bit calls need workspaces of their own")
 
     def get(self, nbytes: int) -> torch.Tensor | None:
         if nbytes == 0:
@@ -153,6 +162,7 @@ def _ws_args(ws: Workspace | None, need: int):
         return None, 0
     if ws is None:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"a workspace of {need} bytes is required")
+    ws.claim(False)
     buf = ws.get(need)
     return _ptr(buf), buf.numel()
 
@@ -491,8 +501,11 @@ def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_table
 
 
 def _ws8(workspace: Workspace | None, need: int, dev: int):
-    if workspace is None or not need:
-        return _ws_args(workspace, need)
+    if not need:
+        return None, 0
+    if workspace is None:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"a workspace of {need} bytes is required")
+    workspace.claim(True)
     if torch._C._cuda_getDevice() == dev:
         buf = workspace.get(need)
     else:

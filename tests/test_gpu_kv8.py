@@ -433,6 +433,50 @@ def test_one_workspace_two_graphs_and_other_calls(device):
     assert ops.device_status() == 0
 
 
+def test_graphs_of_any_sizes_share_a_workspace(device):
+    # Captured largest first: many tickets, then few, then a prefill's copy; replayed in all orders.
+    from itertools import permutations
+    ws = ops.Workspace()
+    ws.get(96 << 20)
+    cases, graphs = [], []
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    for Hq, Hkv, ctx, seed in ((32, 8, [700] * 100, 50), (8, 2, [5000, 3000], 51)):
+        pool, q, bt, cl, want, tol = decode_case(device, torch.int8, torch.bfloat16, Hq, Hkv, 128, ctx, seed)
+        ref = run_decode(pool, q, bt, cl, ctx, Hkv)
+        assert_close(ref, want, tol)
+        out, g = torch.empty_like(q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            run_decode(pool, q, bt, cl, ctx, Hkv, ws, out=out)
+        cases.append((out, ref, pool, q, bt, cl))
+        graphs.append(g)
+    _, _, pool, _, bt, cl = cases[1]
+    qp = torch.randn((90, 8, 128), device=device, generator=gen_of(device, 52)).to(torch.bfloat16)
+    args = (qp, *pool, i32([0, 50, 90], device), cl, bt, 4, inv_sqrt(128), 50, 5000, 501)
+    ref = ops.paged_prefill_kv8(*args, ops.Workspace())
+    out, g = torch.empty_like(qp), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        ops.paged_prefill_kv8(*args, ws, out=out)
+    cases.append((out, ref))
+    graphs.append(g)
+    for order in permutations(range(3)):
+        for i in order:
+            cases[i][0].zero_()
+            graphs[i].replay()
+            assert torch.equal(cases[i][0], cases[i][1]), (order, i)
+    del graphs, g
+    assert ops.device_status() == 0
+
+
+def test_a_16_bit_workspace_is_refused(device):
+    pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, [40, 5000], 53)
+    ws = ops.Workspace()
+    kc = torch.zeros(pool[0].shape, dtype=torch.bfloat16, device=device)
+    ops.paged_decode(q, kc, kc, bt, cl, 4, 0.1, 5000, ws)
+    with pytest.raises(FlourAttnError):
+        ops.paged_decode_kv8(q, *pool, bt, cl, 4, 0.1, 5000, ws)
+
+
 def test_side_stream_and_append_then_decode_chain(device):
     # One step as a server runs it: prompts appended and attended, then 20 tokens one by one,
     # all on a side stream, against the plain forms on the same codes.
@@ -564,6 +608,52 @@ def test_offsets_past_32_bits(device):
     last = q[[59, 134]].contiguous()
     assert torch.equal(run_decode(big, last, i32(bt, device), i32(ctx, device), ctx, H),
                        run_decode(pool, last, i32(bt_small, device), i32(ctx, device), ctx, H))
+    assert ops.device_status() == 0
+
+
+def test_a_layer_from_activations_to_answers(device):
+    # qkv_rope_cache into a staging layer of one block, append, attention, o_proj, logits and their
+    # log probabilities: a prompt and then a decode step, as the integration notes describe.
+    from flour_b200.paged import rope_tables
+    H, Hq, d, hidden, V = 2, 8, 128, 256, 1024
+    g = gen_of(device, 54)
+    rnd = lambda *s: torch.randn(s, device=device, generator=g)  # noqa: E731
+    w = (rnd((Hq + 2 * H) * d, hidden) / 16).to(torch.bfloat16)
+    wo, head = (rnd(hidden, Hq * d) / 32).to(torch.bfloat16), rnd(V, hidden).to(torch.bfloat16)
+    cos, sin = rope_tables(d, 64, 10000.0, torch.bfloat16, device)
+    lens = [21, 40]
+    bt, nb = make_tables([c + 1 for c in lens], 16, 54)
+    pool = random_pool(nb, H, 16, d, torch.float8_e4m3fn, g, device)
+    ws = ops.Workspace()
+    for step in range(2):
+        new = lens if step == 0 else [1, 1]
+        ctx = [c + step for c in lens]
+        n = sum(new)
+        x = rnd(n, hidden).to(torch.bfloat16)
+        pos = i32(np.concatenate([np.arange(c - k, c) for c, k in zip(ctx, new)]), device)
+        kst, vst = (torch.zeros((1, H, n, d), device=device, dtype=torch.bfloat16) for _ in "kv")
+        q = ops.qkv_rope_cache(x, w, kst, vst, pos, torch.arange(n, dtype=torch.int32, device=device), Hq, cos, sin)
+        key, value = kst[0].transpose(0, 1), vst[0].transpose(0, 1)
+        before = clone(pool)
+        run_append(pool, key, value, bt, ctx, new, device, one=step == 1)
+        check_append(pool, before, key, value, bt, ctx, new)
+        if step == 0:
+            out = run_prefill(pool, q, bt, ctx, new, H, device, ws=ws)
+        else:
+            out = run_decode(pool, q, i32(bt, device), i32(ctx, device), ctx, H, ws)
+        want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, 4,
+                                  inv_sqrt(d), 2.0 ** -8 if step == 0 else U16)
+        assert_close(out, want, tol)
+        y = ops.o_proj_residual(out.reshape(n, -1), wo, x)
+        logits = ops.last_token_logits(y, i32(np.concatenate([[0], np.cumsum(new)]), device), head)
+        picked = logits.argmax(1).to(torch.int32)
+        lp, ent, ids, top = ops.token_logprobs(logits, picked, 4)
+        ref = torch.log_softmax(logits.double(), 1)
+        # f32 results: 2^-24 for the subtraction of the maximum and of ln Z, sums to 2.4e-6 (see
+        # test_gpu_logprobs), the entropy twice that times ln V + 2.
+        assert (lp - ref.max(1).values).abs().max() < 1e-5 * logits.abs().max()
+        assert torch.equal(ids[:, 0], picked) and torch.equal(top[:, 0], lp)
+        assert (ent - -(ref.exp() * ref).sum(1)).abs().max() < 1e-4
     assert ops.device_status() == 0
 
 

@@ -120,6 +120,16 @@ def test_logprobs_refusals():
     assert call(R=0) == _lib.FA_OK
 
 
+def test_a_workspace_serves_8_bit_calls_or_the_others():
+    ws = ops.Workspace()
+    ws.claim(True)
+    ws.claim(True)
+    with pytest.raises(FlourAttnError):
+        ws.claim(False)
+    with pytest.raises(FlourAttnError):
+        ops._ws_args(ws, 256)
+
+
 def test_cpu_tensors_are_refused():
     kc = torch.zeros((4, 2, 16, 64), dtype=torch.int8)
     sc = torch.ones((4, 2))
