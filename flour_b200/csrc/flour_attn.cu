@@ -1019,18 +1019,24 @@ fa_status launch_generic8(const fa_kv8_layer *L, const void *q, void *out, int32
 // ---- log probabilities ------------------------------------------------------------------------
 
 constexpr int kLpPartTile = fa::kLpPartThreads * fa::kLpPartLogits;
-constexpr int kLpPartCtasPerSm = 2;
 constexpr int kLpSmallTile = fa::kLpSmallThreads * fa::kLpPartLogits;
 
 template <typename T>
 fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t stream, const char *who) {
   // 15 more logits: a row that does not start on 16 bytes fills its first vector partly.
   const int64_t span = int64_t(p.vocab) + 15;
+  // A vocabulary that 128 threads hold: 16 rows per SM at once (4096 x 1000 bf16: 18.6 us, 55.6 with
+  // 512 threads a row).
   if (span <= kLpSmallTile)
     return launch_pdl(who, fa::logprobs_part_kernel<T, fa::kLpSmallThreads>, dim3(unsigned(rows)),
                       fa::kLpSmallThreads, 0, stream, 1, p);
   const int64_t ranks = (span + kLpPartTile - 1) / kLpPartTile;
-  if (ranks <= fa::kLpMaxCluster && rows * ranks <= kLpPartCtasPerSm * int64_t(sm_count())) {
+  // Two CTAs of the part kernel fit an SM. One CTA a row stays ahead of streaming for eight a
+  // SM (10000 logits, bf16, 20 alternatives: 600 rows 17.8 us against 19.9, 2000 rows 49.4 against
+  // 48.7); clusters do for two and a half (128256 logits: 48 rows 14.6 against 16.5, 64 rows 17.8
+  // against 17.1, 148 rows 35.6 against 29.3).
+  const int64_t ctas = rows * ranks, sms = sm_count();
+  if (ranks <= fa::kLpMaxCluster && (ranks == 1 ? ctas <= 8 * sms : 2 * ctas <= 5 * sms)) {
     auto kern = fa::logprobs_part_kernel<T, fa::kLpPartThreads>;
     if (ranks > 8) {
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -1038,7 +1044,10 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     }
     return launch_pdl(who, kern, dim3(unsigned(rows * ranks)), fa::kLpPartThreads, 0, stream, int(ranks), p);
   }
-  int split = 1;  // few rows too long for registers
+  // Otherwise a CTA a row, or as many as are resident at once (four per SM): 256 rows of 128256 in
+  // two CTAs each take 32.5 us; past one wave a split only adds cluster launches (2048 x 151643:
+  // 135 us, 180 in two CTAs each).
+  int split = 1;
   while (split < 8 && int64_t(rows) * split * 2 <= int64_t(sm_count()) * 4) split *= 2;
   return launch_pdl(who, fa::logprobs_stream_kernel<T>, dim3(unsigned(rows * split)), fa::kLpStreamThreads, 0,
                     stream, split, p);
