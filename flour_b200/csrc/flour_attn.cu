@@ -1044,13 +1044,21 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     }
     return launch_pdl(who, kern, dim3(unsigned(rows * ranks)), fa::kLpPartThreads, 0, stream, int(ranks), p);
   }
-  // Otherwise a CTA a row, or as many as are resident at once (four per SM): 256 rows of 128256 in
-  // two CTAs each take 32.5 us; past one wave a split only adds cluster launches (2048 x 151643:
-  // 135 us, 180 in two CTAs each).
-  int split = 1;
-  while (split < 8 && int64_t(rows) * split * 2 <= int64_t(sm_count()) * 4) split *= 2;
-  return launch_pdl(who, fa::logprobs_stream_kernel<T>, dim3(unsigned(rows * split)), fa::kLpStreamThreads, 0,
-                    stream, split, p);
+  // Streaming: the most threads a row that still leave all rows resident at once, one CTA a row
+  // (128256 f32 logits, 20 alternatives, 256 / 512 / 1024 threads: 148 rows 31.9 / 22.9 / 20.9 us,
+  // 296 rows 37.5 / 33.2 / 40.4, 592 rows 56.5 / 62.3 / 78.1). Clusters of smaller CTAs cost more to
+  // launch than they balance (64 rows in eight CTAs of 256 threads each 19.3 us, two of 1024 16.7;
+  // 592 rows in two of 256 69.3), so a row is cut only where fewer than half the SMs have one.
+  auto stream_in = [&](auto kern, int threads, int split) {
+    return launch_pdl(who, kern, dim3(unsigned(rows * split)), threads, 0, stream, split, p);
+  };
+  if (rows <= sms) {
+    int split = 1;
+    while (split < 8 && int64_t(rows) * split * 2 <= sms) split *= 2;
+    return stream_in(fa::logprobs_stream_kernel<T, 1024>, 1024, split);
+  }
+  if (rows <= 2 * sms) return stream_in(fa::logprobs_stream_kernel<T, 512>, 512, 1);
+  return stream_in(fa::logprobs_stream_kernel<T, 256>, 256, 1);
 }
 
 // Whether the tcgen05 prefill serves a call, over a copy of the cache in the query type.

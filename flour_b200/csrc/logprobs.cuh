@@ -31,7 +31,6 @@ constexpr int kLpMaxCluster = 16;    // 16 CTAs a cluster is opt-in; 8 without
 constexpr int kLpPartLogits = 32;    // a thread's logits in the part kernel
 constexpr int kLpPartThreads = 512;
 constexpr int kLpSmallThreads = 128; // vocabularies that fit one CTA of this size
-constexpr int kLpStreamThreads = 256;
 
 struct LogprobParams {
   const void *logits;        // row r at r * row_stride elements
@@ -377,7 +376,7 @@ struct LpList {
 
 // The CTA's candidates: keys of the logits that passed the bound when their tile was read. One
 // that comes when the pool is full is counted only, and the row's part is read again with lists.
-constexpr int kLpPool = 1024;
+constexpr int kLpPool = 2048;
 struct LpPool {
   uint64_t key[kLpPool];
   int n;
@@ -579,10 +578,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
 
 // A part once more, with a list a warp (the pool was too small). Out of line: its registers are not
 // the streaming loop's.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, float bound, uint64_t *cand,
                                            int K) {
-  constexpr int THREADS = kLpStreamThreads, NV = 4;
+  constexpr int NV = 4;
   const int tid = threadIdx.x;
   LpList list;
   list.cand = cand;
@@ -600,16 +599,15 @@ __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, flo
 }
 
 // ---- stream kernel ------------------------------------------------------------------------------
-// Tiles of 64 bytes a thread, the next one in flight. The 32 groups of the CTA (eight lanes each)
-// keep their running maxima in shared memory, and the warps take a new bound from them after tiles
+// Tiles of 64 bytes a thread, the next one in flight. The 32 groups of the CTA (THREADS / 32 lanes
+// each) keep their running maxima in shared memory, and the warps take a new bound from them after tiles
 // 1, 2, 4, 8, ...: without a barrier but the first, for maxima that a warp sees too early are still
 // a lower bound. About 32 ln(32 / (32 - k)) logits pass in each doubling. Where more than the pool
 // holds pass (ascending rows, many equal logits) the part is read a second time, with a list a warp.
-template <typename T>
-__global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(const LogprobParams p) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_stream_kernel(const LogprobParams p) {
   using Row = LpRow<T>;
-  constexpr int NV = 4;
-  constexpr int THREADS = kLpStreamThreads, WARPS = THREADS / 32;
+  constexpr int NV = 4, WARPS = THREADS / 32, GROUP = THREADS / 32;  // 32 groups
   __shared__ LpState s_state[WARPS];
   __shared__ volatile float s_max[32];
   __shared__ LpPool s_pool;
@@ -645,8 +643,8 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
       if ((tile & (tile + 1)) == 0) {
         float m = st.m;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane % 8 == 0) s_max[tid / 8] = m;
+        for (int o = 1; o < GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane % GROUP == 0) s_max[tid / GROUP] = m;
         if (tile == 0) __syncthreads();
         __syncwarp();
         bound = fmaxf(bound, __shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
@@ -661,7 +659,7 @@ __global__ void __launch_bounds__(kLpStreamThreads, 4) logprobs_stream_kernel(co
   const int n = s_pool.n;
   uint64_t top = 0;
   if (n > kLpPool) {
-    s_top[warp][lane] = lp_reread<T>(r, v0, v1, bound, s_pool.key + warp * 64, K);
+    s_top[warp][lane] = lp_reread<T, THREADS>(r, v0, v1, bound, s_pool.key + warp * 64, K);
     __syncthreads();
     if (warp == 0)
       for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);

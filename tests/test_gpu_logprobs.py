@@ -68,7 +68,7 @@ def logits(R, V, dtype, device, seed, scale=3.0, pad=0, shift=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("R, V, k", [(1, 1, 1), (2, 7, 5), (3, 31, 32), (5, 257, 20), (1, 8191, 1), (4, 8193, 20),
-                                     (1, 151936, 20), (9, 50257, 5), (64, 128256, 20), (700, 1003, 0),
+                                     (1, 151936, 20), (9, 50257, 5), (64, 128256, 20), (700, 1003, 0), (100, 40009, 20), (1, 300001, 32), (250, 33001, 5), (400, 21000, 20),
                                      (1200, 2049, 8)])
 def test_sizes(device, dtype, R, V, k):
     x = logits(R, V, dtype, device, R + V)
@@ -94,7 +94,7 @@ def test_neighbours_of_a_row_do_not_leak(device):
         check(flat[None, off + 10000:off + 10000 + 4999], [17], 10)
 
 
-@pytest.mark.parametrize("R", [1, 40, 400])
+@pytest.mark.parametrize("R", [1, 40, 120, 400])
 def test_ties_go_to_the_lowest_id(device, R):
     V = 40000
     check(torch.zeros((R, V), device=device), [V - 1] * R, 20)                       # all equal
