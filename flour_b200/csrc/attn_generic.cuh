@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
     }
     s = lo;
     const int q0 = p.cu_seqlens_q[s], q1 = p.cu_seqlens_q[s + 1];
+    if (k8 && s == p.num_seqs - 1 && q0 >= 0 && q0 <= q1 && q1 <= qi) return;  // behind the last sequence
     if (q0 > qi || q1 <= qi || q1 > p.total_q) {
       if (tid == 0) report(FA_DEVERR_SEQLEN);
       for (int x = tid; x < D; x += kGenericThreads) out[orow + x] = Elem<T>::from_f(0.f);

@@ -932,9 +932,10 @@ Decode8Workspace decode8_workspace_layout(int num_heads, int num_kv_heads, int h
   return w;
 }
 
-fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *ctx,
-                         const int32_t *tables, int max_blocks, int num_seqs, int num_heads, int n_rep,
-                         int max_context_len, float scale, void *ws, size_t ws_bytes, cudaStream_t stream) {
+fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_t dtype, const int32_t *cu,
+                         const int32_t *ctx, const int32_t *tables, int max_blocks, int num_seqs,
+                         int num_heads, int n_rep, int max_context_len, float scale, void *ws, size_t ws_bytes,
+                         cudaStream_t stream) {
   const Decode8Plan plan = plan_decode8(num_seqs, L->num_kv_heads, max_context_len);
   const Decode8Workspace w = decode8_workspace_layout(num_heads, L->num_kv_heads, L->head_dim, plan);
   if (!ws) return fail(FA_EINVAL, "paged_decode_kv8: workspace is NULL but %zu bytes are needed", w.bytes);
@@ -962,8 +963,10 @@ fa_status launch_decode8(const fa_kv8_layer *L, const void *q, void *out, int32_
   const size_t row_bytes = size_t(num_heads) * L->head_dim * 2;
   for (int s0 = 0; s0 < num_seqs; s0 += plan.seqs) {
     p.num_seqs = std::min(plan.seqs, num_seqs - s0);
-    p.q = static_cast<const char *>(q) + s0 * row_bytes;
-    p.out = static_cast<char *>(out) + s0 * row_bytes;
+    p.q = static_cast<const char *>(q) + (cu ? 0 : s0 * row_bytes);
+    p.out = static_cast<char *>(out) + (cu ? 0 : s0 * row_bytes);
+    p.cu_seqlens_q = cu ? cu + s0 : nullptr;
+    p.total_q = num_seqs;
     p.context_lens = ctx + s0;
     p.block_tables = tables + size_t(s0) * max_blocks;
     const fa_status st = with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
@@ -1772,7 +1775,7 @@ fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *query, void
   if (num_seqs > 65535) return fail(FA_EUNSUPPORTED, "%s: more than 65535 sequences per call", who);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (decode8_fast_path(layer, n_rep, dtype, query, out))
-    return launch_decode8(layer, query, out, dtype, context_lens, block_tables, max_blocks_per_seq,
+    return launch_decode8(layer, query, out, dtype, nullptr, context_lens, block_tables, max_blocks_per_seq,
                           num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
                           workspace_bytes, st);
   return launch_generic8(layer, query, out, dtype, nullptr, context_lens, block_tables, max_blocks_per_seq,
@@ -1815,12 +1818,13 @@ fa_status fa_paged_prefill_kv8(const fa_kv8_layer *layer, const void *query, voi
   if (max_seqlen_q > max_context_len)
     return fail(FA_ERANGE, "%s: max_seqlen_q %d > max_context_len %d", who, max_seqlen_q, max_context_len);
   if (total_q == 0 || num_seqs == 0) return ok();
-  if (max_seqlen_q == 1 && total_q == num_seqs)  // one new token each
-    return fa_paged_decode_kv8(layer, query, out, dtype, context_lens, block_tables, max_blocks_per_seq,
-                               num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
-                               workspace_bytes, stream);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (prefill8_fast_path(layer, n_rep, dtype, scale, query, out, num_seqs, total_blocks))
+  const bool single = max_seqlen_q == 1 && total_q == num_seqs;  // at most one new token each
+  if (single && decode8_fast_path(layer, n_rep, dtype, query, out))
+    return launch_decode8(layer, query, out, dtype, cu_seqlens_q, context_lens, block_tables,
+                          max_blocks_per_seq, num_seqs, num_heads, n_rep, max_context_len, scale, workspace,
+                          workspace_bytes, st);
+  if (!single && prefill8_fast_path(layer, n_rep, dtype, scale, query, out, num_seqs, total_blocks))
     return launch_prefill8(layer, query, out, dtype, cu_seqlens_q, context_lens, block_tables,
                            max_blocks_per_seq, num_seqs, num_heads, n_rep, total_q, max_context_len,
                            total_blocks, scale, workspace, workspace_bytes, st);

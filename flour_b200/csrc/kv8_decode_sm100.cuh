@@ -32,7 +32,8 @@
 // length), and the factor returns with the score's scale. P is rounded to f16, which loses 8 times
 // less than the bf16 of the 16-bit decode. The scale of K multiplies a score in f32; the larger of
 // the pair's two scales of V multiplies its product in f32, and the other page's probabilities take
-// the ratio (a power of two for scales of the append, and then exact).
+// the ratio (a power of two for scales of the append, and then exact). Probabilities are rounded at
+// 2^12 times their size, so that the ratio does not push them among f16's subnormals.
 #pragma once
 
 #include "decode_sm100.cuh"
@@ -53,6 +54,8 @@ constexpr int kKv8Pieces = 10;     // of a CTA in the workspace: 4 warps x (firs
 struct Kv8DecodeParams {
   const void *q;                 // [num_seqs, num_heads, HD]
   void *out;
+  const int32_t *cu_seqlens_q;   // given: sequence s's token is row cu[s] of total_q, if it has one
+  int32_t total_q;
   const int32_t *context_lens;
   const int32_t *block_tables;
   const float *k_scale;          // [num_blocks, num_kv_heads]
@@ -127,6 +130,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   }
   pdl_wait();
 
+  auto has_token = [&](int s) {
+    if (!p.cu_seqlens_q) return true;
+    const int row = p.cu_seqlens_q[s];
+    return row >= 0 && row < p.total_q && p.cu_seqlens_q[s + 1] == row + 1;
+  };
+  auto token_of = [&](int s) { return p.cu_seqlens_q ? p.cu_seqlens_q[s] : s; };
+
   // ---- prefix sums of the sequences' pairs; 128 sequences a turn ------------------------------
   int longest = 0;
   for (int s0 = 0, carry = 0; s0 < p.num_seqs; s0 += kDecodeThreads) {
@@ -135,7 +145,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     if (s < p.num_seqs) {
       const int ctx = p.context_lens[s];
       const bool ok = ctx >= 1 && ctx <= p.max_context_len &&
-                      int64_t(ctx) <= int64_t(p.max_blocks_per_seq) * kPage;
+                      int64_t(ctx) <= int64_t(p.max_blocks_per_seq) * kPage && has_token(s);
       n = ok ? (ctx + 2 * kPage - 1) / (2 * kPage) : 0;
       s_ctx[s] = ctx;
     }
@@ -167,9 +177,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
   auto pairs_of = [&](int s) { return offs[s + 1] - offs[s]; };
   for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
     if (pairs_of(s) > 0) continue;
+    if (!has_token(s)) {  // no row of its own: fine when it has no token, an error otherwise
+      if (tid == 0 && p.cu_seqlens_q[s + 1] != p.cu_seqlens_q[s]) report(FA_DEVERR_SEQLEN);
+      continue;
+    }
     // Nothing valid to attend to: one CTA zeroes the sequence's heads and reports.
     if (tid == 0) report(FA_DEVERR_CONTEXT);
-    uint2 *o = reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + size_t(s) * p.num_heads * HD);
+    uint2 *o = reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + size_t(token_of(s)) * p.num_heads * HD);
     for (int x = tid; x < p.num_heads * (HD / 4); x += kDecodeThreads) o[x] = make_uint2(0u, 0u);
   }
   // Short contexts of few (sequence, KV head) items: a CTA takes one item each, a warp a quarter of
@@ -279,7 +293,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     uint32_t qb[CH][2];
     float f0, f1;  // score factors of heads 2t, 2t+1
     {
-      const T *qrow = static_cast<const T *>(p.q) + (size_t(pr.s) * p.num_heads + hq0 + g) * HD;
+      const T *qrow = static_cast<const T *>(p.q) + (size_t(token_of(pr.s)) * p.num_heads + hq0 + g) * HD;
       uint2 raw[CH];
       float amax = 0.f;
 #pragma unroll
@@ -308,8 +322,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     Pair next{};
     if (i + seg < n_my) {  // the next segment's queries, on their way while this one is worked on
       next = find(w0 + i + seg);
-      const char *at = reinterpret_cast<const char *>(static_cast<const T *>(p.q) +
-                                                      (size_t(next.s) * p.num_heads + next.kvh * n_rep) * HD);
+      const char *at = reinterpret_cast<const char *>(
+          static_cast<const T *>(p.q) + (size_t(token_of(next.s)) * p.num_heads + next.kvh * n_rep) * HD);
       if (lane * 128 < n_rep * HD * 2) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + lane * 128));
     }
     float m0 = neg_inf(), m1 = neg_inf(), l0 = 0.f, l1 = 0.f;  // heads 2t, 2t+1
@@ -410,8 +424,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
       l1 += (ca[1] + ca[3]) + (cb[1] + cb[3]);
       const float vs0 = w.vs[0][e32], vs1 = w.vs[1][e32];
       const float vs = fmaxf(vs0, vs1);
-      const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.2e-38f;
-      const float inv = vs > 0.f ? 1.f / vs : 0.f;  // both scales 0: nothing to add
+      const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.e-34f;
+      const float inv = vs > 0.f ? 4096.f / vs : 0.f;  // both scales 0: nothing to add
       const float ra = apart ? 1.f : vs0 * inv, rb = apart ? 0.f : vs1 * inv;
       const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0] * ra, ca[1] * ra));
       const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2] * ra, ca[3] * ra));
@@ -444,7 +458,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
         }
       };
       if (!apart) {
-        values(pa0, pa1, pb0, pb1, vs);
+        values(pa0, pa1, pb0, pb1, vs * (1.f / 4096.f));
       } else {  // more than a factor 64 between the pages: one after the other
 #pragma unroll 1
         for (int x = 0; x < 2; ++x) {
@@ -465,7 +479,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
     }
     const float i0 = 1.f / l0, i1 = 1.f / l1;
     if (seg == pr.of) {
-      T *out = static_cast<T *>(p.out) + (size_t(pr.s) * p.num_heads + hq0) * HD + 2 * g;
+      T *out = static_cast<T *>(p.out) + (size_t(token_of(pr.s)) * p.num_heads + hq0) * HD + 2 * g;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (2 * t < n_rep)
@@ -547,7 +561,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
         *reinterpret_cast<float4 *>(dst + h * HD + d) = make_float4(O.x * i, O.y * i, O.z * i, O.w * i);
         if (d == 0) dst_lse[h] = M + __log2f(W);
       } else {
-        T *out = static_cast<T *>(p.out) + (size_t(item / H) * p.num_heads + (item % H) * n_rep + h) * HD + d;
+        T *out = static_cast<T *>(p.out) +
+                 (size_t(token_of(item / H)) * p.num_heads + (item % H) * n_rep + h) * HD + d;
         *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
       }
     }

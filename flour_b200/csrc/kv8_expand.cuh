@@ -7,13 +7,24 @@
 // budget (96 a thread at 18 warps) has no room.
 //
 // byte * scale is exact in bf16 for the append's power-of-two scales; in f16 it is exact above
-// f16's subnormals. Rows behind the last token are written as zeros: NaN bytes that an earlier
+// f16's subnormals, and what is larger than f16's largest becomes that: the codes of 65504 itself
+// stand for 65536, whose infinity would make NaN of a finite row. Rows behind the last token are written as zeros: NaN bytes that an earlier
 // owner left there would survive a probability of 0.
 #pragma once
 
 #include "kv8_common.cuh"
 
 namespace fa {
+
+template <typename T> __device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 top = __half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
+    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), top), __hneg2(top));
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    return pack2<T>(a, b);
+  }
+}
 
 struct Kv8ExpandParams {
   const uint8_t *cache[2];       // [num_blocks, num_kv_heads, block_size, head_dim]
@@ -128,10 +139,10 @@ __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Kv8Exp
           if (i >= live) f[0] = f[1] = f[2] = f[3] = make_float2(0.f, 0.f);
           if constexpr (sizeof(T) == 2) {
             uint4 v;
-            v.x = pack2<T>(f[0].x * sc, f[0].y * sc);
-            v.y = pack2<T>(f[1].x * sc, f[1].y * sc);
-            v.z = pack2<T>(f[2].x * sc, f[2].y * sc);
-            v.w = pack2<T>(f[3].x * sc, f[3].y * sc);
+            v.x = pack2_sat<T>(f[0].x * sc, f[0].y * sc);
+            v.y = pack2_sat<T>(f[1].x * sc, f[1].y * sc);
+            v.z = pack2_sat<T>(f[2].x * sc, f[2].y * sc);
+            v.w = pack2_sat<T>(f[3].x * sc, f[3].y * sc);
             *reinterpret_cast<uint4 *>(out + i) = v;
           } else {
             float4 *o4 = reinterpret_cast<float4 *>(out + i);

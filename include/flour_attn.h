@@ -328,9 +328,10 @@ typedef struct fa_kv8_layer {
  * Infinities saturate; NaN is stored as e4m3's NaN or int8's 0; either sets FA_DEVERR_VALUE and
  * leaves the scale to the finite values.
  * A block that receives tokens must appear once, in one sequence's table (a shared prefix block is
- * copied before it is written): where it does not, its bytes are those of any of the writers. Rows of key/value behind cu_seqlens_q[num_seqs] are not read. A
- * sequence with bad lengths (FA_DEVERR_CONTEXT / FA_DEVERR_SEQLEN) or block ids
- * (FA_DEVERR_BLOCK_ID) is not written there. No workspace. */
+ * copied before it is written): where it does not, its bytes are those of any of the writers.
+ * Rows of key/value behind cu_seqlens_q[num_seqs] are not read. A sequence with bad lengths
+ * (FA_DEVERR_CONTEXT / FA_DEVERR_SEQLEN) or block ids (FA_DEVERR_BLOCK_ID) is not written there.
+ * No workspace. */
 FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key, const void *value,
                                      int32_t dtype, int64_t key_stride_token, int64_t key_stride_head,
                                      int64_t value_stride_token, int64_t value_stride_head,
@@ -368,9 +369,12 @@ FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *quer
  * has too few query rows for the SMs, contexts are cut into parts whose results (f32, in the
  * workspace) one more launch joins. Sequences that no
  * longer fit total_blocks give zeros and FA_DEVERR_CONTEXT. Other shapes, and total_blocks 0, run
- * the generic kernel, which needs no workspace. One new token per sequence (max_seqlen_q 1,
- * total_q == num_seqs) is fa_paged_decode_kv8. Output rows behind cu_seqlens_q[num_seqs] are not
- * written by the tensor-core path. */
+ * the generic kernel, which needs no workspace. At most one new token per sequence (max_seqlen_q
+ * 1, total_q == num_seqs) runs the decode's kernel; a sequence with more is then FA_DEVERR_SEQLEN
+ * and not written. Output rows behind cu_seqlens_q[num_seqs] are not written. The copy holds
+ * f16's range for FA_F16 queries: magnitudes above 65504 become 65504, and below 2^-14 they are
+ * rounded to steps of 2^-24 (the decode takes any f32 value of byte * scale). A NaN among the keys
+ * and values of a sequence may reach all of its queries. */
 FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
                                                   int32_t num_kv_heads, int32_t block_size,
                                                   int32_t head_dim, int32_t total_q,
@@ -486,7 +490,8 @@ FA_API int32_t fa_gemm_tile_width(int32_t M, int32_t N, int32_t K);
  * first weight tiles while the preceding kernel on the stream finishes, and waits for that
  * kernel's completion before it reads activations or writes outputs. So are the decode kernels,
  * fa_tp_sync, fa_reshape_and_cache, fa_paged_prefill, the 8-bit cache's entry points and
- * fa_token_logprobs, which set up only on-chip state before that wait. For a caller this changes nothing: stream order holds for every call. */
+ * fa_token_logprobs, which set up only on-chip state before that wait. For a caller this changes
+ * nothing: stream order holds for every call. */
 
 /* ---- head-sharded decode (tensor parallel over KV heads, one process per GPU) ----------
  * The reference runs attention on one CPU and has no sharding (its plan shards sequences,

@@ -229,6 +229,25 @@ def test_decode_scales_that_differ_from_page_to_page(device):
     assert_close(run_decode(pool, q, bt, cl, ctx, 2), want, tol)
 
 
+@pytest.mark.parametrize("first, second", [(2.0 ** -12, 2.0 ** -6), (2.0 ** -6, 2.0 ** -12), (0.02, 0.0007),
+                                           (1e-33, 1e-34), (3e-35, 2e-35)])
+def test_decode_small_probabilities_of_a_quiet_page(device, first, second):
+    # Two pages of one step, the scales of V up to 64 apart, and probabilities of all sizes: those
+    # of the quiet page must keep their bits.
+    ctx = [17 + s % 16 for s in range(60)]
+    pool, q, bt, cl, _, _ = decode_case(device, torch.float8_e4m3fn, torch.float16, 8, 2, 128, ctx, 46,
+                                        q_scale=3.0)
+    pool[3][bt[:, 0].long()] = first
+    pool[3][bt[:, 1].long()] = second
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, bt, ctx, [1] * 60, 4, inv_sqrt(128), U16)
+    out = run_decode(pool, q, bt, cl, ctx, 2)
+    assert_close(out, want, tol)
+    out = run_decode(pool, q.to(torch.bfloat16), bt, cl, ctx, 2)
+    want, tol = attention_ref(q.to(torch.bfloat16).double().cpu().numpy(), pool, bt, ctx, [1] * 60, 4,
+                              inv_sqrt(128), U16)
+    assert_close(out, want, tol)
+
+
 @pytest.mark.parametrize("q_scale", [2.0 ** -60, 2.0 ** 40, 0.0])
 def test_decode_queries_outside_f16(device, q_scale):
     ctx = [100]
@@ -380,6 +399,74 @@ def test_prefill_rows_behind_the_last_sequence_stay(device):
     want, tol = attention_ref(q[:160].double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, ctx, 4,
                               inv_sqrt(128), 2.0 ** -8)
     assert_close(out[:160], want, tol)
+
+
+@pytest.mark.parametrize("Hq, Hkv, d, dtype, S, hi", [
+    (8, 2, 128, torch.bfloat16, 9, 300), (14, 2, 64, torch.float16, 900, 40), (4, 2, 40, torch.float32, 9, 60)])
+def test_prefill_of_at_most_one_token_each(device, Hq, Hkv, d, dtype, S, hi):
+    # Every third sequence has no new token (some of those no context either), so a row's number is
+    # not its sequence's; the batch is padded to one row per sequence.
+    rng = np.random.default_rng(35)
+    ctx = rng.integers(1, hi, S).tolist()
+    new = [0 if s % 3 == 0 else 1 for s in range(S)]
+    ctx[3] = 0
+    bt, nb = make_tables(ctx, 16, 35)
+    g = gen_of(device, 35)
+    pool = random_pool(nb, Hkv, 16, d, torch.float8_e4m3fn, g, device)
+    q = torch.randn((S, Hq, d), device=device, generator=g).to(dtype)
+    rows = sum(new)
+    q[rows:] = math.nan
+    out = torch.full_like(q, 7.0)
+    ops.device_status()
+    cu = i32(np.concatenate([[0], np.cumsum(new)]), device)
+    ops.paged_prefill_kv8(q, *pool, cu, i32(ctx, device), i32(bt, device), Hq // Hkv, inv_sqrt(d), 1, max(ctx),
+                          nb, ops.Workspace(), out)
+    assert ops.device_status() == 0
+    ctx[3] = 1  # no row of it is compared
+    want, tol = attention_ref(q[:rows].double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, Hq // Hkv,
+                              inv_sqrt(d), 0.0 if dtype == torch.float32 else U16)
+    assert_close(out[:rows], want, tol)
+    assert (out[rows:] == 7.0).all()
+
+
+def test_prefill_of_one_token_each_reports_more(device):
+    ctx = [40, 50, 60]
+    bt, nb = make_tables(ctx, 16, 36)
+    g = gen_of(device, 36)
+    pool = random_pool(nb, 2, 16, 128, torch.int8, g, device)
+    q = torch.randn((3, 8, 128), device=device, generator=g).to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    ops.device_status()
+    ops.paged_prefill_kv8(q, *pool, i32([0, 2, 2, 3], device), i32(ctx, device), i32(bt, device), 4, inv_sqrt(128),
+                          1, 60, nb, ops.Workspace(), out)
+    assert ops.device_status() == _lib.FA_DEVERR_SEQLEN
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [2, 0, 1], 4,
+                              inv_sqrt(128), U16)
+    assert_close(out[2:], want[2:], tol[2:])
+    assert (out[:2] == 7.0).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_prefill_of_the_largest_f16_values(device, fmt):
+    # 65504 rounds to 65536 in both formats, which f16 does not hold. Equal keys: means of values.
+    ctx, new = [70], [70]
+    bt, nb = make_tables(ctx, 16, 37)
+    g = gen_of(device, 37)
+    pool = random_pool(nb, 2, 16, 128, fmt, g, device)
+    key = torch.full((70, 2, 128), 65504.0, dtype=torch.float16, device=device)
+    value = torch.randn((70, 2, 128), device=device, generator=g).half()
+    value[:, 1] = -65504.0
+    run_append(pool, key, value, bt, ctx, new, device)
+    q = (torch.randn((70, 8, 128), device=device, generator=g) * 2.0 ** -10).half()
+    out = run_prefill(pool, q, bt, ctx, new, 2, device)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, new, 4, inv_sqrt(128),
+                              2.0 ** -8)
+    assert_close(out[:, :4], want[:, :4], tol[:, :4])
+    np.testing.assert_allclose(want[:, 4:], -65536.0, rtol=1e-12)  # 70 sums in 64 bits
+    # The copy's -65504 times probabilities rounded to f16, both ways and twice (P, then 1 / l).
+    err = (out[:, 4:].double() + 65504.0).abs()
+    assert err.max() <= 65504.0 * 2.0 ** -9
+    assert ops.device_status() == 0
 
 
 def test_bad_lengths_and_ids_are_reported(device):
