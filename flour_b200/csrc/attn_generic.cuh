@@ -265,7 +265,12 @@ __global__ void __launch_bounds__(kGenericThreads, 1) generic_attn_kernel(const 
 #pragma unroll
     for (int w = 0; w < kGenericWarps; ++w)
       if (ms[w] != neg_inf()) o += expf(ms[w] - M) * accs[w * kGenericMaxDim + x];
-    out[orow + x] = Elem<T>::from_f(o / wsum);  // cpu.rs:111: acc / running_sum, cast to q's dtype
+    if constexpr (k8 && std::is_same<T, __half>::value) {
+      const uint32_t r = pack2_sat<T>(o / wsum, 0.f);
+      out[orow + x] = __ushort_as_half(uint16_t(r));
+    } else {
+      out[orow + x] = Elem<T>::from_f(o / wsum);  // cpu.rs:111: acc / running_sum, cast to q's dtype
+    }
   }
 }
 

@@ -483,9 +483,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (2 * t < n_rep)
-          *reinterpret_cast<uint32_t *>(out + (2 * t) * HD + c * 16) = pack2<T>(o[c][0] * i0, o[c][2] * i0);
+          *reinterpret_cast<uint32_t *>(out + (2 * t) * HD + c * 16) = pack2_sat<T>(o[c][0] * i0, o[c][2] * i0);
         if (2 * t + 1 < n_rep)
-          *reinterpret_cast<uint32_t *>(out + (2 * t + 1) * HD + c * 16) = pack2<T>(o[c][1] * i1, o[c][3] * i1);
+          *reinterpret_cast<uint32_t *>(out + (2 * t + 1) * HD + c * 16) = pack2_sat<T>(o[c][1] * i1, o[c][3] * i1);
       }
     } else {
       const int which = i == seg ? 0 : 1;  // the range's first segment, or its last
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
       } else {
         T *out = static_cast<T *>(p.out) +
                  (size_t(token_of(item / H)) * p.num_heads + (item % H) * n_rep + h) * HD + d;
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack2_sat<T>(O.x * i, O.y * i), pack2_sat<T>(O.z * i, O.w * i));
       }
     }
   };

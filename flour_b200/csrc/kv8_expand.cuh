@@ -2,29 +2,18 @@
 //
 // A prompt's attention is tensor-bound: every cache byte meets up to 64 n_rep query rows per work
 // item, so the bytes are turned into the query type once (1 byte read, 2 written, 2 read again
-// through L2: 20 of the 188 us of 16 prompts with 18k cached and new tokens), and the tcgen05 kernel
-// (prefill_sm100.cuh) then runs as it is, fed by TMA. Converting inside it would need converter warps, for which its register
-// budget (96 a thread at 18 warps) has no room.
+// through L2: 20 of the 188 us of 16 prompts with 18k cached and new tokens), and the tcgen05
+// kernel (prefill_sm100.cuh) then runs as it is, fed by TMA. Converting inside it would need
+// converter warps, for which its register budget (96 a thread at 18 warps) has no room.
 //
 // byte * scale is exact in bf16 for the append's power-of-two scales; in f16 it is exact above
-// f16's subnormals, and what is larger than f16's largest becomes that: the codes of 65504 itself
-// stand for 65536, whose infinity would make NaN of a finite row. Rows behind the last token are written as zeros: NaN bytes that an earlier
-// owner left there would survive a probability of 0.
+// f16's subnormals, and saturates (pack2_sat). Rows behind the last token are written as zeros:
+// NaN bytes that an earlier owner left there would survive a probability of 0.
 #pragma once
 
 #include "kv8_common.cuh"
 
 namespace fa {
-
-template <typename T> __device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 top = __half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
-    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), top), __hneg2(top));
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    return pack2<T>(a, b);
-  }
-}
 
 struct Kv8ExpandParams {
   const uint8_t *cache[2];       // [num_blocks, num_kv_heads, block_size, head_dim]

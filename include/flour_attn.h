@@ -342,7 +342,8 @@ FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key,
 /* fa_paged_decode over an 8-bit cache: query/out [num_seqs, num_heads, head_dim] of `dtype` (an
  * fa_dtype). Scores, softmax and sums in f32; the bytes enter the products exactly, probabilities
  * rounded to f16. Rows of the last page behind the context are not used, whatever they hold (NaN
- * bytes among them). A sequence with an invalid length gives zeros and FA_DEVERR_CONTEXT.
+ * bytes among them). A sequence with an invalid length gives zeros and FA_DEVERR_CONTEXT. FA_F16
+ * outputs saturate (65504 quantises to 65536 in both formats).
  * The fast kernel takes FA_BF16 / FA_F16 queries, block_size 16, head_dim 64 or 128, n_rep <= 8,
  * 16-byte aligned slabs and an 8-byte aligned query; everything else runs the generic kernel.
  * Workspace: fa_paged_decode_kv8_workspace_size bytes (0: none), 256-byte aligned, zero-filled once
@@ -373,8 +374,8 @@ FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *quer
  * 1, total_q == num_seqs) runs the decode's kernel; a sequence with more is then FA_DEVERR_SEQLEN
  * and not written. Output rows behind cu_seqlens_q[num_seqs] are not written. The copy holds
  * f16's range for FA_F16 queries: magnitudes above 65504 become 65504, and below 2^-14 they are
- * rounded to steps of 2^-24 (the decode takes any f32 value of byte * scale). A NaN among the keys
- * and values of a sequence may reach all of its queries. */
+ * rounded to steps of 2^-24 (the decode takes any f32 value of byte * scale); outputs saturate as
+ * there. A NaN among the keys and values of a sequence may reach all of its queries. */
 FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
                                                   int32_t num_kv_heads, int32_t block_size,
                                                   int32_t head_dim, int32_t total_q,

@@ -466,6 +466,12 @@ def test_prefill_of_the_largest_f16_values(device, fmt):
     # The copy's -65504 times probabilities rounded to f16, both ways and twice (P, then 1 / l).
     err = (out[:, 4:].double() + 65504.0).abs()
     assert err.max() <= 65504.0 * 2.0 ** -9
+    # The decode's and the generic kernel's f32 sums are -65536: the largest f16, not an infinity.
+    one = run_decode(pool, q[:1], i32(bt, device), i32(ctx, device), ctx, 2)
+    assert (one[:, 4:] == -65504.0).all()
+    slow = ops.paged_prefill_kv8(q, *pool, i32([0, 70], device), i32(ctx, device), i32(bt, device), 4,
+                                 inv_sqrt(128), 70, 70, 0, ops.Workspace())
+    assert (slow[:, 4:] == -65504.0).all()
     assert ops.device_status() == 0
 
 
