@@ -1061,6 +1061,9 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     return stream_in(fa::logprobs_stream_kernel<T, 1024>, 1024, split);
   }
   if (rows <= 2 * sms) return stream_in(fa::logprobs_stream_kernel<T, 512>, 512, 1);
+  const int64_t slots = 8 * sms, waves = (rows + slots - 1) / slots;
+  if (rows > 4 * sms && (5 * rows >= 4 * waves * slots || (sizeof(T) == 4 && waves == 1)))
+    return stream_in(fa::logprobs_stream_kernel<T, 128>, 128, 1);
   return stream_in(fa::logprobs_stream_kernel<T, 256>, 256, 1);
 }
 

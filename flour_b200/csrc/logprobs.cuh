@@ -95,8 +95,8 @@ __device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b) {
   return v;
 }
 
-// A part of a row: m its largest logit, z = sum e^(x - m), w = sum e^(x - m) (x - m). A part
-// without a finite logit has m = -inf, z = 0. A NaN logit makes z NaN, for good.
+// A part of a row: m a reference near its largest logit, z = sum e^(x - m), w = sum e^(x - m) (x - m).
+// A part without a finite logit has m = -inf, z = 0. A NaN logit makes z NaN, for good.
 struct LpState {
   float m, z, w;
 };
@@ -133,6 +133,28 @@ __device__ __forceinline__ LpState lp_warp_join(LpState st) {
   return st;
 }
 
+// Two floats of one instruction.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 f32x2_parts(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
 // Logits e, e + 1 of the vectors `raw` (e even and constant once unrolled).
 template <typename T, int NV>
 __device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
@@ -146,10 +168,35 @@ __device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
     return unpack2<T>(i == 0 ? v.x : i == 2 ? v.y : i == 4 ? v.z : v.w);
 }
 
-// z and w of one vector of logits with care: masked logits (whose 0 * -inf must not count), a NaN,
-// logits whose product with log2(e) overflows, or none but -inf (m = -inf: only NaN counts).
-template <typename T>
-__device__ __forceinline__ float2 lp_sums_slow(uint4 v, float m) {
+// Sums of e^(x - m) and e^(x - m) (x - m) over N logits in vectors, against a reference m that no
+// logit passes by much. Four operations a logit: with L = log2(e), M = m L rounded and r = m L - M
+// (one fma, so exact), s = x L - M is one fma, e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r
+// leaves the sums. All but the exponential are done for two logits an instruction (2048 x 151643
+// bf16 -4.9 us). The second sum is NaN for a NaN, no reference (m = -inf), logits whose product with
+// log2(e) overflows, and without kMasked for masked logits (0 * -inf).
+template <typename T, bool kMasked, int NV>
+__device__ __forceinline__ float2 lp_sums_fast(const uint4 (&raw)[NV], float m) {
+  constexpr int N = NV * 16 / sizeof(T);
+  const float M = m * kLog2e, r = fmaf(m, kLog2e, -M);
+  const uint64_t L2 = f32x2(kLog2e, kLog2e), M2 = f32x2(-M, -M);
+  uint64_t z2 = 0, w2 = 0;
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 x = lp_pair<T>(raw, j);
+    uint64_t s2 = f32x2_fma(f32x2(x.x, x.y), L2, M2);
+    const float2 s = f32x2_parts(s2);
+    const uint64_t e2 = f32x2(ex2(s.x), ex2(s.y));
+    if (kMasked) s2 = f32x2(fmaxf(s.x, -1e30f), fmaxf(s.y, -1e30f));
+    z2 = f32x2_add(z2, e2);
+    w2 = f32x2_fma(e2, s2, w2);
+  }
+  const float2 zz = f32x2_parts(z2), ww = f32x2_parts(w2);
+  const float back = ex2(-r), z = zz.x + zz.y;
+  return make_float2(z * back, fmaf(-r, z, ww.x + ww.y) * (back * 0.693147180559945f));
+}
+
+// The same of one vector with care, where lp_sums_fast fails.
+template <typename T> __device__ __forceinline__ float2 lp_sums_slow(uint4 v, float m) {
   const uint4 raw[1] = {v};
   float z = 0.f, w = 0.f;
 #pragma unroll
@@ -168,44 +215,11 @@ __device__ __forceinline__ float2 lp_sums_slow(uint4 v, float m) {
   return make_float2(z, w);
 }
 
-template <typename T> __device__ __noinline__ float2 lp_sums_slow_call(uint4 v, float m) {
-  return lp_sums_slow<T>(v, m);
-}
-
-// z and w of the logits in `raw` against m >= all of them. Four operations a logit: with
-// L = log2(e), M = m L rounded and r = m L - M (one fma, so exact), s = x L - M is one fma,
-// e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r leaves the sums. Where that fails (see above; all
-// such cases make the sum NaN) the vectors are summed once more with care: by a call in the streaming
-// loop, whose code has to stay in the instruction cache (-2.5 %), in place in the part kernel, where
-// every row's last threads come here (-0.5 us).
-template <typename T, bool kCall, int NV>
-__device__ __forceinline__ void lp_sums(const uint4 (&raw)[NV], float m, float &z, float &w) {
-  constexpr int N = NV * 16 / sizeof(T);
-  const float M = m * kLog2e, r = fmaf(m, kLog2e, -M);
-  float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    const float2 x = lp_pair<T>(raw, j);
-    const float s0 = fmaf(x.x, kLog2e, -M), s1 = fmaf(x.y, kLog2e, -M);
-    const float e0 = ex2(s0), e1 = ex2(s1);
-    z0 += e0;
-    z1 += e1;
-    w0 = fmaf(e0, s0, w0);
-    w1 = fmaf(e1, s1, w1);
-  }
-  const float back = ex2(-r);
-  float zs = (z0 + z1) * back, ws = fmaf(-r, z0 + z1, w0 + w1) * (back * 0.693147180559945f);
-  if (ws != ws) {
-    zs = ws = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float2 a = kCall ? lp_sums_slow_call<T>(raw[i], m) : lp_sums_slow<T>(raw[i], m);
-      zs += a.x;
-      ws += a.y;
-    }
-  }
-  z += zs;
-  w += ws;
+// One vector that may hold masked logits.
+template <typename T> __device__ __noinline__ float2 lp_sums_vec(uint4 v, float m) {
+  const uint4 raw[1] = {v};
+  const float2 f = lp_sums_fast<T, true>(raw, m);
+  return f.y == f.y ? f : lp_sums_slow<T>(v, m);
 }
 
 // Logits e0 .. e0 + 15 bytes of x[0 .. end), -inf outside. Out of line: few vectors take it.
@@ -253,8 +267,14 @@ template <typename T> struct LpRow {
   __device__ __forceinline__ int index(int v) const { return v * VE - off; }
 };
 
-// The largest logit of each vector, and of all; -inf where there is no number. 16-bit ones are
-// compared two at a time.
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The largest logit of each vector, and of all; NaN if one is. 16-bit ones are compared two at a
+// time.
 template <typename T, int NV>
 __device__ __forceinline__ float lp_maxima(const uint4 (&raw)[NV], float (&vm)[NV]) {
   float tm = neg_inf();
@@ -263,14 +283,14 @@ __device__ __forceinline__ float lp_maxima(const uint4 (&raw)[NV], float (&vm)[N
     if constexpr (sizeof(T) == 2) {
       using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
       const T2 *w = reinterpret_cast<const T2 *>(&raw[i]);
-      const T2 m2 = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      const T2 m2 = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
       const float2 m = unpack2<T>(*reinterpret_cast<const uint32_t *>(&m2));
-      vm[i] = fmaxf(m.x, m.y);
+      vm[i] = max_nan(m.x, m.y);
     } else {
       const float2 a = lp_pair<T>(raw, i * 4), b = lp_pair<T>(raw, i * 4 + 2);
-      vm[i] = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+      vm[i] = max_nan(max_nan(a.x, a.y), max_nan(b.x, b.y));
     }
-    tm = fmaxf(tm, vm[i]);
+    tm = max_nan(tm, vm[i]);
   }
   return tm;
 }
@@ -396,13 +416,13 @@ __device__ __forceinline__ void lp_pool_add(LpPool &pool, const uint4 (&raw)[NV]
   }
 }
 
-// The best 32 of the pool, one key to a lane of warp 0. Each warp sorts every WARPS-th run of 32.
+// The best 32 of n keys, one key to a lane of warp 0. Each warp sorts every WARPS-th run of 32.
 template <int WARPS>
-__device__ __forceinline__ uint64_t lp_pool_top(const LpPool &pool, int n, uint64_t (&s_top)[WARPS][32]) {
+__device__ __forceinline__ uint64_t lp_pool_top(const uint64_t *keys, int n, uint64_t (&s_top)[WARPS][32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t top = 0;
   for (int i = 32 * warp; i < n; i += 32 * WARPS) {
-    const uint64_t c = warp_sort(i + lane < n ? pool.key[i + lane] : 0);
+    const uint64_t c = warp_sort(i + lane < n ? keys[i + lane] : 0);
     top = i == 32 * warp ? c : warp_merge(top, c);
   }
   const int lists = min(WARPS, (n + 31) / 32);
@@ -542,7 +562,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
   float z = 0.f, w = 0.f;
-  lp_sums<T, false>(raw, m, z, w);
+  const float2 f = lp_sums_fast<T, false>(raw, m);
+  if (f.y == f.y) {
+    z = f.x;
+    w = f.y;
+  } else {  // in place: every row's last threads come here (-0.5 us against a call)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float2 v = lp_sums_slow<T>(raw[i], m);
+      z += v.x;
+      w += v.y;
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -565,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_part_kernel(
     if (warp == 0)
       for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
   } else {
-    top = lp_pool_top<WARPS>(s_pool, n, s_top);
+    top = lp_pool_top<WARPS>(s_pool.key, n, s_top);
   }
   LpState st{m, 0.f, 0.f};
 #pragma unroll
@@ -602,15 +633,29 @@ __device__ __noinline__ uint64_t lp_reread(const LpRow<T> r, int v0, int v1, flo
 // Tiles of 64 bytes a thread, the next one in flight. The 32 groups of the CTA (THREADS / 32 lanes
 // each) keep their running maxima in shared memory, and the warps take a new bound from them after tiles
 // 1, 2, 4, 8, ...: without a barrier but the first, for maxima that a warp sees too early are still
-// a lower bound. About 32 ln(32 / (32 - k)) logits pass in each doubling. Where more than the pool
-// holds pass (ascending rows, many equal logits) the part is read a second time, with a list a warp.
+// a lower bound. About 32 ln(32 / (32 - k)) logits pass in each doubling. The vectors that hold them
+// are kept whole, and their logits looked at once behind the loop, a thread each, against the last
+// bound (2048 x 151643, 20 alternatives, f16: 133 us, 151 with the logits picked out in the loop, and
+// 120 without alternatives). Where more pass than the lists hold (ascending rows, many equal logits)
+// the part is read a second time, with a list a warp.
+constexpr int kLpVecs = 512, kLpKeys = 512;
+template <int WARPS> struct LpStreamPool {
+  union {
+    uint4 vec[kLpVecs];
+    uint64_t cand[WARPS * 64];  // of the second reading
+  };
+  int at[kLpVecs];              // a vector's number in the row
+  uint64_t key[kLpKeys];
+  int vecs, keys;
+};
+
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_stream_kernel(const LogprobParams p) {
   using Row = LpRow<T>;
-  constexpr int NV = 4, WARPS = THREADS / 32, GROUP = THREADS / 32;  // 32 groups
+  constexpr int NV = 4, WARPS = THREADS / 32, GROUP = THREADS / 32, TILE = THREADS * NV;  // 32 groups
   __shared__ LpState s_state[WARPS];
   __shared__ volatile float s_max[32];
-  __shared__ LpPool s_pool;
+  __shared__ LpStreamPool<WARPS> s_pool;
   __shared__ uint64_t s_top[WARPS][32];
   __shared__ LpPart s_parts[kLpMaxCluster];
   const int ranks = int(cooperative_groups::this_cluster().num_blocks());
@@ -619,52 +664,110 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_stream_kerne
   lp_cluster_arrive();
   if (tid == 0) {
     pdl_trigger();
-    s_pool.n = 0;
+    s_pool.vecs = s_pool.keys = 0;
   }
   pdl_wait();
   const int64_t row = blockIdx.x / ranks;
   const Row r(p, row);
   const int per = (r.nv + ranks - 1) / ranks, v0 = rank * per, v1 = min(r.nv, v0 + per);
   LpState st{neg_inf(), 0.f, 0.f};
-  float bound = -3.402823466e38f;  // no -inf passes
+  float largest = neg_inf(), bound = -3.402823466e38f;  // no -inf passes
+  auto put_max = [&] {
+    float m = largest;
+#pragma unroll
+    for (int o = 1; o < GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane % GROUP == 0) s_max[tid / GROUP] = m;
+  };
+  auto raise_bound = [&] { bound = fmaxf(bound, __shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1)); };
   uint4 next[NV];
   r.load_tile(next, v0, v0 + tid, THREADS, v1);
   int tile = 0;
-  for (int vt = v0; vt < v1; vt += THREADS * NV, ++tile) {
+  bool masked = false;  // a tile held masked logits: the others are taken to do so too
+  for (int vt = v0; vt < v1; vt += TILE, ++tile) {
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = next[i];
-    if (vt + THREADS * NV < v1)
-      r.load_tile(next, vt + THREADS * NV, vt + THREADS * NV + tid, THREADS, v1);
+    if (vt + TILE < v1) r.load_tile(next, vt + TILE, vt + TILE + tid, THREADS, v1);
     float vm[NV];
     const float tm = lp_maxima<T>(raw, vm);
-    if (tm > st.m) lp_shift(st, tm);
+    largest = fmaxf(largest, tm);
+    // The reference moves only where e^(x - m) would leave e^8 behind: hardly ever after the first
+    // tile, where some lane of a warp finds a new maximum in most tiles (-1.9 us).
+    if (tm > st.m + 8.f) lp_shift(st, tm);
     if (K > 0) {
       if ((tile & (tile + 1)) == 0) {
-        float m = st.m;
-#pragma unroll
-        for (int o = 1; o < GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane % GROUP == 0) s_max[tid / GROUP] = m;
+        put_max();
         if (tile == 0) __syncthreads();
         __syncwarp();
-        bound = fmaxf(bound, __shfl_sync(0xffffffffu, warp_sort(float(s_max[lane])), K - 1));
+        raise_bound();
       }
-      if (tm >= bound) lp_pool_add(s_pool, raw, vm, bound, r, vt + tid, THREADS);
+      if (tm >= bound) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (vm[i] >= bound) {
+            const int at = atomicAdd(&s_pool.vecs, 1);
+            if (at < kLpVecs) {
+              s_pool.vec[at] = raw[i];
+              s_pool.at[at] = vt + tid + i * THREADS;
+            }
+          }
+      }
     }
-    lp_sums<T, true>(raw, st.m, st.z, st.w);
+    if (!(tm > neg_inf())) {  // masked logits only, or a NaN
+      if (tm != tm) st.z = tm;
+      continue;
+    }
+    // The sums; vector by vector, and by a call (the loop's code has to stay in the instruction
+    // cache), in the last tile, whose vectors behind the row are left out, and where logits are masked.
+    if (!masked && vt + TILE <= v1) {
+      const float2 f = lp_sums_fast<T, false>(raw, st.m);
+      if (f.y == f.y) {
+        st.z += f.x;
+        st.w += f.y;
+        continue;
+      }
+      masked = tile > 0;  // the first may fail for what lies before the row
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (vm[i] > neg_inf()) {
+        const float2 f = lp_sums_vec<T>(raw[i], st.m);
+        st.z += f.x;
+        st.w += f.y;
+      }
   }
+  if (K > 0) put_max();
   st = lp_warp_join(st);
   if (lane == 0) s_state[warp] = st;
   __syncthreads();
-  const int n = s_pool.n;
   uint64_t top = 0;
-  if (n > kLpPool) {
-    s_top[warp][lane] = lp_reread<T, THREADS>(r, v0, v1, bound, s_pool.key + warp * 64, K);
+  if (K > 0) {
+    const int n = s_pool.vecs;
+    raise_bound();
+    for (int i = tid; i < n && n <= kLpVecs; i += THREADS) {
+      const uint4 one[1] = {s_pool.vec[i]};
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < Row::VE; j += 2) {
+        const float2 x = lp_pair<T>(one, j);
+        if (x.x >= bound) bits |= 1u << j;
+        if (x.y >= bound) bits |= 2u << j;
+      }
+      const T *x = reinterpret_cast<const T *>(&s_pool.vec[i]);
+      for (; bits; bits &= bits - 1) {
+        const int j = __ffs(bits) - 1, at = atomicAdd(&s_pool.keys, 1);
+        if (at < kLpKeys) s_pool.key[at] = lp_key(Elem<T>::to_f(x[j]), r.index(s_pool.at[i]) + j);
+      }
+    }
     __syncthreads();
-    if (warp == 0)
-      for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
-  } else {
-    top = lp_pool_top<WARPS>(s_pool, n, s_top);
+    if (n <= kLpVecs && s_pool.keys <= kLpKeys) {
+      top = lp_pool_top<WARPS>(s_pool.key, s_pool.keys, s_top);
+    } else {
+      s_top[warp][lane] = lp_reread<T, THREADS>(r, v0, v1, bound, s_pool.cand + warp * 64, K);
+      __syncthreads();
+      if (warp == 0)
+        for (int i = 0; i < WARPS; ++i) top = warp_merge(top, s_top[i][lane]);
+    }
   }
   st = lp_warp_join(lane < WARPS ? s_state[lane] : LpState{neg_inf(), 0.f, 0.f});
   lp_finish<T>(p, r.x, row, st, top, s_parts);
