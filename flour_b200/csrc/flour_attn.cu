@@ -1034,12 +1034,12 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     return launch_pdl(who, fa::logprobs_part_kernel<T, fa::kLpSmallThreads>, dim3(unsigned(rows)),
                       fa::kLpSmallThreads, 0, stream, 1, p);
   const int64_t ranks = (span + kLpPartTile - 1) / kLpPartTile;
-  // Two CTAs of the part kernel fit an SM. One CTA a row stays ahead of streaming for eight a
-  // SM (10000 logits, bf16, 20 alternatives: 600 rows 17.8 us against 19.9, 2000 rows 49.4 against
-  // 48.7); clusters do for two and a half (128256 logits: 48 rows 14.6 against 16.5, 64 rows 17.8
-  // against 17.1, 148 rows 35.6 against 29.3).
+  // Two CTAs of the part kernel fit an SM; while all are resident it is ahead of streaming (10000
+  // logits, bf16, 20 alternatives: 148 rows 7.8 us against 9.8, 296 rows 9.2 against 9.8, 592 rows
+  // 15.8 against 10.3), clusters up to two and a half an SM (128256 logits: 32 rows 11.1 against
+  // 11.7, 48 rows 14.2 against 13.8, 148 rows 34 against 17).
   const int64_t ctas = rows * ranks, sms = sm_count();
-  if (ranks <= fa::kLpMaxCluster && (ranks == 1 ? ctas <= 8 * sms : 2 * ctas <= 5 * sms)) {
+  if (ranks <= fa::kLpMaxCluster && (ranks == 1 ? ctas <= 2 * sms : 2 * ctas <= 5 * sms)) {
     auto kern = fa::logprobs_part_kernel<T, fa::kLpPartThreads>;
     if (ranks > 8) {
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -1048,10 +1048,14 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     return launch_pdl(who, kern, dim3(unsigned(rows * ranks)), fa::kLpPartThreads, 0, stream, int(ranks), p);
   }
   // Streaming: the most threads a row that still leave all rows resident at once, one CTA a row
-  // (128256 f32 logits, 20 alternatives, 256 / 512 / 1024 threads: 148 rows 31.9 / 22.9 / 20.9 us,
-  // 296 rows 37.5 / 33.2 / 40.4, 592 rows 56.5 / 62.3 / 78.1). Clusters of smaller CTAs cost more to
-  // launch than they balance (64 rows in eight CTAs of 256 threads each 19.3 us, two of 1024 16.7;
-  // 592 rows in two of 256 69.3), so a row is cut only where fewer than half the SMs have one.
+  // (128256 f32 logits, 20 alternatives, 256 / 512 / 1024 threads: 148 rows 28.8 / 20.7 / 19.9 us,
+  // 296 rows 34.1 / 30.5 / 38.2, 592 rows 51.6 / 57.2 / 73). Clusters of smaller CTAs cost more to
+  // launch than they balance (64 rows in eight CTAs of 256 threads each 19.3 us, two of 1024 16.7),
+  // so a row is cut only where fewer than half the SMs have one.
+  // 128 threads start and end a row with less: for short rows from 2 and 4 rows an SM (592 x 10000
+  // bf16 10.3 us, 12.4 with 256; 1184 x 20000 21.3, 27.4), for others where they fill waves of eight
+  // rows an SM to four fifths (151643 bf16: 2048 rows 113, 118 with 256; 1500 rows 96.6, 94.5; 888
+  // rows 68, 59) or, f32, which HBM bounds, fill the only one in part (1024 rows of 128256 83, 88).
   auto stream_in = [&](auto kern, int threads, int split) {
     return launch_pdl(who, kern, dim3(unsigned(rows * split)), threads, 0, stream, split, p);
   };
@@ -1061,9 +1065,11 @@ fa_status launch_logprobs(const fa::LogprobParams &p, int rows, cudaStream_t str
     return stream_in(fa::logprobs_stream_kernel<T, 1024>, 1024, split);
   }
   if (rows <= 2 * sms) return stream_in(fa::logprobs_stream_kernel<T, 512>, 512, 1);
-  const int64_t slots = 8 * sms, waves = (rows + slots - 1) / slots;
-  if (rows > 4 * sms && (5 * rows >= 4 * waves * slots || (sizeof(T) == 4 && waves == 1)))
-    return stream_in(fa::logprobs_stream_kernel<T, 128>, 128, 1);
+  const int64_t slots = 8 * sms, waves = (rows + slots - 1) / slots, bytes = span * sizeof(T);
+  const bool narrow = rows <= 4 * sms ? bytes <= 32 * 1024
+                                      : bytes <= 64 * 1024 || 5 * rows >= 4 * waves * slots ||
+                                            (sizeof(T) == 4 && waves == 1);
+  if (narrow) return stream_in(fa::logprobs_stream_kernel<T, 128>, 128, 1);
   return stream_in(fa::logprobs_stream_kernel<T, 256>, 256, 1);
 }
 

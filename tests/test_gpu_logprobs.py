@@ -41,10 +41,12 @@ def reference(x, ids, k):
     return lp, ent, top_i, top_l
 
 
-def check(x, ids, k, out=None):
+def check(x, ids, k, out=None, kinds=None):
+    """kinds: the rows are repetitions of the first so many."""
     ids = np.asarray(ids, np.int32)
     lp, ent, ti, tl = out or ops.token_logprobs(x, torch.as_tensor(ids, device=x.device), k)
-    wlp, went, wti, wtl = reference(x, ids, k)
+    n = kinds or x.shape[0]
+    wlp, went, wti, wtl = [np.concatenate([w] * (x.shape[0] // n)) for w in reference(x[:n], ids[:n], k)]
     V = x.shape[1]
     rel = 2.0 ** -24 * math.sqrt(V) + 2.0 ** -21
     np.testing.assert_array_equal(ti.cpu().numpy(), wti)
@@ -68,7 +70,8 @@ def logits(R, V, dtype, device, seed, scale=3.0, pad=0, shift=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("R, V, k", [(1, 1, 1), (2, 7, 5), (3, 31, 32), (5, 257, 20), (1, 8191, 1), (4, 8193, 20),
-                                     (1, 151936, 20), (9, 50257, 5), (64, 128256, 20), (700, 1003, 0), (100, 40009, 20), (1, 300001, 32), (250, 33001, 5), (400, 21000, 20),
+                                     (1, 151936, 20), (9, 50257, 5), (64, 128256, 20), (700, 1003, 0), (100, 40009, 20), (1, 300001, 32),
+                                     (250, 33001, 5), (400, 21000, 20), (400, 8200, 20), (650, 17001, 32),
                                      (1200, 2049, 8)])
 def test_sizes(device, dtype, R, V, k):
     x = logits(R, V, dtype, device, R + V)
@@ -128,6 +131,39 @@ def test_masked_rows(device):
     lp = ops.token_logprobs(x[:7], torch.tensor(dead, dtype=torch.int32, device=device))[0]
     assert (lp == -math.inf).all()
     check(torch.where(keep, x, torch.finfo(torch.float32).min)[1:], ids[1:], 20)  # masks of the lowest value
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [144, 288, 576, 1176])  # of 1024, 512, 256 and 128 threads
+def test_rows_of_all_kinds_streamed(device, R, dtype):
+    # 33001 logits: every row starts at another offset from 16 bytes.
+    V, kinds, info = 33001, 12, torch.finfo(dtype)
+    x = logits(kinds, V, torch.float32, device, 20)
+    i = torch.arange(V, device=device)
+    x[1] = -math.inf
+    x[2, i != 30000] = -math.inf
+    x[3, i % 1600 != 7] = -math.inf             # 21 left
+    x[4, i % 2 == 0] = -math.inf
+    x[5] = i * 1e-3                             # ascending: every tile holds new candidates
+    x[6] = i * -1e-3
+    x[7] += 1e4
+    x[8] = i * 1e-2                             # and new references
+    x[9] = 1.5
+    x[10, i % 3 > 0] = info.min                 # masks of the lowest value
+    x[11, 7], x[11, 8] = info.max, info.min
+    x = x.to(dtype).repeat(R // kinds, 1)
+    ids = [int((x[r] > -math.inf).nonzero()[-1]) if r != 1 else -1 for r in range(kinds)] * (R // kinds)
+    check(x, ids, 20, kinds=kinds)
+    bad = torch.tensor([3, 20, R - 1], device=device)
+    x[bad, torch.tensor([0, 16000, V - 1], device=device)] = torch.tensor([math.nan, math.inf, math.nan],
+                                                                         device=device, dtype=dtype)
+    x[bad[2], :V - 1] = -math.inf
+    out = ops.token_logprobs(x, torch.tensor(ids, dtype=torch.int32, device=device), 20)
+    for t in (out[0], out[1], out[3]):
+        assert t[bad].isnan().all()
+    assert (out[2][bad] == -1).all()
+    good = [r for r in range(kinds, 2 * kinds) if r != 20]
+    check(x[good], [ids[r] for r in good], 20, tuple(t[good] for t in out))
 
 
 def test_large_offsets_and_spreads(device):
