@@ -1,6 +1,7 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits rows.
 //
-// With m = max x and Z = sum e^(x - m) over a row's logits x:
+// With m near max x (the streaming form lets it lag by up to 8) and Z = sum e^(x - m) over a row's
+// logits x:
 //   log p(t) = x_t - m - ln Z,   H = -sum p ln p = ln Z - (1/Z) sum e^(x - m) (x - m),
 // and the k tokens of highest logit, ties to the lower index. A logit of -inf is a token that a
 // mask took out: it has probability 0, adds nothing, and is not listed.
@@ -485,7 +486,8 @@ __device__ __forceinline__ void lp_finish(const LogprobParams &p, const T *x, in
   }
   if (warp != 0) return;
   // A NaN or +inf logit makes z NaN and with it everything said of the row. A row without a
-  // finite logit says that nothing can come: -inf for any token, no alternatives, entropy 0.
+  // finite logit says that nothing can come: -inf for any token, no alternatives, entropy 0. No
+  // rounding makes a probability larger than 1.
   const bool bad = st.z != st.z || st.m == -neg_inf();
   const bool none = st.m == neg_inf();
   const float ln_z = none ? 0.f : logf(st.z);
@@ -498,7 +500,7 @@ __device__ __forceinline__ void lp_finish(const LogprobParams &p, const T *x, in
         report(FA_DEVERR_TOKEN);
         lp = nan;
       } else if (t >= 0) {
-        lp = bad ? nan : none ? neg_inf() : (Elem<T>::to_f(x[t]) - st.m) - ln_z;
+        lp = bad ? nan : none ? neg_inf() : fminf((Elem<T>::to_f(x[t]) - st.m) - ln_z, 0.f);
       }
       p.logprobs[row] = lp;
     }
@@ -507,7 +509,7 @@ __device__ __forceinline__ void lp_finish(const LogprobParams &p, const T *x, in
   if (lane < K) {
     const bool has = top != 0 && !bad;
     p.top_ids[row * K + lane] = has ? int32_t(0xffffffffu - uint32_t(top)) : -1;
-    p.top_logprobs[row * K + lane] = bad ? nan : has ? (lp_value(top) - st.m) - ln_z : neg_inf();
+    p.top_logprobs[row * K + lane] = bad ? nan : has ? fminf((lp_value(top) - st.m) - ln_z, 0.f) : neg_inf();
   }
 }
 
