@@ -33,7 +33,8 @@
 // less than the bf16 of the 16-bit decode. The scale of K multiplies a score in f32; the larger of
 // the pair's two scales of V multiplies its product in f32, and the other page's probabilities take
 // the ratio (a power of two for scales of the append, and then exact). Probabilities are rounded at
-// 2^12 times their size, so that the ratio does not push them among f16's subnormals.
+// 2^12 times their size, so that neither the ratio nor a loud page (whose scale multiplies the
+// rounding of its small probabilities) meets f16's subnormals above 2^-26.
 #pragma once
 
 #include "decode_sm100.cuh"
@@ -426,13 +427,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
       const float vs = fmaxf(vs0, vs1);
       const bool apart = fminf(vs0, vs1) < vs * 0.015625f || vs < 1.e-34f;
       const float inv = vs > 0.f ? 4096.f / vs : 0.f;  // both scales 0: nothing to add
-      const float ra = apart ? 1.f : vs0 * inv, rb = apart ? 0.f : vs1 * inv;
+      const float ra = apart ? 4096.f : vs0 * inv, rb = apart ? 4096.f : vs1 * inv;
       const uint32_t pa0 = movmatrix_t(pack2<__half>(ca[0] * ra, ca[1] * ra));
       const uint32_t pa1 = movmatrix_t(pack2<__half>(ca[2] * ra, ca[3] * ra));
       const uint32_t pb0 = movmatrix_t(pack2<__half>(cb[0] * rb, cb[1] * rb));
       const uint32_t pb1 = movmatrix_t(pack2<__half>(cb[2] * rb, cb[3] * rb));
-      // o += (P_a V_a + P_b V_b) factor
-      auto values = [&](uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, float factor) {
+      // o += (P_a V_a + P_b V_b) down factor
+      auto values = [&](uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, float down, float factor) {
 #pragma unroll
         for (int ch = 0; ch < CH; ch += 2) {
           float ta[2][4];
@@ -454,18 +455,15 @@ __global__ void __launch_bounds__(kDecodeThreads, 3)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q], factor, o[ch + e][q]);
+            for (int q = 0; q < 4; ++q) o[ch + e][q] = fmaf(ta[e][q] * down, factor, o[ch + e][q]);
         }
       };
       if (!apart) {
-        values(pa0, pa1, pb0, pb1, vs * (1.f / 4096.f));
-      } else {  // more than a factor 64 between the pages: one after the other
+        values(pa0, pa1, pb0, pb1, 1.f, vs * (1.f / 4096.f));
+      } else {  // more than a factor 64 between the pages, or tiny scales: one after the other
 #pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t q0 = movmatrix_t(pack2<__half>(cb[0], cb[1]));
-          const uint32_t q1 = movmatrix_t(pack2<__half>(cb[2], cb[3]));
-          values(x ? 0u : pa0, x ? 0u : pa1, x ? q0 : 0u, x ? q1 : 0u, x ? vs1 : vs0);
-        }
+        for (int x = 0; x < 2; ++x)
+          values(x ? 0u : pa0, x ? 0u : pa1, x ? pb0 : 0u, x ? pb1 : 0u, 1.f / 4096.f, x ? vs1 : vs0);
       }
       __syncwarp();
       if (lane == 0 && i + NSTAGE < n_my) issue(i + NSTAGE);

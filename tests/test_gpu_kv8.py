@@ -248,6 +248,39 @@ def test_decode_small_probabilities_of_a_quiet_page(device, first, second):
     assert_close(out, want, tol)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("first, second", [(2.0 ** 6, 2.0 ** -14), (2.0 ** -14, 2.0 ** 6), (0.9, 0.0007),
+                                           (0.0007, 0.9), (2.0 ** -126, 2.0 ** -112), (1.3e-34, 1.7e-36)])
+def test_decode_small_probabilities_of_a_loud_page(device, dtype, first, second):
+    # Two pages of one step, the scales of V more than 64 apart, and the louder page's probabilities
+    # near 2^-22 of the largest: its scale multiplies their rounding. Probabilities are rounded at
+    # 2^12 times their size, so under the smallest normal f16 they move in half steps of 2^-37.
+    ctx, d, Hkv, n_rep = [32, 29, 32], 128, 2, 4
+    bt, nb = make_tables(ctx, 16, 60)
+    g = gen_of(device, 60)
+    pool = random_pool(nb, Hkv, 16, d, torch.int8, g, device)
+    loud = 0 if first > second else 1
+    k = torch.randint(-8, 9, pool[0].shape, device=device, generator=g, dtype=torch.int8)
+    k[..., 0] = 127
+    k[torch.as_tensor(bt[:, loud], device=device).long(), :, :, 0] = 0
+    scales = torch.empty_like(pool[3])
+    scales[torch.as_tensor(bt[:, 0], device=device).long()] = first
+    scales[torch.as_tensor(bt[:, 1], device=device).long()] = second
+    pool = (k, pool[1], torch.full_like(pool[2], 1 / 64.0), scales)
+    q = torch.randn((3, Hkv * n_rep, d), device=device, generator=g)
+    q[..., 0] = 22 * math.log(2.0) / (127 / 64.0 * inv_sqrt(d))
+    q = q.to(dtype)
+    want, tol = attention_ref(q.double().cpu().numpy(), pool, torch.as_tensor(bt), ctx, [1] * 3, n_rep,
+                              inv_sqrt(d), U16)
+    v = np.abs(_kv8.dequant(pool[1], pool[3]))
+    for s, L in enumerate(ctx):  # sum |v| over a sequence's tokens, a row for each query head
+        total = np.concatenate([v[b] for b in bt[s]], 1)[:, :L].sum(1).repeat(n_rep, 0)
+        tol[s] += (2.0 ** -37 - 2.0 ** -24) * total
+    out = run_decode(pool, q, i32(bt, device), i32(ctx, device), ctx, Hkv)
+    assert_close(out, want, tol)
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("q_scale", [2.0 ** -60, 2.0 ** 40, 0.0])
 def test_decode_queries_outside_f16(device, q_scale):
     ctx = [100]
