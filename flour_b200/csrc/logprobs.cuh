@@ -174,7 +174,9 @@ __device__ __forceinline__ float2 lp_pair(const uint4 (&raw)[NV], int e) {
 // (one fma, so exact), s = x L - M is one fma, e^(x - m) = 2^(s - r) and x - m = (s - r) / L; r
 // leaves the sums. All but the exponential are done for two logits an instruction (2048 x 151643
 // bf16 -4.9 us). The second sum is NaN for a NaN, no reference (m = -inf), logits whose product with
-// log2(e) overflows, and without kMasked for masked logits (0 * -inf).
+// log2(e) overflows, and without kMasked for masked logits (0 * -inf). It is made NaN where |r| > 1
+// (|m| from 2^25 / log2(e) on): s near r is then rounded in steps that show in e^(x - m), and from
+// |r| = 126 on 2^s is 0.
 template <typename T, bool kMasked, int NV>
 __device__ __forceinline__ float2 lp_sums_fast(const uint4 (&raw)[NV], float m) {
   constexpr int N = NV * 16 / sizeof(T);
@@ -192,7 +194,7 @@ __device__ __forceinline__ float2 lp_sums_fast(const uint4 (&raw)[NV], float m) 
     w2 = f32x2_fma(e2, s2, w2);
   }
   const float2 zz = f32x2_parts(z2), ww = f32x2_parts(w2);
-  const float back = ex2(-r), z = zz.x + zz.y;
+  const float back = fabsf(r) <= 1.f ? ex2(-r) : __int_as_float(0x7fc00000), z = zz.x + zz.y;
   return make_float2(z * back, fmaf(-r, z, ww.x + ww.y) * (back * 0.693147180559945f));
 }
 

@@ -194,6 +194,20 @@ def test_large_offsets_and_spreads(device):
     check(big, [7, 7, 7, 7], 3)
 
 
+@pytest.mark.parametrize("V", [1000, 4000, 9000, 16300, 40000])
+@pytest.mark.parametrize("R", [8, 160, 1200])
+def test_logits_of_any_size(device, R, V):
+    # f32 rows of one value c, and of c and its neighbour, from 1e6 to 3e38 of both signs: c log2(e)
+    # is then far from an f32 number, and what is left of it must not push e^(x - m) out of range.
+    c = torch.logspace(6, 38, 8, dtype=torch.float64)
+    c[1], c[3], c[4], c[5] = 1.581e9, -1.2e10, 1.7e9, -1.591e9
+    c[6] *= -1
+    x = c.float().to(device)[:, None].repeat(1, V)
+    x[:, V // 2] = torch.nextafter(x[:, 0], torch.full((8,), math.inf, device=device))
+    x[1::4, V // 2] = x[1::4, 0]
+    check(x.repeat(R // 8, 1), [V // 2, V - 1] * (R // 2), 5, kinds=8)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_nan_and_inf_rows(device, bad, dtype):
