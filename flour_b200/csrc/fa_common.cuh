@@ -49,6 +49,18 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   return *reinterpret_cast<uint32_t *>(&v);
 }
 
+// pack2, but what is larger than f16's largest becomes that: the codes of 65504 itself stand for
+// 65536, whose infinity would make NaN of a finite row. NaN stays.
+template <typename T> __device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 top = __half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
+    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), top), __hneg2(top));
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    return pack2<T>(a, b);
+  }
+}
+
 // ---- the reference's score rounding (FA_SCORES_REFERENCE) ---------------------------------
 // src/backend/cpu.rs:84-85 computes `(q.matmul(k^T) * scale).to_dtype(F32)` in the model dtype:
 // the q.k product is rounded to the dtype, multiplied by the scale rounded to the dtype, and the

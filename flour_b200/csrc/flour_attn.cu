@@ -388,11 +388,11 @@ int sm_count() {
   return cached[dev];
 }
 
-template <typename T, bool kRef, bool kSplit = false>
+template <typename T, bool kRef, bool kSplit = false, bool kSat = false>
 fa_status launch_prefill_t(const fa::PrefillParams &p, const CUtensorMap &tq, const CUtensorMap &tk,
                            const CUtensorMap &tv, int grid_x, cudaStream_t stream) {
   using S = fa::PrefillSmem;
-  auto kern = fa::paged_prefill_kernel<T, kRef, kSplit>;
+  auto kern = fa::paged_prefill_kernel<T, kRef, kSplit, kSat>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAllocMax);
   if (e != cudaSuccess) return fail(FA_ECUDA, "prefill: set smem attribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
@@ -410,8 +410,9 @@ fa_status launch_prefill_t(const fa::PrefillParams &p, const CUtensorMap &tq, co
   return check_launch("paged_prefill");
 }
 
-// The split form of a prefill: parts of part_tiles KV tiles, their rows in `part` (f32 outputs and,
-// behind parts * total_q * num_heads * 128 of them, the log2-sum-exps).
+// How an 8-bit cache's copy is attended (f16 outputs saturate): contexts in parts of part_tiles KV
+// tiles, their rows in `part` (f32 outputs and, behind parts * total_q * num_heads * 128 of them, the
+// log2-sum-exps), or in one part, which leaves nothing there.
 struct PrefillSplit {
   int parts, part_tiles;
   float *part;
@@ -457,7 +458,7 @@ fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const i
     p.context_lens = ctx + s0;
     p.block_tables = tables + size_t(s0) * max_blocks;
     int64_t items = ((int64_t(total_q) + chunk - 1) / chunk + p.num_seqs) * L->num_kv_heads;
-    if (split) {  // one launch: callers split no batch of more than kPfMaxSeqs sequences
+    if (split && split->parts > 1) {  // one launch: callers split no batch of more than kPfMaxSeqs sequences
       p.part_tiles = split->part_tiles;
       p.part_o = split->part;
       p.part_lse = split->part + size_t(split->parts) * total_q * num_heads * 128;
@@ -471,8 +472,9 @@ fa_status launch_prefill(const fa_kv_layer *L, const void *q, void *out, const i
         L->dtype == FA_BF16
             ? (ref ? launch_prefill_t<__nv_bfloat16, true>(p, tmq, tk, tv, grid, stream)
                    : launch_prefill_t<__nv_bfloat16, false>(p, tmq, tk, tv, grid, stream))
-            : (ref ? launch_prefill_t<__half, true>(p, tmq, tk, tv, grid, stream)
-                   : launch_prefill_t<__half, false>(p, tmq, tk, tv, grid, stream));
+            : (ref     ? launch_prefill_t<__half, true>(p, tmq, tk, tv, grid, stream)
+               : split ? launch_prefill_t<__half, false, false, true>(p, tmq, tk, tv, grid, stream)
+                       : launch_prefill_t<__half, false>(p, tmq, tk, tv, grid, stream));
     if (st != FA_OK) return st;
   }
   return ok();
@@ -1188,7 +1190,7 @@ fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32
   split.part = reinterpret_cast<float *>(wsb + w.part_off);
   st = launch_prefill(&copy, pad ? e.q_out : q, out, cu, e.out_ctx, e.out_tables, e.out_width, num_seqs,
                       num_heads, n_rep, total_q, scale, FA_SCORES_F32, ws, kPrefillWorkspace, stream,
-                      pad ? box : 0, split.parts > 1 ? &split : nullptr);
+                      pad ? box : 0, &split);
   if (st != FA_OK || split.parts == 1) return st;
   fa::PrefillParams j{};
   j.out = out;

@@ -93,18 +93,6 @@ template <class F> __device__ __forceinline__ float pow2_scale(float a) {
   return __uint_as_float(uint32_t(max(e, -126) + 127) << 23);
 }
 
-// pack2, but what is larger than f16's largest becomes that: the codes of 65504 itself stand for
-// 65536, whose infinity would make NaN of a finite row. NaN stays.
-template <typename T> __device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 top = __half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
-    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), top), __hneg2(top));
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    return pack2<T>(a, b);
-  }
-}
-
 struct Kv8AppendParams {
   const void *x[2];              // key, value: x[t*stride_t + h*stride_h + i]
   int64_t stride_t[2], stride_h[2];

@@ -131,7 +131,9 @@ __device__ __forceinline__ int prefill_parts(int L, int part_tiles) {
 }
 
 // kRef: the reference's dtype rounding of the scores (ref_score, FA_SCORES_REFERENCE).
-template <typename T, bool kRef, bool kSplit = false>
+// kSat: f16 outputs saturate. P is rounded and the row sum is not, so that O / l may pass the largest
+// value by 2^-11 of it, and 65504 of an 8-bit cache's copy would become an infinity.
+template <typename T, bool kRef, bool kSplit = false, bool kSat = false>
 __global__ void __launch_bounds__(kPfThreads, 1)
     paged_prefill_kernel(const __grid_constant__ PrefillParams p,
                          const __grid_constant__ CUtensorMap tm_q,
@@ -608,7 +610,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            pk[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            pk[e] = kSat ? pack2_sat<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv)
+                         : pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
           // Two full 32-byte sectors per store: each row half is written by one thread, so
           // wider stores mean fewer scattered transactions clogging the load/store pipe.
           st_global_v8(orow + c * 32, pk);
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const PrefillParams p
   }
   const float i = 1.f / W;  // part 0 holds position 0, which every row sees
   *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + rh * 128 + lane * 4) =
-      make_uint2(pack2<T>(O.x * i, O.y * i), pack2<T>(O.z * i, O.w * i));
+      make_uint2(pack2_sat<T>(O.x * i, O.y * i), pack2_sat<T>(O.z * i, O.w * i));
 }
 
 }  // namespace fa

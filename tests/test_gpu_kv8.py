@@ -508,6 +508,28 @@ def test_prefill_of_the_largest_f16_values(device, fmt):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("ctx, new", [([128], [128]), ([2944], [40])])  # in one piece, split over the context
+def test_prefill_f16_outputs_saturate(device, ctx, new):
+    # Values of 65504, one key of each 128 with probability 1 and the others just above the middle
+    # of two f16 numbers at 0.5: rounded up, they carry the mean to 65534, which f16 rounds to inf.
+    H, n_rep, d = 2, 4, 128
+    bt, nb = make_tables(ctx, 16, 61)
+    g = gen_of(device, 61)
+    pool = random_pool(nb, H, 16, d, torch.float8_e4m3fn, g, device)
+    key = torch.zeros((ctx[0], H, d), dtype=torch.float16, device=device)
+    key[::128, :, 0] = 1.0
+    value = torch.full_like(key, 65504.0)
+    value[:, 1] = -65504.0
+    run_append(pool, key, value, bt, ctx, ctx, device)
+    q = torch.zeros((new[0], H * n_rep, d), dtype=torch.float16, device=device)
+    q[..., 0] = 1.0
+    scale = math.log(2.0) - 1.05 * 2.0 ** -11  # e^-scale = 0.5 (1 + 1.05 * 2^-11)
+    out = ops.paged_prefill_kv8(q, *pool, i32([0, new[0]], device), i32(ctx, device), i32(bt, device), n_rep,
+                                scale, new[0], ctx[0], nb, ops.Workspace())
+    assert (out[:, :n_rep] == 65504.0).all() and (out[:, n_rep:] == -65504.0).all()
+    assert ops.device_status() == 0
+
+
 def test_bad_lengths_and_ids_are_reported(device):
     ctx = [40, 50]
     pool, q, bt, cl, want, tol = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, ctx, 34)
