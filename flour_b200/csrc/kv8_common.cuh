@@ -2,7 +2,9 @@
 //
 // A cache value is byte * scale[block, kv head], K and V apart. The append writes scales that are
 // powers of two, which makes every quotient x / scale exact (one rounding, to the 8-bit grid) and
-// every dequantised value exact in bf16 (e4m3 has 4 significant bits, an int8 magnitude 7).
+// every dequantised value exact in bf16 (e4m3 has 4 significant bits, an int8 magnitude 7). A
+// part-filled block of a cache quantised elsewhere may keep another scale: its quotients are formed
+// in 64 bits (to_odd), so that they too are rounded once.
 #pragma once
 
 #include "fa_common.cuh"
@@ -137,7 +139,16 @@ __device__ __forceinline__ float append_scale(float amax, float before, bool hel
   return after;
 }
 
-// One warp appends one run to one head of K or V: any head_dim, block_size and alignment.
+__device__ __forceinline__ bool is_pow2(float s) { return (__float_as_uint(s) & 0x7fffffu) == 0; }
+
+// x in f32 with what was cut off kept in the last bit, so that rounding the result to 8 significant
+// bits or fewer gives what rounding x would: no border between two codes has that bit.
+__device__ __forceinline__ float to_odd(double x) {
+  const float f = __double2float_rz(x);
+  return double(f) == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// One warp appends one run to one head of K or V: any head_dim, block_size, alignment and scale.
 template <typename T, class F>
 __device__ __forceinline__ bool append_run(const Kv8AppendParams &p, const Kv8Run &r, int h, int kv) {
   const int lane = threadIdx.x & 31, D = p.head_dim;
@@ -156,12 +167,17 @@ __device__ __forceinline__ bool append_run(const Kv8AppendParams &p, const Kv8Ru
   }
   float move;
   const float after = append_scale<F>(warp_max(amax), before, r.row0 > 0, move), inv = 1.f / after;
+  const bool exact = is_pow2(after) && is_pow2(move);
   if (move != 1.f)
-    for (int i = lane; i < r.row0 * D; i += 32)
-      page[i] = uint8_t(to_bytes2<F>(byte_to_f<F>(page[i]) * move, 0.f));
-  for (int i = lane; i < r.n * D; i += 32)
-    page[size_t(r.row0) * D + i] = uint8_t(
-        to_bytes2<F>(Elem<T>::to_f(x[int64_t(i / D) * p.stride_t[kv] + i % D]) * inv, 0.f));
+    for (int i = lane; i < r.row0 * D; i += 32) {
+      const float b = byte_to_f<F>(page[i]);
+      page[i] = uint8_t(to_bytes2<F>(exact ? b * move : to_odd(double(b) * double(move)), 0.f));
+    }
+  for (int i = lane; i < r.n * D; i += 32) {
+    const float f = Elem<T>::to_f(x[int64_t(i / D) * p.stride_t[kv] + i % D]);
+    page[size_t(r.row0) * D + i] =
+        uint8_t(to_bytes2<F>(exact ? f * inv : to_odd(double(f) / double(after)), 0.f));
+  }
   if (lane == 0) *sc = after;
   return bad;
 }
@@ -169,7 +185,8 @@ __device__ __forceinline__ bool append_run(const Kv8AppendParams &p, const Kv8Ru
 // The same for block_size 16, head_dim D of 64 or 128 and 16-byte aligned rows: the run's rows are
 // loaded at once, 8 values a lane and row (4 KB of bf16 a warp in flight at D = 128), and stay in
 // registers between the maximum and the rounding. Magnitudes are compared as integers, two 16-bit
-// ones an instruction; a run with an infinity or NaN (the largest patterns) takes append_run.
+// ones an instruction; a run with an infinity or NaN (the largest patterns), and a block whose scale
+// is or was not a power of two, takes append_run.
 template <typename T, class F, int D>
 __device__ __forceinline__ bool append_run_vec(const Kv8AppendParams &p, const Kv8Run &r, int h, int kv) {
   constexpr int LANES = D / 8, ROWS = 32 / LANES, PASSES = 16 / ROWS, W = sizeof(T) * 2;
@@ -212,9 +229,9 @@ __device__ __forceinline__ bool append_run_vec(const Kv8AppendParams &p, const K
     amax = unpack2<T>(mx).x;
     fin = mx < (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
   }
-  if (!fin) return append_run<T, F>(p, r, h, kv);
   float move;
   const float after = append_scale<F>(amax, before, r.row0 > 0, move), inv = 1.f / after;
+  if (!fin || !is_pow2(after) || !is_pow2(move)) return append_run<T, F>(p, r, h, kv);
   if (move != 1.f) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {

@@ -323,8 +323,10 @@ typedef struct fa_kv8_layer {
  *           count), else max(scale, need)
  *   rows before o: re-encoded when the scale grew, q' = round(q * old / new); else untouched
  *   new rows: round(x / scale), to nearest, ties to even; rows behind them: untouched.
- * A scale only grows while its block fills, at most by factors of two or more, so re-encoding
- * loses at most one int8 step in all, and nothing in e4m3 above its subnormals.
+ * A scale only grows while its block fills, and among powers of two by factors of two or more, so
+ * re-encoding loses at most one int8 step in all, and nothing in e4m3 above its subnormals. A
+ * part-filled block of a cache quantised elsewhere may have any finite scale >= 0: it keeps it
+ * until a new row needs more, and quotients are still rounded once (in 64 bits, at less speed).
  * Infinities saturate; NaN is stored as e4m3's NaN or int8's 0; either sets FA_DEVERR_VALUE and
  * leaves the scale to the finite values.
  * A block that receives tokens must appear once, in one sequence's table (a shared prefix block is

@@ -112,6 +112,39 @@ def test_append_values_at_the_borders(device, fmt):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("fmt, ratio", [(torch.int8, 1 / 6), (torch.float8_e4m3fn, 17 / 208)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [128, 40])
+def test_append_into_blocks_of_any_scale(device, fmt, ratio, dtype, d):
+    # Part-filled blocks of a cache quantised elsewhere, scales that are not powers of two: one
+    # sequence whose scale stays, with new values next to the borders between two codes, and one
+    # whose scale grows by 1 / ratio, which brings old codes next to such borders.
+    H, ctx, new = 3, [14, 14], [7, 7]
+    bt, nb = make_tables([16, 16], 16, 62)
+    g = gen_of(device, 62)
+    top = _kv8.QMAX[fmt]
+    pool = random_pool(nb, H, 16, d, fmt, g, device)
+    stays, grows = float(np.float32(0.0123)), float(np.float32(ratio)) * 2.0 ** -5
+    for s in pool[2:]:
+        s[int(bt[0, 0])], s[int(bt[1, 0])] = stays, grows
+    key = torch.randn((14, H, d), device=device, generator=g, dtype=torch.float64)
+    # The scale stays up to its largest code times 2^-7, the power of two below it: 80 and 284 codes.
+    if fmt == torch.int8:
+        codes = torch.randint(-80, 80, (7, H, d), device=device, generator=g) + 0.5
+    else:  # 5 significant bits, at most 248
+        codes = (torch.randint(8, 16, (7, H, d), device=device, generator=g) * 2 + 1) * \
+            torch.exp2(torch.randint(-4, 4, (7, H, d), device=device, generator=g).double())
+    key[:7] = codes * stays
+    key[7:] *= 0.25 * top * 2.0 ** -5 / key[7:].abs().amax((0, 2), keepdim=True)
+    key[7:, :, 0] = 0.9 * top * 2.0 ** -5  # the new scale is 2^-5
+    key = key.to(dtype)
+    before = clone(pool)
+    run_append(pool, key, -key, bt, ctx, new, device)
+    assert (pool[2][int(bt[0, 0])] == stays).all() and (pool[2][int(bt[1, 0])] == 2.0 ** -5).all()
+    check_append(pool, before, key, -key, bt, ctx, new)
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_append_nonfinite_values_are_reported_and_do_not_set_the_scale(device, fmt):
     bt, nb = make_tables([20], 16, 7)
