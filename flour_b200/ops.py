@@ -129,15 +129,23 @@ def workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: i
                                                        head_dim, max_context_len, max_seqlen_q))
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class Workspace:
     """Caller-owned, zero-initialised scratch for the split-K partials (grown on demand).
     One Workspace per stream: concurrent calls must not share it. The 8-bit entry points (kv8)
-    keep a Workspace of their own, apart from the others'."""
+    keep a Workspace of their own, apart from the others'. A CUDA graph holds the address of the
+    buffer that its calls were captured with: keep the Workspace as long as such graphs. A buffer
+    that it outgrows stays allocated if a captured call used it."""
 
     def __init__(self, device=None):
         self.device = torch.device(device if device is not None else "cuda")
         self.buf: torch.Tensor | None = None
         self.kv8: bool | None = None  # which entry points use it, from the first call that needs it
+        self.captured = False         # a graph may hold the address of buf
+        self.kept: list[torch.Tensor] = []  # outgrown buffers whose address a graph may hold
 
     def claim(self, kv8: bool) -> None:
         if self.kv8 is None:
@@ -150,10 +158,14 @@ class Workspace:
         if nbytes == 0:
             return self.buf
         if self.buf is None or self.buf.numel() < nbytes:
+            if self.captured:
+                self.kept.append(self.buf)
+                self.captured = False
             self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
             # A fresh zero-filled buffer: bookkeeping kept for an earlier buffer at the same
             # address (the caching allocator reuses addresses) no longer applies.
             check(lib().fa_workspace_reset(_ptr(self.buf)), "workspace_reset")
+        self.captured |= _capturing(self.device)
         return self.buf
 
 

@@ -649,6 +649,33 @@ def test_graphs_of_any_sizes_share_a_workspace(device):
     assert ops.device_status() == 0
 
 
+def test_a_workspace_grows_under_a_captured_graph(device):
+    # A decode captured on a warmed workspace, a prefill that outgrows it, other tensors where its
+    # buffer would have been: the replay gives the same bits and touches none of them.
+    ctx, new = [3000, 2500], [200, 100]
+    pool, q, bt, cl, want, tol = decode_case(device, torch.float8_e4m3fn, torch.bfloat16, 8, 2, 128, ctx, 63)
+    qp = torch.randn((300, 8, 128), device=device, generator=gen_of(device, 64)).to(torch.bfloat16)
+    ws = ops.Workspace()
+    ref = run_decode(pool, q, bt, cl, ctx, 2, ws)
+    assert_close(ref, want, tol)
+    size, out = ws.get(1).numel(), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_decode(pool, q, bt, cl, ctx, 2, ws, out=out)
+    want_p = run_prefill(pool, qp, bt.cpu().numpy(), ctx, new, 2, device)
+    assert torch.equal(run_prefill(pool, qp, bt.cpu().numpy(), ctx, new, 2, device, ws=ws), want_p)
+    assert ws.get(1).numel() > size
+    others = [torch.full((size,), 0x5A, dtype=torch.uint8, device=device) for _ in range(8)]
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, ref)
+        assert torch.equal(run_prefill(pool, qp, bt.cpu().numpy(), ctx, new, 2, device, ws=ws), want_p)
+    assert all((t == 0x5A).all() for t in others)
+    del graph
+    assert ops.device_status() == 0
+
+
 def test_a_16_bit_workspace_is_refused(device):
     pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, [40, 5000], 53)
     ws = ops.Workspace()

@@ -2,6 +2,7 @@
 launch; the plain forms used by the GPU tests hold their own definition."""
 
 import ctypes
+import weakref
 
 import numpy as np
 import pytest
@@ -128,6 +129,22 @@ def test_a_workspace_serves_8_bit_calls_or_the_others():
         ws.claim(False)
     with pytest.raises(FlourAttnError):
         ops._ws_args(ws, 256)
+
+
+def test_a_workspace_keeps_outgrown_buffers_that_graphs_hold(monkeypatch):
+    ws = ops.Workspace("cpu")
+    old = weakref.ref(ws.get(100))
+    ws.get(1000)
+    assert old() is None                  # no graph: freed
+    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    held = weakref.ref(ws.get(500))
+    monkeypatch.undo()
+    at = held().data_ptr()
+    assert ws.get(1000).data_ptr() == at  # still large enough
+    for n in (2000, 3000):
+        ws.get(n)
+        assert held() is not None and held().data_ptr() == at
+    assert ws.get(10).numel() == 3000
 
 
 def test_cpu_tensors_are_refused():
