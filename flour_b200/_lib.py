@@ -26,6 +26,7 @@ FA_DEVERR_LAUNCH = 0x80
 FA_DEVERR_VALUE = 0x100
 FA_DEVERR_TOKEN = 0x200
 FA_KV8_E4M3, FA_KV8_I8 = 16, 17
+FA_KV8_WORKSPACE_HEAD = 256 * 1024
 FA_MAX_TOP_LOGPROBS = 32
 FA_MAX_COPY_LAYERS = 128
 FA_NOALLOC_DECODE_SCRATCH_BYTES = 8 * 1024 * 1024

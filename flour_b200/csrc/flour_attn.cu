@@ -876,7 +876,7 @@ fa_status launch_pdl(const char *who, void (*kern)(KArgs...), dim3 grid, int thr
 // Start of an 8-bit workspace: the prefill kernel's work counters, then the decode's tickets, both
 // zero between launches. What calls leave behind lies past it, so calls of any sizes, captured or
 // not, may share a workspace without clearing anything.
-constexpr size_t kKv8Reserved = 256 * 1024;
+constexpr size_t kKv8Reserved = FA_KV8_WORKSPACE_HEAD;
 constexpr int kKv8MaxTickets = int((kKv8Reserved - kPrefillWorkspace) / 4);
 
 bool decode8_fast_shape(int32_t dtype, int n_rep, int block_size, int head_dim) {

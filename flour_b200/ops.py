@@ -138,7 +138,9 @@ class Workspace:
     One Workspace per stream: concurrent calls must not share it. The 8-bit entry points (kv8)
     keep a Workspace of their own, apart from the others'. A CUDA graph holds the address of the
     buffer that its calls were captured with: keep the Workspace as long as such graphs. A buffer
-    that it outgrows stays allocated if a captured call used it."""
+    that it outgrows stays allocated if a captured call used it. Grow it before a capture (by an
+    eager call, or `get`): a captured call that finds it too small takes memory of the graph's
+    own, which every replay has to clear."""
 
     def __init__(self, device=None):
         self.device = torch.device(device if device is not None else "cuda")
@@ -146,6 +148,7 @@ class Workspace:
         self.kv8: bool | None = None  # which entry points use it, from the first call that needs it
         self.captured = False         # a graph may hold the address of buf
         self.kept: list[torch.Tensor] = []  # outgrown buffers whose address a graph may hold
+        self.lent: torch.Tensor | None = None  # what the last captured call took instead
 
     def claim(self, kv8: bool) -> None:
         if self.kv8 is None:
@@ -154,10 +157,19 @@ class Workspace:
             raise _lib.FlourAttnError(_lib.FA_EINVAL,
                                       "8-bit and 16/32-bit calls need workspaces of their own")
 
-    def get(self, nbytes: int) -> torch.Tensor | None:
+    def get(self, nbytes: int, head: int | None = None) -> torch.Tensor | None:
+        """A buffer of at least `nbytes`; `head`: how many of them have to start as zero (all)."""
         if nbytes == 0:
             return self.buf
         if self.buf is None or self.buf.numel() < nbytes:
+            if _capturing(self.device):
+                # Allocated and cleared within the capture: it holds zeros only once this graph
+                # has been replayed, so no other graph and no eager call may be given it.
+                self.lent = None  # its memory serves the next captured call
+                self.lent = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+                self.lent[:head].zero_()
+                check(lib().fa_workspace_reset(_ptr(self.lent)), "workspace_reset")
+                return self.lent
             if self.captured:
                 self.kept.append(self.buf)
                 self.captured = False
@@ -519,10 +531,10 @@ def _ws8(workspace: Workspace | None, need: int, dev: int):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"a workspace of {need} bytes is required")
     workspace.claim(True)
     if torch._C._cuda_getDevice() == dev:
-        buf = workspace.get(need)
+        buf = workspace.get(need, _lib.FA_KV8_WORKSPACE_HEAD)
     else:
         with torch.cuda.device(dev):
-            buf = workspace.get(need)
+            buf = workspace.get(need, _lib.FA_KV8_WORKSPACE_HEAD)
     if buf.get_device() != dev:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"workspace on {buf.device}, tensors on cuda:{dev}")
     return buf.data_ptr(), buf.numel()

@@ -348,12 +348,13 @@ FA_API fa_status fa_paged_append_kv8(const fa_kv8_layer *layer, const void *key,
  * outputs saturate (65504 quantises to 65536 in both formats).
  * The fast kernel takes FA_BF16 / FA_F16 queries, block_size 16, head_dim 64 or 128, n_rep <= 8,
  * 16-byte aligned slabs and an 8-byte aligned query; everything else runs the generic kernel.
- * Workspace: fa_paged_decode_kv8_workspace_size bytes (0: none), 256-byte aligned, zero-filled once
- * before its first use. One workspace may serve 8-bit decodes and prefills of all sizes, also from
+ * Workspace: fa_paged_decode_kv8_workspace_size bytes (0: none), 256-byte aligned, its first
+ * FA_KV8_WORKSPACE_HEAD bytes zero-filled once before its first use. One workspace may serve 8-bit decodes and prefills of all sizes, also from
  * several CUDA graphs, as long as they do not overlap on the GPU; the 16-bit entry points need
  * another (their partial results land where the 8-bit calls keep their tickets). The generic
  * kernel needs none; buffers that are not aligned for the fast kernel run it whatever the
  * workspace. */
+#define FA_KV8_WORKSPACE_HEAD (256 * 1024)
 FA_API size_t fa_paged_decode_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
                                                  int32_t num_kv_heads, int32_t block_size,
                                                  int32_t head_dim, int32_t max_context_len);

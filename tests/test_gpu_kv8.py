@@ -676,6 +676,30 @@ def test_a_workspace_grows_under_a_captured_graph(device):
     assert ops.device_status() == 0
 
 
+def test_graphs_captured_on_a_fresh_workspace(device):
+    # No call before the captures, the largest first: graphs are replayed in any order, and eager
+    # calls come before the first replay.
+    ws, cases = ops.Workspace(), []
+    for Hq, Hkv, ctx, seed in ((32, 8, [700] * 100, 65), (8, 2, [5000, 3000], 66), (8, 2, [900], 67)):
+        pool, q, bt, cl, want, tol = decode_case(device, torch.int8, torch.bfloat16, Hq, Hkv, 128, ctx, seed)
+        ref = run_decode(pool, q, bt, cl, ctx, Hkv)
+        assert_close(ref, want, tol)
+        out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(2):
+                run_decode(pool, q, bt, cl, ctx, Hkv, ws, out=out)
+        cases.append((graph, out, ref, (pool, q, bt, cl, ctx, Hkv)))
+    for order in ((2, 1), (1, 2, 0), (0, 2, 1)):
+        for i in order:
+            graph, out, ref, args = cases[i]
+            assert torch.equal(run_decode(*args, ws), ref)
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, ref)
+    del graph, cases
+    assert ops.device_status() == 0
+
+
 def test_a_16_bit_workspace_is_refused(device):
     pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, [40, 5000], 53)
     ws = ops.Workspace()

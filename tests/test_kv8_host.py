@@ -147,6 +147,26 @@ def test_a_workspace_keeps_outgrown_buffers_that_graphs_hold(monkeypatch):
     assert ws.get(10).numel() == 3000
 
 
+def test_a_workspace_born_in_a_capture_belongs_to_that_graph(monkeypatch):
+    # What a captured call allocates holds zeros only after a replay: every captured call clears
+    # its own, and eager calls take another buffer.
+    ws = ops.Workspace("cpu")
+    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    first = ws.get(100)
+    first.fill_(7)
+    again = ws.get(100)
+    assert not again.any()
+    again.fill_(7)
+    monkeypatch.undo()
+    eager = ws.get(100)
+    assert eager.data_ptr() not in (first.data_ptr(), again.data_ptr()) and not eager.any()
+    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    assert ws.get(100) is eager           # large enough: the graph shares it
+    assert ws.get(1000).data_ptr() != eager.data_ptr()
+    monkeypatch.undo()
+    assert ws.get(100) is eager
+
+
 def test_cpu_tensors_are_refused():
     kc = torch.zeros((4, 2, 16, 64), dtype=torch.int8)
     sc = torch.ones((4, 2))
