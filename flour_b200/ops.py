@@ -129,13 +129,14 @@ def workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: i
                                                        head_dim, max_context_len, max_seqlen_q))
 
 
-def _capturing(device: torch.device) -> bool:
-    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+def _capturing(cuda: bool) -> bool:
+    return cuda and torch._C._cuda_isCurrentStreamCapturing()
 
 
 class Workspace:
     """Caller-owned, zero-initialised scratch for the split-K partials (grown on demand).
-    One Workspace per stream: concurrent calls must not share it. The 8-bit entry points (kv8)
+    One Workspace per stream: concurrent calls must not share it, and calls on several streams
+    are the caller's to order (its zero-fill and its freeing are ordered here). The 8-bit entry points (kv8)
     keep a Workspace of their own, apart from the others'. A CUDA graph holds the address of the
     buffer that its calls were captured with: keep the Workspace as long as such graphs. A buffer
     that it outgrows stays allocated if a captured call used it. Grow it before a capture (by an
@@ -144,11 +145,15 @@ class Workspace:
 
     def __init__(self, device=None):
         self.device = torch.device(device if device is not None else "cuda")
+        self.cuda = self.device.type == "cuda"
         self.buf: torch.Tensor | None = None
+        self.size, self.index = 0, -1  # of buf: bytes, CUDA device
         self.kv8: bool | None = None  # which entry points use it, from the first call that needs it
         self.captured = False         # a graph may hold the address of buf
         self.kept: list[torch.Tensor] = []  # outgrown buffers whose address a graph may hold
         self.lent: torch.Tensor | None = None  # what the last captured call took instead
+        self.filled: torch.cuda.Event | None = None  # behind the zero-fill of buf
+        self.streams: set[int] = set()  # those that are in order with it
 
     def claim(self, kv8: bool) -> None:
         if self.kv8 is None:
@@ -161,23 +166,37 @@ class Workspace:
         """A buffer of at least `nbytes`; `head`: how many of them have to start as zero (all)."""
         if nbytes == 0:
             return self.buf
-        if self.buf is None or self.buf.numel() < nbytes:
-            if _capturing(self.device):
-                # Allocated and cleared within the capture: it holds zeros only once this graph
-                # has been replayed, so no other graph and no eager call may be given it.
-                self.lent = None  # its memory serves the next captured call
-                self.lent = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-                self.lent[:head].zero_()
-                check(lib().fa_workspace_reset(_ptr(self.lent)), "workspace_reset")
-                return self.lent
-            if self.captured:
-                self.kept.append(self.buf)
-                self.captured = False
-            self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
-            # A fresh zero-filled buffer: bookkeeping kept for an earlier buffer at the same
-            # address (the caching allocator reuses addresses) no longer applies.
-            check(lib().fa_workspace_reset(_ptr(self.buf)), "workspace_reset")
-        self.captured |= _capturing(self.device)
+        capturing = _capturing(self.cuda)
+        if self.size >= nbytes:
+            if capturing:  # begins behind the fill
+                self.captured = True
+            elif self.filled is not None and torch._C._cuda_getCurrentRawStream(self.index) not in self.streams:
+                stream = torch.cuda.current_stream(self.index)
+                stream.wait_event(self.filled)
+                self.buf.record_stream(stream)  # freed only behind this stream's calls
+                self.streams.add(stream.cuda_stream)
+            return self.buf
+        if capturing:
+            # Allocated and cleared within the capture: it holds zeros only once this graph has
+            # been replayed, so no other graph and no eager call may be given it.
+            self.lent = None  # its memory serves the next captured call
+            self.lent = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            self.lent[:head].zero_()
+            check(lib().fa_workspace_reset(_ptr(self.lent)), "workspace_reset")
+            return self.lent
+        if self.captured:
+            self.kept.append(self.buf)
+            self.captured = False
+        self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        self.size = nbytes
+        # A fresh zero-filled buffer: bookkeeping kept for an earlier buffer at the same
+        # address (the caching allocator reuses addresses) no longer applies.
+        check(lib().fa_workspace_reset(_ptr(self.buf)), "workspace_reset")
+        if self.cuda:
+            self.index = self.buf.get_device()
+            stream = torch.cuda.current_stream(self.index)
+            self.filled = stream.record_event()
+            self.streams = {stream.cuda_stream}
         return self.buf
 
 
@@ -427,19 +446,30 @@ def _device(*tensors: torch.Tensor | None) -> int:
     return dev
 
 
-def _call_on(dev: int, stream, what: str, fn, *args) -> None:
-    """fn(*args, stream) on `stream`, or on the device's current stream, with it current."""
-    if stream is None:
-        raw = torch._C._cuda_getCurrentRawStream(dev)  # current_stream().cuda_stream, 2 us less
-    elif stream.device.index != dev:
+def _away(dev: int, stream) -> bool:
+    """Whether another device or stream has to become the current one for a call."""
+    return torch._C._cuda_getDevice() != dev or (
+        stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _there(dev: int, stream, what: str, fn, *args, **kw):
+    """fn(*args, stream=stream, **kw) with the device and `stream` (or the device's current one) current, so that
+    its allocations, fills and copies are in order with its launches. What it returns may be used
+    on the caller's stream once that waits for `stream`."""
+    if stream is not None and stream.device.index != dev:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"{what}: stream of {stream.device}, tensors on cuda:{dev}")
-    else:
-        raw = stream.cuda_stream
-    if torch._C._cuda_getDevice() == dev:
-        st = fn(*args, raw)
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, raw)
+    caller = torch.cuda.current_stream(dev)
+    with torch.cuda.device(dev), torch.cuda.stream(stream):
+        res = fn(*args, stream=stream, **kw)
+    for t in res if isinstance(res, tuple) else (res,):
+        if t is not None:
+            t.record_stream(caller)
+    return res
+
+
+def _call(dev: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the device's current stream (current_stream().cuda_stream, 2 us less)."""
+    st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if st != _lib.FA_OK:
         check(st, what)
 
@@ -500,6 +530,10 @@ def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_table
     holds context_lens[s] tokens, the new ones (cu_seqlens_q[s] .. cu_seqlens_q[s+1], or one each
     when cu_seqlens_q is None) included. A block's scale is a power of two that grows as it
     fills. A block that receives tokens belongs to one sequence of the call."""
+    dev = _device(k_cache, v_cache, k_scale, v_scale, key, value, block_tables, context_lens, cu_seqlens_q)
+    if _away(dev, stream):
+        return _there(dev, stream, "paged_append_kv8", paged_append_kv8, k_cache, v_cache, k_scale, v_scale,
+                      key, value, block_tables, context_lens, cu_seqlens_q)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     shape = key.shape
     if value.shape != shape or value.dtype is not key.dtype or len(shape) != 3 or \
@@ -518,10 +552,9 @@ def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_table
         S = context_lens.numel()
         cu = _cu(cu_seqlens_q, S)
     bt, cl = _tables(block_tables, context_lens, S)
-    dev = _device(k_cache, v_cache, k_scale, v_scale, key, value, bt, cl, cu)
-    _call_on(dev, stream, "paged_append_kv8", lib().fa_paged_append_kv8, ctypes.byref(layer),
-             key.data_ptr(), value.data_ptr(), fa_dtype(key.dtype), k_token, k_head, v_token, v_head,
-             None if cu is None else cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1], S, T)
+    _call(dev, "paged_append_kv8", lib().fa_paged_append_kv8, ctypes.byref(layer),
+          key.data_ptr(), value.data_ptr(), fa_dtype(key.dtype), k_token, k_head, v_token, v_head,
+          None if cu is None else cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1], S, T)
 
 
 def _ws8(workspace: Workspace | None, need: int, dev: int):
@@ -529,33 +562,32 @@ def _ws8(workspace: Workspace | None, need: int, dev: int):
         return None, 0
     if workspace is None:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"a workspace of {need} bytes is required")
-    workspace.claim(True)
-    if torch._C._cuda_getDevice() == dev:
-        buf = workspace.get(need, _lib.FA_KV8_WORKSPACE_HEAD)
-    else:
-        with torch.cuda.device(dev):
-            buf = workspace.get(need, _lib.FA_KV8_WORKSPACE_HEAD)
+    if workspace.kv8 is not True:
+        workspace.claim(True)
+    buf = workspace.get(need, _lib.FA_KV8_WORKSPACE_HEAD)
     if buf.get_device() != dev:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"workspace on {buf.device}, tensors on cuda:{dev}")
-    return buf.data_ptr(), buf.numel()
+    return buf.data_ptr(), need
 
 
 def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
                      n_rep: int, scale: float, max_context_len: int,
                      workspace: Workspace | None = None, out=None, stream=None):
     """paged_decode over an 8-bit pool: query [B, Hq, d] (bf16, f16 or f32) -> out [B, Hq, d]."""
+    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, block_tables, context_lens)
+    if _away(dev, stream):
+        return _there(dev, stream, "paged_decode_kv8", paged_decode_kv8, query, k_cache, v_cache, k_scale, v_scale,
+                      block_tables, context_lens, n_rep, scale, max_context_len, workspace, out)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     query, out = _query8(query, layer.head_dim, out)
     B, hq, d = query.shape
     bt, cl = _tables(block_tables, context_lens, B)
-    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl)
     L = lib()
     dt = fa_dtype(query.dtype)
     wp, wn = _ws8(workspace, L.fa_paged_decode_kv8_workspace_size(
         dt, B, hq, layer.num_kv_heads, layer.block_size, d, max_context_len), dev)
-    _call_on(dev, stream, "paged_decode_kv8", L.fa_paged_decode_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), dt, cl.data_ptr(), bt.data_ptr(),
-             bt.shape[1], B, hq, n_rep, max_context_len, scale, wp, wn)
+    _call(dev, "paged_decode_kv8", L.fa_paged_decode_kv8, ctypes.byref(layer), query.data_ptr(), out.data_ptr(),
+          dt, cl.data_ptr(), bt.data_ptr(), bt.shape[1], B, hq, n_rep, max_context_len, scale, wp, wn)
     return out
 
 
@@ -565,22 +597,25 @@ def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, c
                       workspace: Workspace | None = None, out=None, stream=None):
     """paged_prefill over an 8-bit pool whose suffix tokens are already appended. `total_blocks`:
     at least the sum of ceil(context_len / block_size) over the batch."""
+    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, block_tables, context_lens, cu_seqlens_q)
+    if _away(dev, stream):
+        return _there(dev, stream, "paged_prefill_kv8", paged_prefill_kv8, query, k_cache, v_cache, k_scale, v_scale,
+                      cu_seqlens_q, context_lens, block_tables, n_rep, scale, max_seqlen_q, max_context_len,
+                      total_blocks, workspace, out)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     query, out = _query8(query, layer.head_dim, out)
     tq, hq, d = query.shape
     S = context_lens.numel()
     bt, cl = _tables(block_tables, context_lens, S)
     cu = _cu(cu_seqlens_q, S)
-    dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, bt, cl, cu)
     L = lib()
     dt = fa_dtype(query.dtype)
     wp, wn = _ws8(workspace, L.fa_paged_prefill_kv8_workspace_size(
         dt, S, hq, layer.num_kv_heads, layer.block_size, d, tq, max_context_len, max_seqlen_q,
         total_blocks), dev)
-    _call_on(dev, stream, "paged_prefill_kv8", L.fa_paged_prefill_kv8, ctypes.byref(layer),
-             query.data_ptr(), out.data_ptr(), dt, cu.data_ptr(), cl.data_ptr(),
-             bt.data_ptr(), bt.shape[1], S, hq, n_rep, tq, max_seqlen_q, max_context_len,
-             total_blocks, scale, wp, wn)
+    _call(dev, "paged_prefill_kv8", L.fa_paged_prefill_kv8, ctypes.byref(layer), query.data_ptr(),
+          out.data_ptr(), dt, cu.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.shape[1], S, hq, n_rep, tq,
+          max_seqlen_q, max_context_len, total_blocks, scale, wp, wn)
     return out
 
 
@@ -591,6 +626,9 @@ def token_logprobs(logits, token_ids=None, top_k: int = 0, stream=None):
     V). token_ids int32 [R] (-1: none) or None. Returns (logprobs f32 [R] or None without
     token_ids, entropy f32 [R], top_ids int32 [R, top_k], top_logprobs f32 [R, top_k]); ties go
     to the lower id, tokens masked with -inf are not listed (id -1, -inf)."""
+    dev = _device(logits, token_ids)
+    if _away(dev, stream):
+        return _there(dev, stream, "token_logprobs", token_logprobs, logits, token_ids, top_k)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, "logits must be [rows, vocab] with unit stride on vocab")
     R, V = logits.shape
@@ -599,14 +637,13 @@ def token_logprobs(logits, token_ids=None, top_k: int = 0, stream=None):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"token_ids must be [{R}]")
     if not 0 <= top_k <= _lib.FA_MAX_TOP_LOGPROBS:
         raise _lib.FlourAttnError(_lib.FA_EINVAL, f"top_k {top_k} outside [0, {_lib.FA_MAX_TOP_LOGPROBS}]")
-    dev = _device(logits, ids)
     device, f32 = logits.device, torch.float32
     logprobs = None if ids is None else torch.empty(R, dtype=f32, device=device)
     entropy = torch.empty(R, dtype=f32, device=device)
     top_ids = torch.empty((R, top_k), dtype=torch.int32, device=device)
     top = torch.empty((R, top_k), dtype=f32, device=device)
-    _call_on(dev, stream, "token_logprobs", lib().fa_token_logprobs, logits.data_ptr(), fa_dtype(logits.dtype),
-             logits.stride(0), R, V, None if ids is None else ids.data_ptr(),
-             None if ids is None else logprobs.data_ptr(), entropy.data_ptr(), top_k,
-             top_ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None)
+    _call(dev, "token_logprobs", lib().fa_token_logprobs, logits.data_ptr(), fa_dtype(logits.dtype),
+          logits.stride(0), R, V, None if ids is None else ids.data_ptr(),
+          None if ids is None else logprobs.data_ptr(), entropy.data_ptr(), top_k,
+          top_ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None)
     return logprobs, entropy, top_ids, top

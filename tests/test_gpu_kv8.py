@@ -745,6 +745,55 @@ def test_side_stream_and_append_then_decode_chain(device):
         assert ops.device_status() == 0
 
 
+def test_an_explicit_stream_is_in_order_with_itself(device):
+    # stream= another stream than the current one, which stands still meanwhile: workspaces fresh,
+    # outgrown and made on the current stream, strided queries, outputs in memory that was in use.
+    ctx, new = [3000, 2500], [200, 100]
+    pool, q, bt, cl, want, tol = decode_case(device, torch.float8_e4m3fn, torch.bfloat16, 8, 2, 128, ctx, 68)
+    cu, blocks = i32([0, 200, 300], device), sum((c + 15) // 16 for c in ctx)
+    qp = torch.randn((300, 8, 128), device=device, generator=gen_of(device, 69)).to(torch.bfloat16)
+    want_p = run_prefill(pool, qp, bt.cpu().numpy(), ctx, new, 2, device)
+    ref = run_decode(pool, q, bt, cl, ctx, 2)
+    assert_close(ref, want, tol)
+    strided = torch.zeros((2, 8, 256), dtype=torch.bfloat16, device=device)
+    strided[..., :128] = q
+    logits = torch.randn((3, 5000), device=device)
+    ids = i32([1, 2, 3], device)
+    ref_l = ops.token_logprobs(logits, ids, 5)
+    key = torch.randn((2, 2, 128), device=device).to(torch.bfloat16)
+    after = clone(pool)
+    ops.paged_append_kv8(*after, key, key, bt, cl)
+    side = torch.cuda.Stream()
+    for junk_on in (torch.cuda.current_stream(), side):  # what fresh memory holds
+        with torch.cuda.stream(junk_on):
+            junk = [torch.full((32 << 20,), 0x5A, dtype=torch.uint8, device=device) for _ in range(6)]
+            del junk
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)  # 0.2 s
+    early = ops.Workspace()
+    early.get(64 << 20)  # filled behind the sleep
+    done.record()
+    ws = ops.Workspace()
+    got = [run_decode(pool, strided[..., :128], bt, cl, ctx, 2, ws, stream=side) for _ in range(2)]
+    got_p = [ops.paged_prefill_kv8(qp, *pool, cu, cl, bt, 4, inv_sqrt(128), 200, 3000, blocks, ws, stream=side)
+             for _ in range(2)]
+    got.append(run_decode(pool, strided[..., :128], bt, cl, ctx, 2, ws, stream=side))
+    got_l = ops.token_logprobs(logits, ids, 5, stream=side)
+    ops.paged_append_kv8(*pool, key, key, bt, cl, stream=side)
+    side.synchronize()
+    assert not done.query()  # none of it waited for the current stream
+    with torch.cuda.stream(side):
+        assert all(torch.equal(o, ref) for o in got) and all(torch.equal(o, want_p) for o in got_p)
+        assert all(torch.equal(a, b) for a, b in zip(got_l, ref_l))
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pool, after))
+    late = run_decode(pool, q, bt, cl, ctx, 2, early, stream=side)
+    side.synchronize()
+    assert done.query()  # the fill it needs is behind the sleep
+    assert torch.equal(late, run_decode(pool, q, bt, cl, ctx, 2))
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("S, ctx_hi", [(500, 40), (1100, 20)])
 def test_many_sequences(device, S, ctx_hi):
     # More sequences than one decode launch takes, more than the append searches in shared memory.

@@ -136,7 +136,7 @@ def test_a_workspace_keeps_outgrown_buffers_that_graphs_hold(monkeypatch):
     old = weakref.ref(ws.get(100))
     ws.get(1000)
     assert old() is None                  # no graph: freed
-    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    monkeypatch.setattr(ops, "_capturing", lambda cuda: True, raising=False)
     held = weakref.ref(ws.get(500))
     monkeypatch.undo()
     at = held().data_ptr()
@@ -151,7 +151,7 @@ def test_a_workspace_born_in_a_capture_belongs_to_that_graph(monkeypatch):
     # What a captured call allocates holds zeros only after a replay: every captured call clears
     # its own, and eager calls take another buffer.
     ws = ops.Workspace("cpu")
-    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    monkeypatch.setattr(ops, "_capturing", lambda cuda: True, raising=False)
     first = ws.get(100)
     first.fill_(7)
     again = ws.get(100)
@@ -160,7 +160,7 @@ def test_a_workspace_born_in_a_capture_belongs_to_that_graph(monkeypatch):
     monkeypatch.undo()
     eager = ws.get(100)
     assert eager.data_ptr() not in (first.data_ptr(), again.data_ptr()) and not eager.any()
-    monkeypatch.setattr(ops, "_capturing", lambda device: True, raising=False)
+    monkeypatch.setattr(ops, "_capturing", lambda cuda: True, raising=False)
     assert ws.get(100) is eager           # large enough: the graph shares it
     assert ws.get(1000).data_ptr() != eager.data_ptr()
     monkeypatch.undo()
