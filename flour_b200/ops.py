@@ -51,6 +51,32 @@ def _i32(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
+def _away(dev: int, stream) -> bool:
+    """Whether another device or stream has to become the current one for a call."""
+    return torch._C._cuda_getDevice() != dev or (
+        stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _there(dev: int, stream, fn, *args, **kw):
+    """fn(*args, stream=stream, **kw) with the device and `stream` (or the device's current one)
+    current, so that its allocations, fills and copies are in order with its launches. What it
+    returns may be used on the caller's stream once that waits for `stream`."""
+    if stream is not None and stream.device.index != dev:
+        raise _lib.FlourAttnError(_lib.FA_EINVAL,
+                                  f"{fn.__name__}: stream of {stream.device}, tensors on cuda:{dev}")
+    caller = torch.cuda.current_stream(dev)
+    with torch.cuda.device(dev), torch.cuda.stream(stream):
+        res = fn(*args, stream=stream, **kw)
+    for t in res if isinstance(res, tuple) else (res,):
+        if t is not None and t.is_cuda:
+            t.record_stream(caller)
+    return res
+
+
+def _elsewhere(stream) -> bool:
+    return stream is not None and _away(stream.device.index, stream)
+
+
 # ---- block writes / copies ----------------------------------------------------------------
 
 def reshape_and_cache(k_cache, v_cache, key, value, slot_mapping, stream=None) -> None:
@@ -77,6 +103,8 @@ def copy_blocks(k_caches, v_caches, block_mapping, stream=None) -> None:
 
 def write_block(k_cache, v_cache, block_id: int, key, value, stream=None) -> None:
     """PagedKvPool::write_block: key/value (kv_heads, bs, d), host (pinned or not) or device."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, write_block, k_cache, v_cache, block_id, key, value)
     layer = layer_desc(k_cache, v_cache)
     check(lib().fa_write_block(ctypes.byref(layer), block_id, _ptr(key.contiguous()),
                                _ptr(value.contiguous()), _stream(stream)), "write_block")
@@ -97,6 +125,9 @@ def export_bundle_payload(k_caches, v_caches, block_ids, payload=None, stream=No
     """FLKV payload of the physical blocks `block_ids` (logical order) of every layer, in one
     launch: for block, for layer, K then V (kv_heads, bs, d). Returns the device uint8 payload
     (`payload` if given); the caller copies it to the host in one transfer."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, export_bundle_payload, k_caches, v_caches, block_ids,
+                      payload)
     layers = (FaKvLayer * len(k_caches))(*[layer_desc(k, v) for k, v in zip(k_caches, v_caches)])
     ids = _i32(block_ids, "block_ids")
     n = bundle_payload_bytes(k_caches, v_caches, ids.numel())
@@ -216,6 +247,9 @@ def paged_decode(query, k_cache, v_cache, block_tables, context_lens, n_rep: int
     """One query token per sequence: query [B, Hq, d] -> out [B, Hq, d]. `score_flow`:
     FA_SCORES_F32 (default) or FA_SCORES_REFERENCE (the reference's bf16/f16 score rounding,
     src/backend/cpu.rs:84-85)."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, paged_decode, query, k_cache, v_cache, block_tables,
+                      context_lens, n_rep, scale, max_context_len, workspace, out, score_flow=score_flow)
     layer = layer_desc(k_cache, v_cache)
     query = query.contiguous()
     out = torch.empty_like(query) if out is None else out
@@ -236,6 +270,10 @@ def paged_decode_append(query, k_cache, v_cache, key, value, block_tables, conte
     """Write each sequence's new token (key/value [B, kv_heads, d], any token/head strides,
     unit stride on d) at position context_lens[b]-1, then decode query [B, Hq, d] over the whole
     context, in one launch: reshape_and_cache + paged_decode of a decode step."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, paged_decode_append, query, k_cache, v_cache, key, value,
+                      block_tables, context_lens, n_rep, scale, max_context_len, workspace, out,
+                      score_flow=score_flow)
     layer = layer_desc(k_cache, v_cache)
     query = query.contiguous()
     if key.stride(-1) != 1 or value.stride(-1) != 1:
@@ -260,6 +298,9 @@ def paged_decode_noalloc(query, k_cache, v_cache, block_tables, context_lens, n_
                         scale: float, max_context_len: int, out=None, stream=None):
     """paged_decode without a workspace: the split-K scratch is the library's fixed buffer
     (fa_paged_decode_noalloc). Calls on different streams must not overlap on the GPU."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, paged_decode_noalloc, query, k_cache, v_cache,
+                      block_tables, context_lens, n_rep, scale, max_context_len, out)
     layer = layer_desc(k_cache, v_cache)
     query = query.contiguous()
     out = torch.empty_like(query) if out is None else out
@@ -276,6 +317,10 @@ def paged_prefill(query, k_cache, v_cache, cu_seqlens_q, context_lens, block_tab
                   workspace: Workspace | None = None, out=None, stream=None,
                   score_flow: int = _lib.FA_SCORES_F32):
     """Varlen causal attention of packed suffix queries [Tq, Hq, d] over prefix+suffix KV."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, paged_prefill, query, k_cache, v_cache, cu_seqlens_q,
+                      context_lens, block_tables, n_rep, scale, max_seqlen_q, max_context_len, workspace, out,
+                      score_flow=score_flow)
     layer = layer_desc(k_cache, v_cache)
     query = query.contiguous()
     out = torch.empty_like(query) if out is None else out
@@ -297,6 +342,10 @@ def paged_attention_varlen(query, k_cache, v_cache, cu_seqlens_q, context_lens, 
                            workspace: Workspace | None = None, out=None, stream=None,
                            score_flow: int = _lib.FA_SCORES_F32):
     """The general entry (fa_paged_attention): decode or prefill chosen by the library."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, paged_attention_varlen, query, k_cache, v_cache,
+                      cu_seqlens_q, context_lens, block_tables, n_rep, scale, max_seqlen_q, max_context_len,
+                      workspace, out, score_flow=score_flow)
     layer = layer_desc(k_cache, v_cache)
     query = query.contiguous()
     out = torch.empty_like(query) if out is None else out
@@ -346,6 +395,10 @@ def qkv_rope_cache(x, weight, k_cache, v_cache, positions, slot_mapping, num_hea
     x [T, hidden]; weight [(num_heads + 2*kv_heads) * d, hidden] (q_proj, k_proj, v_proj rows
     stacked); positions / slot_mapping int32 [T]; rope_cos / rope_sin f32 [max_position, d/2].
     Returns q [T, num_heads, d]; K/V land in the pool. attention.rs:75-104."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, qkv_rope_cache, x, weight, k_cache, v_cache, positions,
+                      slot_mapping, num_heads, rope_cos, rope_sin, bias, q_norm_weight, k_norm_weight,
+                      rms_eps, q_out)
     layer = layer_desc(k_cache, v_cache)
     dt = k_cache.dtype
     x = _c16(x, "x", dt)
@@ -385,6 +438,9 @@ def last_token_logits(hidden, cu_seqlens, lm_head, norm_weight=None, rms_eps: fl
     """f32 logits [S, vocab] of each sequence's last token: final RMSNorm + lm_head
     (model.rs:56-58) on the rows the engine reads (engine.rs:220-222). hidden [T, H] packed,
     cu_seqlens int32 [S + 1], lm_head [vocab, H]."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, last_token_logits, hidden, cu_seqlens, lm_head,
+                      norm_weight, rms_eps, normed_out, logits_out)
     dt = hidden.dtype
     hidden = _c16(hidden, "hidden", dt)
     lm_head = _c16(lm_head, "lm_head", dt)
@@ -411,6 +467,8 @@ def o_proj_residual(attn, weight, residual=None, out=None, stream=None) -> torch
 
     attn [T, in_features] (heads concatenated), weight [out_features, in_features].
     attention.rs:116 + transformer.rs:37-38."""
+    if _elsewhere(stream):
+        return _there(stream.device.index, stream, o_proj_residual, attn, weight, residual, out)
     dt = attn.dtype
     attn = _c16(attn, "attn", dt)
     weight = _c16(weight, "weight", dt)
@@ -444,27 +502,6 @@ def _device(*tensors: torch.Tensor | None) -> int:
         raise _lib.FlourAttnError(_lib.FA_EINVAL,
                                   f"tensors must be on a CUDA device, not {tensors[0].device}")
     return dev
-
-
-def _away(dev: int, stream) -> bool:
-    """Whether another device or stream has to become the current one for a call."""
-    return torch._C._cuda_getDevice() != dev or (
-        stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(dev))
-
-
-def _there(dev: int, stream, what: str, fn, *args, **kw):
-    """fn(*args, stream=stream, **kw) with the device and `stream` (or the device's current one) current, so that
-    its allocations, fills and copies are in order with its launches. What it returns may be used
-    on the caller's stream once that waits for `stream`."""
-    if stream is not None and stream.device.index != dev:
-        raise _lib.FlourAttnError(_lib.FA_EINVAL, f"{what}: stream of {stream.device}, tensors on cuda:{dev}")
-    caller = torch.cuda.current_stream(dev)
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
-        res = fn(*args, stream=stream, **kw)
-    for t in res if isinstance(res, tuple) else (res,):
-        if t is not None:
-            t.record_stream(caller)
-    return res
 
 
 def _call(dev: int, what: str, fn, *args) -> None:
@@ -532,8 +569,8 @@ def paged_append_kv8(k_cache, v_cache, k_scale, v_scale, key, value, block_table
     fills. A block that receives tokens belongs to one sequence of the call."""
     dev = _device(k_cache, v_cache, k_scale, v_scale, key, value, block_tables, context_lens, cu_seqlens_q)
     if _away(dev, stream):
-        return _there(dev, stream, "paged_append_kv8", paged_append_kv8, k_cache, v_cache, k_scale, v_scale,
-                      key, value, block_tables, context_lens, cu_seqlens_q)
+        return _there(dev, stream, paged_append_kv8, k_cache, v_cache, k_scale, v_scale, key, value,
+                      block_tables, context_lens, cu_seqlens_q)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     shape = key.shape
     if value.shape != shape or value.dtype is not key.dtype or len(shape) != 3 or \
@@ -576,8 +613,8 @@ def paged_decode_kv8(query, k_cache, v_cache, k_scale, v_scale, block_tables, co
     """paged_decode over an 8-bit pool: query [B, Hq, d] (bf16, f16 or f32) -> out [B, Hq, d]."""
     dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, block_tables, context_lens)
     if _away(dev, stream):
-        return _there(dev, stream, "paged_decode_kv8", paged_decode_kv8, query, k_cache, v_cache, k_scale, v_scale,
-                      block_tables, context_lens, n_rep, scale, max_context_len, workspace, out)
+        return _there(dev, stream, paged_decode_kv8, query, k_cache, v_cache, k_scale, v_scale, block_tables,
+                      context_lens, n_rep, scale, max_context_len, workspace, out)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     query, out = _query8(query, layer.head_dim, out)
     B, hq, d = query.shape
@@ -599,9 +636,9 @@ def paged_prefill_kv8(query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, c
     at least the sum of ceil(context_len / block_size) over the batch."""
     dev = _device(k_cache, v_cache, k_scale, v_scale, query, out, block_tables, context_lens, cu_seqlens_q)
     if _away(dev, stream):
-        return _there(dev, stream, "paged_prefill_kv8", paged_prefill_kv8, query, k_cache, v_cache, k_scale, v_scale,
-                      cu_seqlens_q, context_lens, block_tables, n_rep, scale, max_seqlen_q, max_context_len,
-                      total_blocks, workspace, out)
+        return _there(dev, stream, paged_prefill_kv8, query, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q,
+                      context_lens, block_tables, n_rep, scale, max_seqlen_q, max_context_len, total_blocks,
+                      workspace, out)
     layer = kv8_layer_desc(k_cache, v_cache, k_scale, v_scale)
     query, out = _query8(query, layer.head_dim, out)
     tq, hq, d = query.shape
@@ -628,7 +665,7 @@ def token_logprobs(logits, token_ids=None, top_k: int = 0, stream=None):
     to the lower id, tokens masked with -inf are not listed (id -1, -inf)."""
     dev = _device(logits, token_ids)
     if _away(dev, stream):
-        return _there(dev, stream, "token_logprobs", token_logprobs, logits, token_ids, top_k)
+        return _there(dev, stream, token_logprobs, logits, token_ids, top_k)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _lib.FlourAttnError(_lib.FA_EINVAL, "logits must be [rows, vocab] with unit stride on vocab")
     R, V = logits.shape

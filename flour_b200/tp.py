@@ -169,6 +169,10 @@ class HeadShardedGroup:
         from . import ops
         if self._pending:
             raise FlourAttnError(_lib.FA_EINVAL, "decode: the previous decode has not been synced")
+        if ops._elsewhere(stream):
+            return ops._there(stream.device.index, stream, self.decode, query, k_cache, v_cache, block_tables,
+                              context_lens, n_rep, scale, max_context_len, workspace, wait, timeout_ns,
+                              score_flow=score_flow)
         layer = ops.layer_desc(k_cache, v_cache)
         query = query.contiguous()
         B, hq, d = query.shape
