@@ -953,6 +953,29 @@ def test_blocks_are_copied_with_their_scales(device):
         assert torch.equal(now[:7], was[:7])
 
 
+def test_blocks_are_exported_and_imported_with_their_scales(device):
+    # Bundles of an 8-bit pool of two layers: slabs as bf16 of half the head_dim, scales as f32
+    # layers of one element (three heads: runs of 12 bytes).
+    g = gen_of(device, 70)
+    src = [random_pool(12, 3, 16, 128, torch.int8, g, device) for _ in range(2)]
+    dst = [random_pool(9, 3, 16, 128, torch.int8, g, device) for _ in range(2)]
+    before = [clone(p) for p in dst]
+    ids, to = i32([7, 0, 11], device), i32([8, 1, 4], device)
+
+    def views(pools):
+        return (([p[0].view(torch.bfloat16) for p in pools], [p[1].view(torch.bfloat16) for p in pools]),
+                ([p[2][:, :, None, None] for p in pools], [p[3][:, :, None, None] for p in pools]))
+
+    for a, b in zip(views(src), views(dst)):
+        ops.import_bundle_payload(*b, to, ops.export_bundle_payload(*a, ids))
+    for s, d, was in zip(src, dst, before):
+        for x, y, z in zip(s, d, was):
+            assert torch.equal(y[to.long()], x[ids.long()])
+            rest = [i for i in range(9) if i not in (8, 1, 4)]
+            assert torch.equal(y[rest], z[rest])
+    assert ops.device_status() == 0
+
+
 def test_refusals(device):
     ctx = [40, 50]
     pool, q, bt, cl, _, _ = decode_case(device, torch.int8, torch.bfloat16, 8, 2, 128, ctx, 43)
