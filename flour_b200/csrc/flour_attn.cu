@@ -1179,9 +1179,12 @@ fa_status launch_prefill8(const fa_kv8_layer *L, const void *q, void *out, int32
   e.head_dim = L->head_dim;
   e.max_context_len = max_context_len;
   const int grid = std::max(1, std::min(total_blocks, sm_count() * 8));
-  fa_status st = with_types8(dtype, L->dtype, [&](auto t, auto f) {
-    return launch_pdl(who, fa::kv8_expand_kernel<decltype(t), decltype(f), true>, dim3(grid),
-                      fa::kExpandThreads, 0, stream, 1, e);
+  fa_status st = with_types8(dtype, L->dtype, [&](auto t, auto f) -> fa_status {
+    if constexpr (sizeof(t) == 2)
+      return launch_pdl(who, fa::kv8_expand_kernel<decltype(t), decltype(f)>, dim3(grid),
+                        fa::kExpandThreads, 0, stream, 1, e);
+    else
+      return fail(FA_EUNSUPPORTED, "%s: f32 queries take the generic kernel", who);
   });
   if (st != FA_OK) return st;
   const fa_kv_layer copy{wsb + w.k_off, wsb + w.v_off, total_blocks, L->num_kv_heads, L->block_size,

@@ -43,8 +43,9 @@ constexpr int kExpandMaxSeqs = 2048;  // sequences per call (page prefix sums in
 // CTA x takes blocks x, x + gridDim.x, ... of the copy; which sequence's page a block is follows
 // from prefix sums of the page counts, which every CTA computes for itself (a few KB from L2).
 // Sequences are packed in order; one whose pages do not fit total_blocks is refused as a whole.
-template <typename T, class F, bool kVec>
+template <typename T, class F>
 __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Kv8ExpandParams p) {
+  static_assert(sizeof(T) == 2, "a copy in the type of the tensor-core prefill");
   __shared__ int32_t offs[kExpandMaxSeqs + 1];
   __shared__ int32_t warp_sum[kExpandThreads / 32];
   if (threadIdx.x == 0) pdl_trigger();
@@ -113,35 +114,24 @@ __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Kv8Exp
       const float sc = p.scale[kv][src];
       const uint8_t *in = p.cache[kv] + src * page;
       T *out = static_cast<T *>(p.out[kv]) + dst * page;
-      if (kVec) {  // 8 bytes in, 8 elements out; a row is a multiple of 8
-        for (int i = lane * 8; i < page; i += 256) {
-          uint2 r = make_uint2(0u, 0u);
-          if (i < live) r = *reinterpret_cast<const uint2 *>(in + i);
-          float2 f[4];
-          uint32_t a, b;
-          unpack4<F>(r.x, a, b);
-          f[0] = f16x2_to_f2(a);
-          f[1] = f16x2_to_f2(b);
-          unpack4<F>(r.y, a, b);
-          f[2] = f16x2_to_f2(a);
-          f[3] = f16x2_to_f2(b);
-          if (i >= live) f[0] = f[1] = f[2] = f[3] = make_float2(0.f, 0.f);
-          if constexpr (sizeof(T) == 2) {
-            uint4 v;
-            v.x = pack2_sat<T>(f[0].x * sc, f[0].y * sc);
-            v.y = pack2_sat<T>(f[1].x * sc, f[1].y * sc);
-            v.z = pack2_sat<T>(f[2].x * sc, f[2].y * sc);
-            v.w = pack2_sat<T>(f[3].x * sc, f[3].y * sc);
-            *reinterpret_cast<uint4 *>(out + i) = v;
-          } else {
-            float4 *o4 = reinterpret_cast<float4 *>(out + i);
-            o4[0] = make_float4(f[0].x * sc, f[0].y * sc, f[1].x * sc, f[1].y * sc);
-            o4[1] = make_float4(f[2].x * sc, f[2].y * sc, f[3].x * sc, f[3].y * sc);
-          }
-        }
-      } else {
-        for (int i = lane; i < page; i += 32)
-          out[i] = Elem<T>::from_f(i < live ? byte_to_f<F>(in[i]) * sc : 0.f);
+      for (int i = lane * 8; i < page; i += 256) {  // 8 bytes in, 8 elements out; a row is a multiple of 8
+        uint2 r = make_uint2(0u, 0u);
+        if (i < live) r = *reinterpret_cast<const uint2 *>(in + i);
+        float2 f[4];
+        uint32_t a, b;
+        unpack4<F>(r.x, a, b);
+        f[0] = f16x2_to_f2(a);
+        f[1] = f16x2_to_f2(b);
+        unpack4<F>(r.y, a, b);
+        f[2] = f16x2_to_f2(a);
+        f[3] = f16x2_to_f2(b);
+        if (i >= live) f[0] = f[1] = f[2] = f[3] = make_float2(0.f, 0.f);
+        uint4 v;
+        v.x = pack2_sat<T>(f[0].x * sc, f[0].y * sc);
+        v.y = pack2_sat<T>(f[1].x * sc, f[1].y * sc);
+        v.z = pack2_sat<T>(f[2].x * sc, f[2].y * sc);
+        v.w = pack2_sat<T>(f[3].x * sc, f[3].y * sc);
+        *reinterpret_cast<uint4 *>(out + i) = v;
       }
     }
   }
