@@ -1093,7 +1093,9 @@ bool prefill8_fast_path(const fa_kv8_layer *L, int n_rep, int32_t dtype, float s
 // knows total_q, not the lengths) do not fill the SMs a few times. In KV tiles of one item (about
 // 2.1 us): a wave of items lasts its longest part plus 1.2 for the item's start and end, and the
 // join moves every part's rows twice (one tile per 14 MB). One sequence of 509 tokens over 30001 (28
-// query heads, 4 KV heads: 60 items) takes 512 us unsplit and 274 in the 7 parts chosen here.
+// query heads, 4 KV heads: 60 items) takes 512 us unsplit and 274 in the 7 parts chosen here. Every
+// sequence is priced at max_context_len, all that the host knows: beside one long context the rows
+// of short ones are joined too, from the single part that each has.
 PrefillSplit plan_prefill_split(int num_seqs, int num_heads, int num_kv_heads, int total_q, int max_context_len) {
   const int chunk = 2 * (128 / (num_heads / num_kv_heads)), sms = sm_count();
   const int64_t items =

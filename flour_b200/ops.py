@@ -167,18 +167,18 @@ def _capturing(cuda: bool) -> bool:
 class Workspace:
     """Caller-owned, zero-initialised scratch for the split-K partials (grown on demand).
     One Workspace per stream: concurrent calls must not share it, and calls on several streams
-    are the caller's to order (its zero-fill and its freeing are ordered here). The 8-bit entry points (kv8)
-    keep a Workspace of their own, apart from the others'. A CUDA graph holds the address of the
-    buffer that its calls were captured with: keep the Workspace as long as such graphs. A buffer
-    that it outgrows stays allocated if a captured call used it. Grow it before a capture (by an
-    eager call, or `get`): a captured call that finds it too small takes memory of the graph's
-    own, which every replay has to clear."""
+    are the caller's to order (its zero-fill and its freeing are ordered here). The 8-bit entry
+    points (kv8) keep a Workspace of their own, apart from the others'. A CUDA graph holds the
+    address of the buffer that its calls were captured with: keep the Workspace as long as such
+    graphs. A buffer that it outgrows stays allocated if a captured call used it. Grow it before
+    a capture (by an eager call, or `get`): a captured call that finds it too small takes memory
+    of the graph's own, which every replay has to clear."""
 
     def __init__(self, device=None):
         self.device = torch.device(device if device is not None else "cuda")
         self.cuda = self.device.type == "cuda"
         self.buf: torch.Tensor | None = None
-        self.size, self.index = 0, -1  # of buf: bytes, CUDA device
+        self.index = -1  # the CUDA device of buf
         self.kv8: bool | None = None  # which entry points use it, from the first call that needs it
         self.captured = False         # a graph may hold the address of buf
         self.kept: list[torch.Tensor] = []  # outgrown buffers whose address a graph may hold
@@ -198,7 +198,7 @@ class Workspace:
         if nbytes == 0:
             return self.buf
         capturing = _capturing(self.cuda)
-        if self.size >= nbytes:
+        if self.buf is not None and self.buf.numel() >= nbytes:
             if capturing:  # begins behind the fill
                 self.captured = True
             elif self.filled is not None and torch._C._cuda_getCurrentRawStream(self.index) not in self.streams:
@@ -219,7 +219,6 @@ class Workspace:
             self.kept.append(self.buf)
             self.captured = False
         self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
-        self.size = nbytes
         # A fresh zero-filled buffer: bookkeeping kept for an earlier buffer at the same
         # address (the caching allocator reuses addresses) no longer applies.
         check(lib().fa_workspace_reset(_ptr(self.buf)), "workspace_reset")

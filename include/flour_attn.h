@@ -378,7 +378,9 @@ FA_API fa_status fa_paged_decode_kv8(const fa_kv8_layer *layer, const void *quer
  * and not written. Output rows behind cu_seqlens_q[num_seqs] are not written. The copy holds
  * f16's range for FA_F16 queries: magnitudes above 65504 become 65504, and below 2^-14 they are
  * rounded to steps of 2^-24 (the decode takes any f32 value of byte * scale); outputs saturate as
- * there. A NaN among the keys and values of a sequence may reach all of its queries. */
+ * there. As in fa_paged_prefill, that path rounds probabilities to the query type (bf16: half a step
+ * is 2^-8 of each, where the decode's f16 has 2^-11); the generic kernel keeps them in f32. A NaN
+ * among the keys and values of a sequence may reach all of its queries. */
 FA_API size_t fa_paged_prefill_kv8_workspace_size(int32_t dtype, int32_t num_seqs, int32_t num_heads,
                                                   int32_t num_kv_heads, int32_t block_size,
                                                   int32_t head_dim, int32_t total_q,
@@ -474,7 +476,8 @@ FA_API fa_status fa_last_token_logits(const void *hidden, const int32_t *cu_seql
  * A logit of -inf is a token that a mask took out: probability 0, log probability -inf, never
  * among the alternatives; missing alternatives are id -1 with -inf. A row of nothing else gives
  * -inf for any token, entropy 0 and no alternatives. A NaN or +inf logit makes the row's results
- * NaN, its ids -1. A token id outside [-1, vocab) gives NaN and FA_DEVERR_TOKEN. Sums in f32.
+ * NaN, its ids -1. A token id outside [-1, vocab) gives NaN and FA_DEVERR_TOKEN. Sums in f32: a
+ * log probability next to 0 is within about 2^-20 of its value.
  * Results do not depend on the other rows of the call, other than through how many CTAs share a
  * row (the order of the f32 sums). No workspace. */
 #define FA_MAX_TOP_LOGPROBS 32
