@@ -770,7 +770,7 @@ def test_an_explicit_stream_is_in_order_with_itself(device):
             del junk
     torch.cuda.synchronize()
     done = torch.cuda.Event()
-    torch.cuda._sleep(400_000_000)  # 0.2 s
+    torch.cuda._sleep(1_000_000_000)  # 0.5 s
     early = ops.Workspace()
     early.get(64 << 20)  # filled behind the sleep
     done.record()

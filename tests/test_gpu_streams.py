@@ -54,7 +54,7 @@ def test_attention_and_projections_on_a_stream_of_their_own(device):
             del junk
     torch.cuda.synchronize()
     done = torch.cuda.Event()
-    torch.cuda._sleep(400_000_000)  # 0.2 s
+    torch.cuda._sleep(1_000_000_000)  # 0.5 s
     done.record()
     ws = ops.Workspace(device)
     got = step(ws, q, pq, stream=side) + step(ws, q, pq, stream=side)
