@@ -14,8 +14,8 @@
 // 16-bit cache leave half the time to hide them in. Measured: 64 contexts of U[512, 4096], 8 KV
 // heads of 128, 60.4 us (4.95 TB/s; 63.3 with the 16-bit decode's grid of splits and this inner
 // loop); 59 of U[1, 6438], 4 KV heads, 7 query heads each, int8, 52.0 us (61.1); 16 of U[16384,
-// 32768] 148 us (5.77 TB/s of the 6.56 that a copy reaches). With a loud page's probabilities at 2^12
-// too: 61.4, 52.9 and 149.6 where the build before took 61.7, 52.6 and 149.9 in turn.
+// 32768] 148 us (5.77 TB/s of the 6.56 that a copy reaches). Loud pages' probabilities at 2^12 (below)
+// cost these nothing that shows: 61.4, 52.9 and 149.6, in turn with 61.7, 52.6 and 149.9 without.
 // A (sequence, KV head) that ends inside one range is written by its warp; the others leave pieces
 // (O / l, log2-sum-exp) in the workspace, which the CTA joins when its warps are done, and the last
 // CTA of a (sequence, KV head) to finish (a ticket, no waiting) joins the CTAs' pieces. The ranges
